@@ -245,9 +245,10 @@ def _plain_ce(d, c):
     at = (H * W[tt]).sum(dim=1)
     if d["bias"] is not None:
         at = at + d["bias"][tt]
+    # a row without a known item takes no part: its outputs are zeros
     loss = torch.where(known, lse - at, torch.zeros_like(lse))
     if not c["grad"]:
-        return loss, lse
+        return loss, torch.where(known, lse, torch.zeros_like(lse))
     g = torch.where(known, d["weight"], torch.zeros_like(lse))
     dH = torch.zeros_like(H)
     dW, db = [], []
@@ -260,6 +261,7 @@ def _plain_ce(d, c):
         dW.append(p.t() @ H)
         db.append(p.sum(dim=0))
     t = DTYPE[c["type"]]
+    lse = torch.where(known, lse, torch.zeros_like(lse))
     return loss, lse, dH.to(t), torch.cat(dW).to(t), torch.cat(db)
 
 
@@ -330,8 +332,8 @@ def _exact_ce(c, d):
         ok = (y >= 0) & (y < v)
         z = h @ Wd.T + bias
         full = torch.logsumexp(z, dim=1)
-        lse[r:r + rows] = full
         idx = torch.nonzero(ok).flatten()
+        lse[r + idx] = full[idx]
         loss[r + idx] = full[idx] - z[idx, y[idx]]
         if c["grad"]:
             z.sub_(full[:, None]).exp_()
