@@ -25,7 +25,10 @@ ARCH = "gfx950"
 # fast kernels opt back in locally with `#pragma clang fp contract(fast)`.
 # -fno-slp-vectorize: hipcc's SLP pass packs independent f32 FMAs into v_pk_* plus v_mov
 # shuffles, which costs issue slots on the latency chain of the SGD kernels.
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 at all (the results are the same: each half is the scalar
+# operation).  hipcc's host pass warns that it does not know the feature.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-slp-vectorize",
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           f"--offload-arch={ARCH}",
           "-Wall", "-Wno-unused-result", f"-I{INCLUDE}", f"-I{CSRC}"]
 
