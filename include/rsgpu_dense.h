@@ -1,0 +1,59 @@
+/*
+ * rsgpu_dense.h -- C-ABI of librsgpu's dense operators over factor tables (device pointers).  Contexts, status codes
+ * and errors are rsgpu.h's.
+ *
+ * Not functions of the reference: what a model with the factor tables P, Q above needs to be trained for ranking
+ * over the whole catalogue and to answer with the whole catalogue.
+ *
+ * All matrices are row-major device memory of ctx's device with a row stride (ld, in elements) of at least their
+ * columns; element types RS_TYPE_*.  A call enqueues its kernels on `stream` (NULL: the ctx stream,
+ * RS_STREAM_DEFAULT: the device's default stream) and returns without waiting: it synchronises nothing, allocates nothing, keeps nothing, and may be captured into a graph.
+ * `ws` is device scratch of at least the bytes that the operator's _workspace call gives (16-byte aligned); it is
+ * free for other use once the call's kernels have run, and two calls that may overlap need a workspace each.  The
+ * caller's current device is put back before a call returns.  Calls whose sizes leave nothing to do return RS_OK
+ * without a launch.  Sums are held in fp32, int32 or fp64 and each output is rounded once; results do not depend on timing (no
+ * floating-point atomics).  n_factors up to RS_DENSE_MAX_FACTORS. */
+#ifndef RSGPU_DENSE_H
+#define RSGPU_DENSE_H
+
+#include "rsgpu.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define RS_TYPE_F32 0
+#define RS_TYPE_BF16 1
+#define RS_TYPE_F16 2
+#define RS_DENSE_MAX_FACTORS 512
+/* `stream` value of the device's default (null) stream, which NULL does not name here */
+#define RS_STREAM_DEFAULT ((void*)1)
+
+/* Softmax cross entropy of every row of H (n_rows x n_factors: users' vectors) against the whole catalogue W
+ * (n_items x n_factors), without keeping the logits:
+ *   l_nv = h_n . w_v + bias_v      lse_n = log sum_v exp(l_nv)      loss_n = lse_n - l_{n, target_n}
+ * and, where dH, dW and dbias are given (all three or none), the gradient of sum_n weight_n loss_n:
+ *   c_nv = weight_n (exp(l_nv - lse_n) - [v = target_n])   dH_n = sum_v c_nv w_v   dW_v = sum_n c_nv h_n   dbias_v = sum_n c_nv
+ * H, W, dH, dW have the element type `type`; bias, weight, loss, lse and dbias are fp32; target int32.
+ *   bias NULL: zeros.  bias_v = -inf withdraws item v: it takes no part in any row, whatever its row of W holds (NaN
+ *     included), and its rows of dW and dbias are zero.
+ *   weight NULL: ones.  It is read for gradients only.
+ *   target outside [0, n_items) (-1: unknown): the row takes no part, whatever its row of H and its weight hold;
+ *     loss, lse and its row of dH are zero.
+ *   Every item withdrawn: lse -inf, loss 0, no gradient.  target withdrawn, others not: lse as defined, loss +inf,
+ *     no gradient from that row.
+ * RS_TYPE_F32 products run on fp16 pairs (hi + lo, scaled by a power of two from the largest finite element of
+ * each matrix): an element keeps 2^-24 of itself or 2^-39 of the matrix's largest element, whichever is more.
+ * n_items < 2^31, n_rows < 2^31. */
+int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
+                            int64_t* bytes);
+int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, const void* H, int64_t ldh,
+                  const void* W, int64_t ldw, const float* bias, const int32_t* target, const float* weight,
+                  float* loss, float* lse, void* dH, int64_t lddh, void* dW, int64_t lddw, float* dbias,
+                  void* ws, int64_t ws_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* RSGPU_DENSE_H */

@@ -1,0 +1,117 @@
+// dense.hpp -- what the dense operators over factor tables share (softmax_ce.hip, int8.hip, ortho.hip): element
+// types and their roundings, MFMA operand types, the device scope and the checks of device matrices.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "common.hpp"
+#include "rsgpu_dense.h"
+
+namespace rs {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) double f64x4;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(16))) int i32x16;
+
+// Element types: RS_TYPE_F32 / _BF16 / _F16 as C++ types.  Conversions from float round to nearest, ties to even.
+template <int TYPE>
+struct Elem;
+template <>
+struct Elem<RS_TYPE_F32> { using type = float; };
+template <>
+struct Elem<RS_TYPE_BF16> { using type = __bf16; };
+template <>
+struct Elem<RS_TYPE_F16> { using type = _Float16; };
+
+inline int64_t type_size(int32_t type) { return type == RS_TYPE_F32 ? 4 : 2; }
+inline bool type_ok(int32_t type) { return type == RS_TYPE_F32 || type == RS_TYPE_BF16 || type == RS_TYPE_F16; }
+
+// f(Elem<...>) for the runtime type (checked by type_ok before)
+template <typename F>
+void with_type(int32_t type, F&& f) {
+    if (type == RS_TYPE_F32)
+        f(Elem<RS_TYPE_F32>{});
+    else if (type == RS_TYPE_BF16)
+        f(Elem<RS_TYPE_BF16>{});
+    else
+        f(Elem<RS_TYPE_F16>{});
+}
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// The caller's current device is put back when an operator returns (its tensors may live on another device than the
+// one that is current in the calling thread).
+struct DeviceScope {
+    int prev = -1;
+    explicit DeviceScope(int device) {
+        RS_HIP(hipGetDevice(&prev));
+        if (prev != device)
+            RS_HIP(hipSetDevice(device));
+        else
+            prev = -1;
+    }
+    ~DeviceScope() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
+// Operator entry points: the device scope, and exceptions turned into status codes.
+template <typename F>
+int dense_guard(rs_ctx* ctx, F&& body) {
+    if (!ctx) return set_error(nullptr, RS_ERR_INVALID, "ctx is NULL");
+    try {
+        DeviceScope scope(ctx->device);
+        return body();
+    } catch (const HipError& e) {
+        return set_error(ctx, e.code == hipErrorOutOfMemory ? RS_ERR_NOMEM : RS_ERR_HIP, e.what);
+    } catch (const std::bad_alloc&) {
+        return set_error(ctx, RS_ERR_NOMEM, "host allocation failed");
+    } catch (const std::exception& e) {
+        return set_error(ctx, RS_ERR_INVALID, e.what());
+    }
+}
+
+// NULL: the ctx stream (as everywhere in the C-ABI); RS_STREAM_DEFAULT: the device's null stream
+inline hipStream_t pick_stream(rs_ctx* ctx, void* stream) {
+    if (stream == RS_STREAM_DEFAULT) return nullptr;
+    return stream ? static_cast<hipStream_t>(stream) : ctx->stream;
+}
+
+// A device matrix argument: non-null, aligned to its element, its row stride at least its columns.  Returns the
+// complaint, or an empty string.
+inline std::string check_matrix(const char* name, const void* p, int64_t cols, int64_t ld, int64_t elem) {
+    if (!p) return std::string(name) + " is NULL";
+    if (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(elem))
+        return std::string(name) + " is not aligned to its element type";
+    if (ld < cols) return std::string(name) + ": row stride below its columns";
+    return std::string();
+}
+
+// maximum over the wave (64 lanes)
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const uint32_t w = __shfl_xor(v, o);
+        v = v > w ? v : w;
+    }
+    return v;
+}
+__device__ __forceinline__ float wave_sum_f32(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+}  // namespace rs

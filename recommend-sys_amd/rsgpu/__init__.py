@@ -12,7 +12,8 @@ import weakref
 
 import numpy as np
 
-from . import _build
+from . import _build, dense
+from .dense import DENSE_MAX_FACTORS, TYPE_BF16, TYPE_F16, TYPE_F32  # noqa: F401
 
 LIB_PATH = _build.LIB
 _lib = None
@@ -54,7 +55,7 @@ HEADER_SYMBOLS = (
     "rs_comm_info", "rs_rotation_step", "rs_svd_plan_shard_info", "rs_svd_plan_qdelta_info", "rs_svd_plan_inject_fault",
     "rs_svd_plan_time_blocks", "rs_knn_plan_set_tie_order", "rs_fit_refits", "rs_open_r",
     "rs_svd_plan_set_hot_split",
-)
+) + tuple(dense.SIGNATURES)
 COMM_ID_BYTES = 128
 
 
@@ -201,6 +202,7 @@ def lib():
                                                  C.POINTER(_i32)]),
             "rs_svd_plan_qdelta_info": (C.c_int, [_vp, C.POINTER(_i32), C.POINTER(_i32)]),
         }
+        sig.update(dense.SIGNATURES)
         for name, (res, args) in sig.items():
             f = getattr(L, name)
             f.restype = res
@@ -309,8 +311,8 @@ class Ratings:
                         _ptr(self.items), _ptr(self.ratings))
 
 
-class Context:
-    """One HIP stream on one gfx950 device (rs_open / rs_close)."""
+class Context(dense.DenseOps):
+    """One HIP stream on one gfx950 device (rs_open / rs_close), and the dense operators on torch tensors (dense.py)."""
 
     def __init__(self, device: int = 0):
         h = C.c_void_p()

@@ -1,0 +1,106 @@
+"""Dense operators over factor tables, on torch tensors in device memory (rs_softmax_ce, rs_quantize_rows,
+rs_i8_matmul, rs_orthogonalize of include/rsgpu_dense.h).  They are methods of Context.
+
+Each call enqueues its kernels on torch's current stream of the tensors' device and returns at once: nothing is
+synchronised, and a call may be captured into a graph.  Outputs and workspaces are new torch tensors.  Tensors live
+on the context's device, matrices have contiguous rows (any row stride).  The operators return gradients
+themselves; they are not recorded by autograd.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+DENSE_MAX_FACTORS = 512
+STREAM_DEFAULT = 1  # RS_STREAM_DEFAULT: torch's default stream (0 would name the context's own)
+
+_vp, _i32, _i64, _dbl = C.c_void_p, C.c_int32, C.c_int64, C.c_double
+
+SIGNATURES = {
+    "rs_softmax_ce_workspace": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, C.POINTER(_i64)]),
+    "rs_softmax_ce": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+}
+
+
+def _types():
+    import torch
+    return {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+
+
+def _type(t, name):
+    ty = _types().get(t.dtype)
+    if ty is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    return ty
+
+
+class DenseOps:
+    """The device-tensor operators of a Context."""
+
+    def _mat(self, t, name, shape=None, dtype=None):
+        """Checks a 2-D device tensor; returns its row stride in elements."""
+        if t.dim() != 2:
+            raise ValueError(f"{name} must have two dimensions")
+        self._on_device(t, name, dtype)
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{name} must have contiguous rows (stride 1 along the columns)")
+        return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+    def _vec(self, t, name, n, dtype):
+        """Checks a contiguous 1-D device tensor (None passes); returns its pointer."""
+        if t is None:
+            return None
+        if t.dim() != 1 or t.shape[0] != n:
+            raise ValueError(f"{name} must have {n} values, not {tuple(t.shape)}")
+        self._on_device(t, name, dtype)
+        if n > 1 and t.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr()
+
+    def _on_device(self, t, name, dtype):
+        if t.device.type != "cuda" or t.device.index != self.device:
+            raise ValueError(f"{name} is on {t.device}, the context on cuda:{self.device}")
+        if dtype is not None and t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+
+    def _dense(self, name, *args):
+        from . import lib
+        self.check(getattr(lib(), name)(self.h, *args))
+
+    def _stream(self, t):
+        import torch
+        return torch.cuda.current_stream(t.device).cuda_stream or STREAM_DEFAULT
+
+    def softmax_ce(self, H, W, target, bias=None, weight=None, grad=False):
+        """Softmax cross entropy of every row of H (n x k) against the catalogue W (items x k), the logits
+        H W^T + bias never kept (rs_softmax_ce).  target: int32 item ids, -1 (or any id outside the catalogue):
+        the row takes no part.  bias: fp32, -inf withdraws an item.  Returns (loss, lse) of every row, and with
+        grad=True also (dH, dW, dbias), the gradient of sum(weight * loss) (weight None: ones)."""
+        import torch
+        ty = _type(H, "H")
+        ldh, ldw = self._mat(H, "H"), self._mat(W, "W", dtype=H.dtype)
+        (n, k), items = H.shape, W.shape[0]
+        if W.shape[1] != k:
+            raise ValueError(f"H has {k} columns, W {W.shape[1]}")
+        pt = self._vec(target, "target", n, torch.int32)
+        pb = self._vec(bias, "bias", items, torch.float32)
+        pw = self._vec(weight, "weight", n, torch.float32)
+        if n == 0 or items == 0:
+            raise ValueError("softmax_ce needs at least one row and one item")
+        need = _i64(0)
+        self._dense("rs_softmax_ce_workspace", ty, n, items, k, int(bool(grad)), C.byref(need))
+        dev = H.device
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        loss, lse = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
+        dH = dW = db = None
+        if grad:
+            dH = torch.empty(n, k, dtype=H.dtype, device=dev)
+            dW = torch.empty(items, k, dtype=H.dtype, device=dev)
+            db = torch.empty(items, dtype=torch.float32, device=dev)
+        ptr = lambda t: None if t is None else t.data_ptr()
+        self._dense("rs_softmax_ce", ty, n, items, k, H.data_ptr(), ldh, W.data_ptr(), ldw, pb, pt, pw, loss.data_ptr(),
+                    lse.data_ptr(), ptr(dH), k, ptr(dW), k, ptr(db), ws.data_ptr(), need.value, self._stream(H))
+        return (loss, lse, dH, dW, db) if grad else (loss, lse)
