@@ -52,6 +52,24 @@ int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, in
                   float* loss, float* lse, void* dH, int64_t lddh, void* dW, int64_t lddw, float* dbias,
                   void* ws, int64_t ws_bytes, void* stream);
 
+/* Rows in 8 bits with a scale each: scale_r = max_c |x_rc| / 127 (rounded to fp32), q_rc = x_rc / scale_r to the
+ * nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of zeros has scale 0 and q 0; a
+ * row with an infinity or NaN has scale NaN and q 0 (so that all its products are NaN), as has a row whose scale
+ * underflows to 0, but with scale 0.  X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as
+ * they are.  n_cols >= 1. */
+int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_cols, const void* X, int64_t ldx, int8_t* q,
+                     int64_t ldq, float* scale, void* stream);
+
+/* int8 product with a scale per row of A (a user, a token) and per row of B (an item, a channel):
+ *   C_mn = a_scale_m * b_scale_n * sum_k A_mk B_nk + row_bias_m + col_bias_n
+ * A (m x k), B (n x k) int8, any value, any alignment and stride (rows of 16-byte multiples at 16-byte addresses are
+ * read fastest); the sums are exact in int32 (k <= RS_I8_MAX_K); the rest is fp32, C of out_type rounded once.
+ * row_bias, col_bias may be NULL.  An entry of col_bias of -inf gives -inf scores (a withdrawn item).  k >= 1. */
+#define RS_I8_MAX_K 65536
+int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, int64_t lda, const float* a_scale,
+                 const int8_t* B, int64_t ldb, const float* b_scale, const float* row_bias, const float* col_bias,
+                 int32_t out_type, void* C, int64_t ldc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

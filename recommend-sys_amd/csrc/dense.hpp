@@ -46,8 +46,8 @@ void with_type(int32_t type, F&& f) {
         f(Elem<RS_TYPE_F16>{});
 }
 
-inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+__host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 
 // The caller's current device is put back when an operator returns (its tensors may live on another device than the
 // one that is current in the calling thread).

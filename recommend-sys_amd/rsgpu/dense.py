@@ -20,6 +20,8 @@ SIGNATURES = {
     "rs_softmax_ce_workspace": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, C.POINTER(_i64)]),
     "rs_softmax_ce": (C.c_int, [_vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
                                 _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
+    "rs_quantize_rows": (C.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "rs_i8_matmul": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
 }
 
 
@@ -104,3 +106,36 @@ class DenseOps:
         self._dense("rs_softmax_ce", ty, n, items, k, H.data_ptr(), ldh, W.data_ptr(), ldw, pb, pt, pw, loss.data_ptr(),
                     lse.data_ptr(), ptr(dH), k, ptr(dW), k, ptr(db), ws.data_ptr(), need.value, self._stream(H))
         return (loss, lse, dH, dW, db) if grad else (loss, lse)
+
+    def quantize_rows(self, X):
+        """The rows of X in 8 bits with a scale each (rs_quantize_rows): (q int8, scale fp32), x ~ scale * q with
+        scale = max |x| / 127 of the row.  q's rows are 16-byte multiples apart, as i8_matmul reads them fastest."""
+        import torch
+        ty = _type(X, "X")
+        ldx = self._mat(X, "X")
+        m, k = X.shape
+        if k == 0:
+            raise ValueError("X has no columns")
+        q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=X.device)[:, :k]
+        scale = torch.empty(m, dtype=torch.float32, device=X.device)
+        self._dense("rs_quantize_rows", ty, m, k, X.data_ptr(), ldx, q.data_ptr(), (k + 15) // 16 * 16, scale.data_ptr(), self._stream(X))
+        return q, scale
+
+    def i8_matmul(self, A, a_scale, B, b_scale, row_bias=None, col_bias=None, out_dtype=None):
+        """C = (A B^T) * a_scale[:, None] * b_scale + row_bias[:, None] + col_bias for int8 A (m x k) and B (n x k)
+        with a scale per row (rs_i8_matmul); C of out_dtype (float32 by default), m x n."""
+        import torch
+        out_dtype = torch.float32 if out_dtype is None else out_dtype
+        ty = _types().get(out_dtype)
+        if ty is None:
+            raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+        lda, ldb = self._mat(A, "A", dtype=torch.int8), self._mat(B, "B", dtype=torch.int8)
+        (m, k), n = A.shape, B.shape[0]
+        if B.shape[1] != k or k == 0:
+            raise ValueError(f"A has {k} columns, B {B.shape[1]}")
+        pa, pb = self._vec(a_scale, "a_scale", m, torch.float32), self._vec(b_scale, "b_scale", n, torch.float32)
+        pr, pc = self._vec(row_bias, "row_bias", m, torch.float32), self._vec(col_bias, "col_bias", n, torch.float32)
+        out = torch.empty(m, n, dtype=out_dtype, device=A.device)
+        self._dense("rs_i8_matmul", m, n, k, A.data_ptr(), lda, pa, B.data_ptr(), ldb, pb, pr, pc, ty, out.data_ptr(), max(n, 1),
+                    self._stream(A))
+        return out
