@@ -22,6 +22,8 @@ SIGNATURES = {
                                 _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp]),
     "rs_quantize_rows": (C.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
     "rs_i8_matmul": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
+    "rs_orthogonalize_workspace": (C.c_int, [_vp, _i64, _i64, C.POINTER(_i64)]),
+    "rs_orthogonalize": (C.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _i32, _dbl, _dbl, _dbl, _vp, _i64, _vp, _i64, _vp]),
 }
 
 
@@ -139,3 +141,23 @@ class DenseOps:
         self._dense("rs_i8_matmul", m, n, k, A.data_ptr(), lda, pa, B.data_ptr(), ldb, pb, pr, pc, ty, out.data_ptr(), max(n, 1),
                     self._stream(A))
         return out
+
+    def orthogonalize(self, G, steps=5, coef=(3.4445, -4.7750, 2.0315), out=None):
+        """The orthogonalised form of the update G of a factor table by Newton-Schulz products (rs_orthogonalize): G / |G|
+        with every singular value s taken `steps` times through a s + b s^3 + c s^5.  out: where to write it (it may be
+        G itself)."""
+        import torch
+        ty = _type(G, "G")
+        ldg = self._mat(G, "G")
+        rows, cols = G.shape
+        if rows == 0 or cols == 0:
+            raise ValueError("G is empty")
+        X = torch.empty(rows, cols, dtype=G.dtype, device=G.device) if out is None else out
+        ldx = self._mat(X, "out", shape=G.shape, dtype=G.dtype)
+        a, b, c = (float(v) for v in coef)
+        need = _i64(0)
+        self._dense("rs_orthogonalize_workspace", rows, cols, C.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=G.device)
+        self._dense("rs_orthogonalize", ty, rows, cols, G.data_ptr(), ldg, int(steps), a, b, c, X.data_ptr(), ldx, ws.data_ptr(), need.value,
+                    self._stream(G))
+        return X

@@ -1,0 +1,206 @@
+"""Orthogonalised updates (rs_orthogonalize): refusals on the CPU, values against the steps in 64 bits on the GPU.
+
+X = G T / |G| with T the product of the steps' polynomials on the short side, formed in fp64 and rounded to fp32 (u32 of
+each entry), the table's rows times T summed in fp32 over the short side S, then 1 / |G| (two roundings): an element is
+off by at most (S + 4) u32 (|G| |T| / |G|_F) and half a step of its type; T's own fp64 error is below 1e-9 of its
+largest entry for the singular values used here.
+"""
+import ctypes as C
+import math
+
+import pytest
+
+import rsgpu
+
+torch = pytest.importorskip("torch")
+
+T = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U32 = 2.0 ** -24
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def reference(G, steps=5, coef=COEF):
+    """(X, bound): the steps in 64 bits, and |G| |T| / |G|_F."""
+    G = G.double().cpu()
+    norm = torch.linalg.vector_norm(G)
+    if norm == 0:
+        return torch.zeros_like(G), torch.zeros_like(G)
+    a, b, c = coef
+    flip = G.shape[0] < G.shape[1]
+    Y = (G.T if flip else G) / norm
+    Y0 = Y
+    for _ in range(steps):
+        A = Y.T @ Y
+        Y = a * Y + Y @ (b * A + c * (A @ A))
+    w, V = torch.linalg.eigh(Y0.T @ Y0)
+    s = w.clamp(min=0).sqrt()
+    amp = torch.ones_like(s)
+    for _ in range(steps):
+        p = a + b * s ** 2 + c * s ** 4
+        amp, s = amp * p, s * p
+    Tm = V @ torch.diag(amp) @ V.T
+    bound = Y0.abs() @ (Tm.abs() + 1e-9 * 2 ** 24 * Tm.abs().max() / (Y0.shape[1] + 4))
+    return (Y.T, bound.T) if flip else (Y, bound)
+
+
+def check(X, G, steps=5, coef=COEF):
+    ref, bound = reference(G, steps, coef)
+    S = min(G.shape)
+    ut = torch.finfo(X.dtype).eps / 2
+    tiny = torch.finfo(X.dtype).smallest_normal * torch.finfo(X.dtype).eps
+    err = (X.double().cpu() - ref).abs()
+    lim = (S + 4) * U32 * bound * (1 + ut) + ut * ref.abs() + tiny
+    assert (err <= lim).all(), (float((err - lim).max()), float((err / lim.clamp(min=1e-300)).max()))
+
+
+def update(rows, cols, ty, seed=0, scale=1e-2):
+    g = torch.Generator().manual_seed(seed)
+    r = min(4, rows, cols)
+    G = torch.randn(rows, r, generator=g) @ torch.randn(r, cols, generator=g) + torch.randn(rows, cols, generator=g)
+    G *= 0.2 + torch.rand(cols, generator=g)
+    return (G * scale).to(T[ty]).cuda()
+
+
+SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (33, 20), (20, 33), (64, 64), (130, 65), (1682, 20), (100, 600), (700, 129), (257, 256),
+          (300, 511), (2000, 512)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_values(ctx, rows, cols, ty):
+    G = update(rows, cols, ty, seed=rows + cols)
+    keep = G.clone()
+    check(ctx.orthogonalize(G), G)
+    assert torch.equal(G, keep)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 9])
+def test_steps_and_coefficients(ctx, steps):
+    G = update(200, 40, "f32", seed=steps)
+    coef = (1.5, -0.5, 0.0)
+    check(ctx.orthogonalize(G, steps=steps, coef=coef), G, steps, coef)
+    if steps < 5:
+        check(ctx.orthogonalize(G, steps=steps), G, steps)
+
+
+@pytest.mark.gpu
+def test_cubic_steps_end_in_an_orthogonal_matrix(ctx):
+    """(1.5, -0.5, 0) converges: X^T X = 1 within the rounding of its fp32 entries (S u32 and the chain's own)."""
+    G = update(500, 24, "f32", seed=3)
+    X = ctx.orthogonalize(G, steps=16, coef=(1.5, -0.5, 0.0)).double()
+    assert float((X.T @ X - torch.eye(24, device="cuda", dtype=torch.float64)).abs().max()) < 1e-4
+
+
+@pytest.mark.gpu
+def test_degenerate(ctx):
+    Z = torch.zeros(50, 10, device="cuda")
+    assert (ctx.orthogonalize(Z) == 0).all()
+    one = torch.zeros(90, 30, device="cuda")
+    one[17, 5] = -1e-20
+    check(ctx.orthogonalize(one), one)
+    same = torch.ones(60, 12, device="cuda") * 1e15  # rank one
+    check(ctx.orthogonalize(same), same)
+    G = update(80, 16, "f32", seed=5)
+    G[3, 4] = math.nan
+    assert torch.isnan(ctx.orthogonalize(G)).all()
+    G[3, 4] = math.inf
+    assert not torch.isfinite(ctx.orthogonalize(G)).any()
+
+
+@pytest.mark.gpu
+def test_spread_of_singular_values(ctx):
+    """Directions 1000 times weaker than the strongest are amplified by up to a^5 = 485: inside the bound by T."""
+    g = torch.Generator().manual_seed(6)
+    U, _ = torch.linalg.qr(torch.randn(400, 50, generator=g, dtype=torch.float64))
+    V, _ = torch.linalg.qr(torch.randn(50, 50, generator=g, dtype=torch.float64))
+    G = (U @ torch.diag(torch.logspace(0, -3, 50, dtype=torch.float64)) @ V.T).float().cuda()
+    check(ctx.orthogonalize(G), G)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(300, 70), (70, 300)])
+def test_strided_in_place_and_beside(ctx, rows, cols):
+    G = update(rows, cols, "f32", seed=8)
+    want = ctx.orthogonalize(G)
+    big = torch.full((rows, cols + 11), 3.0, device="cuda")
+    big[:, 5:5 + cols] = G
+    assert torch.equal(ctx.orthogonalize(big[:, 5:5 + cols]), want)
+    ctx.orthogonalize(big[:, 5:5 + cols], out=big[:, 5:5 + cols])
+    assert torch.equal(big[:, 5:5 + cols], want)
+    big[:, 5:5 + cols] = 3.0
+    assert (big == 3.0).all()
+
+
+@pytest.mark.gpu
+def test_transposed_update(ctx):
+    """A tall update and its transpose are the same operator: equal up to the order of the sums."""
+    G = update(500, 90, "f32", seed=9)
+    check(ctx.orthogonalize(G), G)
+    check(ctx.orthogonalize(G.T.contiguous()).T, G)
+
+
+@pytest.mark.gpu
+def test_side_stream_and_graph(ctx):
+    G = update(900, 100, "f32", seed=10)
+    ref = ctx.orthogonalize(G)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ctx.orthogonalize(G)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, ref)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ctx.orthogonalize(G)
+        both = ctx.orthogonalize(G, steps=2)
+    for i in range(3):
+        G[i] *= 3.0
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ctx.orthogonalize(G)) and torch.equal(both, ctx.orthogonalize(G, steps=2))
+
+
+@pytest.mark.gpu
+def test_tensor_refusals(ctx):
+    G = update(30, 8, "f32")
+    with pytest.raises(ValueError):
+        ctx.orthogonalize(G.cpu())
+    with pytest.raises(TypeError):
+        ctx.orthogonalize(G.double())
+    with pytest.raises(ValueError):
+        ctx.orthogonalize(G[:, ::2])
+    with pytest.raises(ValueError):
+        ctx.orthogonalize(G, out=G[:20])
+    with pytest.raises(ValueError):
+        ctx.orthogonalize(G[:0])
+    for kw in (dict(steps=0), dict(steps=17), dict(coef=(math.nan, 0, 0))):
+        with pytest.raises(rsgpu.RsError):
+            ctx.orthogonalize(G, **kw)
+    with pytest.raises(rsgpu.RsError) as e:
+        ctx.orthogonalize(torch.zeros(513, 513, device="cuda"))
+    assert e.value.code == rsgpu.RS_ERR_UNSUPPORTED
+
+
+def test_entry_point_refusals():
+    L = rsgpu.lib()
+    need = C.c_int64(-1)
+    assert L.rs_orthogonalize_workspace(None, 100, 20, C.byref(need)) == rsgpu.RS_OK and need.value > 0
+    assert L.rs_orthogonalize_workspace(None, 100, 20, None) == rsgpu.RS_ERR_INVALID
+    assert L.rs_orthogonalize_workspace(None, -1, 20, C.byref(need)) == rsgpu.RS_ERR_INVALID
+    assert L.rs_orthogonalize_workspace(None, 513, 513, C.byref(need)) == rsgpu.RS_ERR_UNSUPPORTED
+    assert L.rs_orthogonalize_workspace(None, 0, 20, C.byref(need)) == rsgpu.RS_OK and need.value == 0
+    buf = C.create_string_buffer(1 << 12)
+    p = (C.addressof(buf) + 255) & ~255
+    good = dict(ty=0, r=4, c=3, G=p, ldg=3, steps=5, a=1.5, b=-0.5, cc=0.0, X=p, ldx=3, ws=p, n=1 << 40)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return L.rs_orthogonalize(None, a["ty"], a["r"], a["c"], a["G"], a["ldg"], a["steps"], a["a"], a["b"], a["cc"], a["X"], a["ldx"], a["ws"], a["n"], None)
+    for kw in (dict(), dict(ty=5), dict(r=-1), dict(G=None), dict(G=p + 2), dict(ldg=2), dict(steps=0), dict(steps=17), dict(a=math.inf),
+               dict(X=None), dict(ldx=2), dict(ldx=4), dict(ws=None), dict(ws=p + 8), dict(n=64)):
+        assert call(**kw) == rsgpu.RS_ERR_INVALID, kw  # (the first: no context)
+    assert call(r=600, c=600, ldg=600, ldx=600) == rsgpu.RS_ERR_UNSUPPORTED
+    assert call(r=0) == rsgpu.RS_OK
