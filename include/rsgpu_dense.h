@@ -42,8 +42,9 @@ extern "C" {
  *     loss, lse and its row of dH are zero.
  *   Every item withdrawn: lse -inf, loss 0, no gradient.  target withdrawn, others not: lse as defined, loss +inf,
  *     no gradient from that row.
- * RS_TYPE_F32 products run on fp16 pairs (hi + lo, scaled by a power of two from the largest finite element of
- * each matrix): an element keeps 2^-24 of itself or 2^-39 of the matrix's largest element, whichever is more.
+ * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
+ * (hi + lo), so an element keeps 2^-24 of itself or 2^-39 of the matrix's largest element, whichever is more;
+ * RS_TYPE_BF16 exactly down to 2^-28 of the largest, and to 2^-39 of it below.
  * n_items < 2^31, n_rows < 2^31. */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);
@@ -52,8 +53,8 @@ int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, in
                   float* loss, float* lse, void* dH, int64_t lddh, void* dW, int64_t lddw, float* dbias,
                   void* ws, int64_t ws_bytes, void* stream);
 
-/* Rows in 8 bits with a scale each: scale_r = max_c |x_rc| / 127 (rounded to fp32), q_rc = x_rc / scale_r to the
- * nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of zeros has scale 0 and q 0; a
+/* Rows in 8 bits with a scale each: scale_r = max_c |x_rc| * (1/127), both factors and the product in fp32,
+ * q_rc = x_rc / scale_r to the nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of zeros has scale 0 and q 0; a
  * row with an infinity or NaN has scale NaN and q 0 (so that all its products are NaN), as has a row whose scale
  * underflows to 0, but with scale 0.  X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as
  * they are.  n_cols >= 1. */

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict_
     }
     m = wave_max_u32(m);
     const bool finite = m < 0x7F800000u;
-    const float s = finite ? __uint_as_float(m) / 127.f : __uint_as_float(0x7FC00000u);
+    const float s = finite ? __uint_as_float(m) * (1.f / 127.f) : __uint_as_float(0x7FC00000u);
     if (lane == 0) scale[r] = s;
     const bool some = finite && s > 0.f, safe = s > 7.9e-31f;
     const float inv = 1.f / s;

@@ -11,9 +11,11 @@
 // transposing LDS reads.
 //
 // Operands are packed into the workspace first: rows padded to tiles and columns to KP with zeros, withdrawn items
-// and rows without a known target zeroed (so NaN or garbage in them reaches no product), fp32 split into two fp16
-// pieces hi + lo (each rounds its rest: 2^-24 of the element is left) of the matrix scaled by a power of two.  The
-// product of two such is hi hi + hi lo + lo hi, three fp16 MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
+// and rows without a known target zeroed (so NaN or garbage in them reaches no product), as fp16 of the matrix scaled by
+// a power of two.  bf16's 8 bits fit fp16's 11: the products are those of bf16, but the coefficients f(S) keep 11 bits
+// where bf16 MFMAs would round them to 8 (dW's error then was 1.5 times that of its own rounding).  fp32 is split into
+// two pieces hi + lo (each rounds its rest: 2^-24 of the element is left); the product of two such is
+// hi hi + hi lo + lo hi, three fp16 MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -26,6 +28,7 @@ namespace {
 constexpr int kTileX = 128;      // stationary rows of a workgroup (4 waves of 32)
 constexpr int kTileY = 32;       // streamed rows of a step
 constexpr int kMaxBlocks = 256;  // blocks of the maxima pass, per matrix
+constexpr float kShift = 14.f;   // p is held as 2^14 p: fp16's range below 1 is short
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 enum Mode { kLoss = 0, kLossGrad = 1, kItems = 2 };
@@ -150,7 +153,7 @@ __device__ __forceinline__ float scale_for(uint32_t max_bits) {
 }
 
 // ---- packing -------------------------------------------------------------------------------------------------------
-template <typename E, typename T, int NP>
+template <typename E, int NP>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) {
     __shared__ uint32_t sm[3];
     if (threadIdx.x < 192) {
@@ -161,9 +164,10 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         if ((threadIdx.x & 63) == 0) sm[which] = m;
     }
     __syncthreads();
-    const float hs = NP == 2 ? scale_for(sm[0]) : 1.f, wsc = NP == 2 ? scale_for(sm[1]) : 1.f;
-    // fp16 coefficients c = weight (p - [target]), |c| <= |weight| cs < 2^14 (bf16 has fp32's range: no scale)
-    const float cs = std::is_same<T, _Float16>::value ? scale_for(a.weight ? sm[2] : 0x3F800000u) : 1.f;
+    constexpr bool kScaled = !std::is_same<E, _Float16>::value;
+    const float hs = kScaled ? scale_for(sm[0]) : 1.f, wsc = kScaled ? scale_for(sm[1]) : 1.f;
+    // coefficients c = weight (p - [target]): |c| <= |weight| cs < 2^14
+    const float cs = scale_for(a.weight ? sm[2] : 0x3F800000u);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         Scal s;
         s.hs = hs, s.wsc = wsc, s.cs = cs;
@@ -186,29 +190,22 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         }
         const E* src = static_cast<const E*>(w ? a.W : a.H) + (there ? r * (w ? a.ldw : a.ldh) : 0);
         const float sc = w ? wsc : hs;
-        u16x8 hi, lo;
+        f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float x = there && c0 + e < a.p.k ? static_cast<float>(src[c0 + e]) : 0.f;
-            const float y = NP == 2 ? x * sc : x;
-            const T h = static_cast<T>(y);
-            hi[e] = __builtin_bit_cast(unsigned short, h);
-            if (NP == 2) lo[e] = __builtin_bit_cast(unsigned short, static_cast<T>(y - static_cast<float>(h)));
+            const float y = x * sc;  // (a power of two: exact)
+            hi[e] = static_cast<_Float16>(y);
+            if (NP == 2) lo[e] = static_cast<_Float16>(y - static_cast<float>(hi[e]));
         }
-        unsigned short* dst = a.at<unsigned short>(w ? a.p.o_w : a.p.o_h) + r * a.p.kp + c0;
-        *reinterpret_cast<u16x8*>(dst) = hi;
-        if (NP == 2) *reinterpret_cast<u16x8*>(dst + (w ? a.p.v_pad : a.p.n_pad) * a.p.kp) = lo;
+        _Float16* dst = a.at<_Float16>(w ? a.p.o_w : a.p.o_h) + r * a.p.kp + c0;
+        *reinterpret_cast<f16x8*>(dst) = hi;
+        if (NP == 2) *reinterpret_cast<f16x8*>(dst + (w ? a.p.v_pad : a.p.n_pad) * a.p.kp) = lo;
     }
 }
 
 // ---- the products --------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ f32x16 mfma16(u16x8 a, u16x8 b, f32x16 c) {
-    if constexpr (std::is_same<T, _Float16>::value)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
+__device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // 16-byte chunk c of row r of an LDS tile sits at chunk c ^ (r mod 16) of the row (fewer where a row has fewer
 // chunks): the row-wise and the transposing reads both spread over the banks.
@@ -219,38 +216,37 @@ __device__ __forceinline__ int lds_chunk(int row, int c) {
 }
 
 // MODE kLoss / kLossGrad: x = users' rows, y = items; kItems: x = items, y = users' rows.
-template <typename T, int NP, int KP, int MODE>
+template <typename E, int NP, int KP, int MODE>
 __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
 #pragma clang fp contract(fast)
     constexpr int OC = KP < 256 ? KP : 256, NB = OC / 32, KS = KP / 16, C = KP / 8;
     constexpr int PIECE = kTileY * KP;                     // elements of one piece of a tile
     constexpr int CHUNKS = kTileY * C * NP, PER = (CHUNKS + 255) / 256;
     constexpr int NM = MODE == kItems ? 3 : 1;             // values per streamed row
-    constexpr float kShift = std::is_same<T, _Float16>::value ? 14.f : 0.f;  // fp16: p is held as 2^14 p
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    unsigned short* tile = reinterpret_cast<unsigned short*>(smem);          // [2][NP][kTileY][KP]
+    _Float16* tile = reinterpret_cast<_Float16*>(smem);          // [2][NP][kTileY][KP]
     float* meta = reinterpret_cast<float*>(smem + 2 * NP * PIECE * 2);       // [2][NM][kTileY]
 
     const CePlan& p = a.p;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lx = lane & 31, half = lane >> 5;
     const bool items = MODE == kItems;
     const int64_t x_pad = items ? p.v_pad : p.n_pad, y_pad = items ? p.n_pad : p.v_pad;
-    const unsigned short* X = a.at<unsigned short>(items ? p.o_w : p.o_h);
-    const unsigned short* Y = a.at<unsigned short>(items ? p.o_h : p.o_w);
+    const _Float16* X = a.at<_Float16>(items ? p.o_w : p.o_h);
+    const _Float16* Y = a.at<_Float16>(items ? p.o_h : p.o_w);
     const int per = items ? p.tiles_w : p.tiles_f;
     const int split = blockIdx.y, oc0 = blockIdx.z * OC;
     const int64_t x = static_cast<int64_t>(blockIdx.x) * kTileX + wave * 32 + lx;
     const int t0 = split * per, t1 = static_cast<int>(min<int64_t>(y_pad / kTileY, t0 + per));
     const Scal sc = *a.at<Scal>(p.o_scal);
 
-    u16x8 xf[NP][KS];
+    f16x8 xf[NP][KS];
 #pragma unroll
     for (int q = 0; q < NP; ++q)
 #pragma unroll
         for (int s = 0; s < KS; ++s)
-            xf[q][s] = *reinterpret_cast<const u16x8*>(X + (q * x_pad + x) * KP + s * 16 + half * 8);
+            xf[q][s] = *reinterpret_cast<const f16x8*>(X + (q * x_pad + x) * KP + s * 16 + half * 8);
 
-    u16x8 stage[PER];
+    f16x8 stage[PER];
     float stage_meta = 0.f;
     auto fetch = [&](int t) {
 #pragma unroll
@@ -258,7 +254,7 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
             const int ch = i * 256 + threadIdx.x;
             if (CHUNKS % 256 == 0 || ch < CHUNKS) {
                 const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
-                stage[i] = *reinterpret_cast<const u16x8*>(Y + (q * y_pad + static_cast<int64_t>(t) * kTileY + r) * KP + c * 8);
+                stage[i] = *reinterpret_cast<const f16x8*>(Y + (q * y_pad + static_cast<int64_t>(t) * kTileY + r) * KP + c * 8);
             }
         }
         if (threadIdx.x < NM * kTileY) {
@@ -273,7 +269,7 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
             const int ch = i * 256 + threadIdx.x;
             if (CHUNKS % 256 == 0 || ch < CHUNKS) {
                 const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
-                *reinterpret_cast<u16x8*>(tile + (b * NP + q) * PIECE + lds_chunk<KP>(r, c) * 8) = stage[i];
+                *reinterpret_cast<f16x8*>(tile + (b * NP + q) * PIECE + lds_chunk<KP>(r, c) * 8) = stage[i];
             }
         }
         if (threadIdx.x < NM * kTileY) meta[b * NM * kTileY + threadIdx.x] = stage_meta;
@@ -292,18 +288,18 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
     for (int t = t0; t < t1; ++t) {
         const int b = (t - t0) & 1;
         if (t + 1 < t1) fetch(t + 1);
-        const unsigned short* tl = tile + b * NP * PIECE;
+        const _Float16* tl = tile + b * NP * PIECE;
         const float* mt = meta + b * NM * kTileY;
 
         f32x16 s = f32x16{0};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const u16x8 y0 = *reinterpret_cast<const u16x8*>(tl + lds_chunk<KP>(lx, ks * 2 + half) * 8);
-            s = mfma16<T>(y0, xf[0][ks], s);
+            const f16x8 y0 = *reinterpret_cast<const f16x8*>(tl + lds_chunk<KP>(lx, ks * 2 + half) * 8);
+            s = mfma16(y0, xf[0][ks], s);
             if constexpr (NP == 2) {
-                const u16x8 y1 = *reinterpret_cast<const u16x8*>(tl + PIECE + lds_chunk<KP>(lx, ks * 2 + half) * 8);
-                s = mfma16<T>(y0, xf[1][ks], s);
-                s = mfma16<T>(y1, xf[0][ks], s);
+                const f16x8 y1 = *reinterpret_cast<const f16x8*>(tl + PIECE + lds_chunk<KP>(lx, ks * 2 + half) * 8);
+                s = mfma16(y0, xf[1][ks], s);
+                s = mfma16(y1, xf[0][ks], s);
             }
         }
         // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the tile
@@ -360,23 +356,22 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
         if constexpr (MODE != kLoss) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                u16x8 c0, c1;
+                f16x8 c0, c1;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float f = s[8 * j + e];
                     // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
                     // product before it would round to another hi now and then
                     if (NP == 2) asm("" : "+v"(f));
-                    const T h = static_cast<T>(f);
-                    c0[e] = __builtin_bit_cast(unsigned short, h);
-                    if (NP == 2) c1[e] = __builtin_bit_cast(unsigned short, static_cast<T>(f - static_cast<float>(h)));
+                    c0[e] = static_cast<_Float16>(f);
+                    if (NP == 2) c1[e] = static_cast<_Float16>(f - static_cast<float>(c0[e]));
                 }
                 // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c0's.  A transposing
                 // read hands lane i of a group of 16 the column i of the 4 x 16 block whose rows its lanes address.
                 const int g = lane & 15, row = 16 * j + 4 * half + (g >> 2), col = oc0 + 16 * ((lane >> 4) & 1) + 4 * (g & 3);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    u16x8 yt[NP];
+                    f16x8 yt[NP];
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
                         const int cc = col + nb * 32;
@@ -385,13 +380,12 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
                                 tl + q * PIECE + lds_chunk<KP>(r, cc >> 3) * 8 + (cc & 7)));
                         };
                         const s16x4 u = rd(row), w = rd(row + 8);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) yt[q][e] = u[e], yt[q][4 + e] = w[e];
+                        yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
                     }
-                    acc[nb] = mfma16<T>(yt[0], c0, acc[nb]);
+                    acc[nb] = mfma16(yt[0], c0, acc[nb]);
                     if constexpr (NP == 2) {
-                        acc[nb] = mfma16<T>(yt[0], c1, acc[nb]);
-                        acc[nb] = mfma16<T>(yt[1], c0, acc[nb]);
+                        acc[nb] = mfma16(yt[0], c1, acc[nb]);
+                        acc[nb] = mfma16(yt[1], c0, acc[nb]);
                     }
                 }
             }
@@ -431,7 +425,6 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
                 *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * j + 4 * half) = o;
             }
     } else if (x < p.v) {
-        using E = typename std::conditional<NP == 2, float, T>::type;
         if (blockIdx.z == 0 && half == 0) a.dbias[x] = sum * sc.inv_cs;
         E* O = static_cast<E*>(a.dW) + x * a.lddw;
 #pragma unroll
@@ -453,7 +446,6 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     const int64_t rows = p.grad ? p.n_pad : p.n;
     if (n >= rows) return;
     const Scal sc = *a.at<Scal>(p.o_scal);
-    const float shift = p.type == RS_TYPE_BF16 ? 0.f : 14.f;
     const bool known = row_known(a, n);
     float m = -INFINITY, s = 0.f;
     if (known)
@@ -477,8 +469,8 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     if (there && a.bias) lt += a.bias[tg];
     // every item withdrawn: m stays -inf and s is 0
     const bool empty = m == -INFINITY && s == 0.f;
-    const float l2 = m + (log2f(s) - shift);
-    const float lse = empty ? -INFINITY : m * kLn2 + logf(s) - shift * kLn2;
+    const float l2 = m + (log2f(s) - kShift);
+    const float lse = empty ? -INFINITY : m * kLn2 + logf(s) - kShift * kLn2;
     if (lane == 0 && n < p.n) {
         a.lse[n] = known ? lse : 0.f;
         a.loss[n] = !known || empty ? 0.f : there ? lse - lt : INFINITY;
@@ -526,12 +518,12 @@ __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     }
 }
 
-template <typename T, int NP, int KP, int MODE>
+template <typename E, int NP, int KP, int MODE>
 void launch_main(const CeArgs& a, hipStream_t st) {
     const CePlan& p = a.p;
     constexpr int NM = MODE == kItems ? 3 : 1;
     constexpr int lds = 2 * NP * kTileY * KP * 2 + 2 * NM * kTileY * 4;
-    auto kern = ce_main_kernel<T, NP, KP, MODE>;
+    auto kern = ce_main_kernel<E, NP, KP, MODE>;
     if (lds > 64 * 1024)
         RS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const dim3 grid(static_cast<uint32_t>((MODE == kItems ? p.v_pad : p.n_pad) / kTileX),
@@ -540,27 +532,26 @@ void launch_main(const CeArgs& a, hipStream_t st) {
     RS_HIP(hipGetLastError());
 }
 
-template <typename E, typename T, int NP>
+template <typename E, int NP>
 void launch_all(const CeArgs& a, hipStream_t st) {
     const CePlan& p = a.p;
-    const bool f16 = std::is_same<T, _Float16>::value;
     int blocks = 0;
-    if (NP == 2 || (f16 && p.grad && a.weight)) {
+    if (!std::is_same<E, _Float16>::value || (p.grad && a.weight)) {
         blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), 4)));
         ce_max_kernel<E><<<dim3(static_cast<uint32_t>(blocks), 3), 256, 0, st>>>(a);
         RS_HIP(hipGetLastError());
     }
     const int64_t chunks = (p.n_pad + p.v_pad) * (p.kp / 8);
-    ce_pack_kernel<E, T, NP><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(chunks, 256), 4096)), 256, 0, st>>>(a, blocks);
+    ce_pack_kernel<E, NP><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(chunks, 256), 4096)), 256, 0, st>>>(a, blocks);
     RS_HIP(hipGetLastError());
     auto mode = [&](auto m) {
         constexpr int M = decltype(m)::value;
         switch (p.kp) {
-            case 32: return launch_main<T, NP, 32, M>(a, st);
-            case 64: return launch_main<T, NP, 64, M>(a, st);
-            case 128: return launch_main<T, NP, 128, M>(a, st);
-            case 256: return launch_main<T, NP, 256, M>(a, st);
-            default: return launch_main<T, NP, 512, M>(a, st);
+            case 32: return launch_main<E, NP, 32, M>(a, st);
+            case 64: return launch_main<E, NP, 64, M>(a, st);
+            case 128: return launch_main<E, NP, 128, M>(a, st);
+            case 256: return launch_main<E, NP, 256, M>(a, st);
+            default: return launch_main<E, NP, 512, M>(a, st);
         }
     };
     if (p.grad)
@@ -635,11 +626,11 @@ extern "C" int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t 
     return dense_guard(ctx, [&]() -> int {
         const hipStream_t st = pick_stream(ctx, stream);
         if (type == RS_TYPE_F32)
-            launch_all<float, _Float16, 2>(a, st);
+            launch_all<float, 2>(a, st);
         else if (type == RS_TYPE_BF16)
-            launch_all<__bf16, __bf16, 1>(a, st);
+            launch_all<__bf16, 1>(a, st);
         else
-            launch_all<_Float16, _Float16, 1>(a, st);
+            launch_all<_Float16, 1>(a, st);
         return RS_OK;
     });
 }

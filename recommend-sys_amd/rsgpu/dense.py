@@ -111,7 +111,7 @@ class DenseOps:
 
     def quantize_rows(self, X):
         """The rows of X in 8 bits with a scale each (rs_quantize_rows): (q int8, scale fp32), x ~ scale * q with
-        scale = max |x| / 127 of the row.  q's rows are 16-byte multiples apart, as i8_matmul reads them fastest."""
+        scale = max |x| * (1/127) of the row.  q's rows are 16-byte multiples apart, as i8_matmul reads them fastest."""
         import torch
         ty = _type(X, "X")
         ldx = self._mat(X, "X")

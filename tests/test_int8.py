@@ -23,7 +23,7 @@ def quantize_reference(x):
     """The definition with the exact quotient: fractions of 64-bit integers."""
     x = x.float().cpu().numpy()
     amax = np.abs(x).max(axis=1)
-    s = (amax / np.float32(127)).astype(np.float32)
+    s = (amax * (np.float32(1) / np.float32(127))).astype(np.float32)
     q = np.zeros(x.shape, np.int64)
     ok = np.isfinite(amax) & (s > 0)
     # |x| against the ties (j + 1/2) s, exact in 64 bits
