@@ -75,8 +75,8 @@ int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, 
  *   X_0 = G / |G|_F      X_{j+1} = a X_j + (b A_j + c A_j^2) X_j,  A_j = X_j X_j^T      X = X_steps
  * (for rows > cols the same with A_j = X_j^T X_j on the other side): every singular value s of X_0 becomes
  * p(p(..p(s))), p(s) = a s + b s^3 + c s^5; (3.4445, -4.7750, 2.0315) in 5 steps brings all but the smallest near 1.
- * G = 0 gives X = 0.  G and X have the element type `type`; X may be G itself (same pointer and stride), otherwise they
- * must not overlap.  The shorter side is at most RS_DENSE_MAX_FACTORS, 1 <= steps <= RS_ORTHO_MAX_STEPS.
+ * G = 0 gives X = 0.  G and X have the element type `type`; X may be G itself (same pointer and stride; the
+ * shorter side at most 256), otherwise they must not overlap.  The shorter side is at most RS_DENSE_MAX_FACTORS, 1 <= steps <= RS_ORTHO_MAX_STEPS.
  * The polynomials are formed on the shorter side's Gram matrix in fp64, so the table is read twice and written once;
  * with t the largest |p(p(..p(s))) / s|, X is off by a few t 2^-24 of itself at most, plus its rounding. */
 #define RS_ORTHO_MAX_STEPS 16

@@ -15,28 +15,30 @@
 namespace rs {
 namespace {
 
-constexpr int kGT = 64;   // tile of the Gram matrix
-constexpr int kGR = 32;   // long-side rows of a step
-constexpr int kAR = 128;  // long-side rows of an apply tile
+constexpr int kThreads = 512;     // the two passes over the table: 8 waves
+constexpr int kStage = 8192;      // table elements of one stage of the Gram pass (per panel)
 
 struct OrthoPlan {
-    int64_t r;         // long side
-    int32_t s, sp;     // short side, and padded to kGT
-    int32_t nb, pairs; // Gram tiles per side, tiles of the lower triangle
-    int32_t splits;
-    int64_t per;       // long-side rows of a split
-    int64_t o_part, o_mat[6], bytes;  // A0, A, M, U, Ta, Tb
+    int64_t r;       // long side
+    int32_t s, sp;   // short side; padded to 64, 128, 256 or 512
+    int32_t sm;      // side of the chain's matrices: 32, or sp
+    int32_t panels;  // the Gram matrix is panels x panels blocks of at most 256 x 256
+    int32_t splits;  // pieces of the long side, one per workgroup
+    int64_t per;     // long-side rows of a piece
+    int64_t o_part, o_pscale, o_mat[6], o_t, o_scale, bytes;  // A0, A, M, U, Ta, Tb; T's fp16 pieces and their scales
 };
 
 OrthoPlan make_plan(int64_t rows, int64_t cols) {
     OrthoPlan p{};
     p.r = std::max(rows, cols);
     p.s = static_cast<int32_t>(std::min(rows, cols));
-    p.sp = static_cast<int32_t>(round_up(p.s, kGT));
-    p.nb = p.sp / kGT;
-    p.pairs = p.nb * (p.nb + 1) / 2;
-    const int64_t want = std::max<int64_t>(1, 1024 / p.pairs);
-    p.per = round_up(std::max<int64_t>(ceil_div(p.r, want), 64), kGR);
+    p.sp = p.s <= 64 ? 64 : p.s <= 128 ? 128 : p.s <= 256 ? 256 : 512;
+    p.sm = p.s <= 32 ? 32 : p.sp;
+    p.panels = p.sp > 256 ? 2 : 1;
+    const int64_t kr = kStage / std::min(p.sp, 256) / p.panels, stages = ceil_div(p.r, kr);
+    // one workgroup per CU, and a few stages each: the pieces' sums are written and read again
+    p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(256 / (p.panels * p.panels), ceil_div(stages, 4))));
+    p.per = ceil_div(stages, p.splits) * kr;
     p.splits = static_cast<int32_t>(ceil_div(p.r, p.per));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -44,94 +46,271 @@ OrthoPlan make_plan(int64_t rows, int64_t cols) {
         at += round_up(bytes, 256);
         return o;
     };
-    p.o_part = take(static_cast<int64_t>(p.splits) * p.pairs * kGT * kGT * 8);
-    for (int64_t& o : p.o_mat) o = take(static_cast<int64_t>(p.sp) * p.sp * 8);
+    p.o_part = take(static_cast<int64_t>(p.splits) * p.sp * p.sp * 4);
+    p.o_pscale = take(static_cast<int64_t>(p.splits) * p.panels * p.panels * 4);
+    for (int64_t& o : p.o_mat) o = take(static_cast<int64_t>(p.sm) * p.sm * 8);
+    p.o_t = take(static_cast<int64_t>(2) * p.sp * p.sp * 2);
+    p.o_scale = take((p.sp + 1) * 4);
     p.bytes = at;
     return p;
 }
 
-// element (long index r, short index i) of the table
-template <typename E, bool WIDE>
-__device__ __forceinline__ float elem(const E* G, int64_t ld, int64_t r, int i) {
-    return static_cast<float>(WIDE ? G[i * ld + r] : G[r * ld + i]);
+// four elements of the table, consecutive along its contiguous side: long index r, short index i of the first
+template <typename E, bool WIDE, bool VEC>
+__device__ __forceinline__ f32x4 load4(const E* G, int64_t ld, int64_t r, int64_t r1, int i, int s) {
+    typedef __attribute__((ext_vector_type(4))) E e4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (WIDE ? i >= s : r >= r1) return v;
+    const E* src = G + (WIDE ? i * ld + r : r * ld + i);
+    const int n = WIDE ? static_cast<int>(min<int64_t>(r1 - r, 4)) : min(s - i, 4);
+    if (VEC && n >= 4) {
+        const e4 x = *reinterpret_cast<const e4*>(src);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(x[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e < n) v[e] = static_cast<float>(src[e]);
+    }
+    return v;
 }
 
-// ---- Gram tiles of a piece of the long side (fp64 sums of exact products) ------------------------------------------
-template <typename E, bool WIDE>
-__global__ __launch_bounds__(256) void ortho_gram_kernel(const E* __restrict__ G, int64_t ld, OrthoPlan p, double* __restrict__ part) {
-    __shared__ float gi[kGR][kGT + 1], gj[kGR][kGT + 1];
-    int ib = 0, t = blockIdx.x;
-    while (t > ib) t -= ++ib;  // tile t of the lower triangle: row ib, column t
-    const int jb = t;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 15, lk = lane >> 4;
-    const int wi = (wave & 1) * 32, wj = (wave >> 1) * 32;
-    const int64_t r0 = blockIdx.y * p.per, r1 = min(p.r, r0 + p.per);
-    f64x4 acc[2][2];
+// 16-byte chunk c of row r of an LDS tile of W 16-bit columns sits at chunk c ^ (r mod 16) of its row (fewer where a
+// row has fewer): element offset
+template <int W>
+__device__ __forceinline__ int lds_at(int row, int col) {
+    constexpr int C = W / 8, M = C < 16 ? C - 1 : 15;
+    return (row * C + ((col >> 3) ^ (row & M))) * 8 + (col & 7);
+}
+
+// ---- Gram matrix of a piece of the long side -----------------------------------------------------------------------
+// On fp16 MFMAs, the table scaled by a power of two that follows the largest element seen (a stage four times
+// larger than the last reference moves it, and the sums with it: both exact), so any magnitudes are right.  16-bit
+// tables: G^T G by one product.  fp32 as pairs g = h + l: with B = h (h / 2 + l), two products, G^T G is B + B^T up to
+// 2^-24 of its terms.  The long side is the contraction: the operands come from a row-major LDS stage by
+// transposing reads.
+// SP: columns of a panel (64, 128, 256); eight waves as WI x WJ blocks of 64 x 64 or (SP = 256) 64 x 128, NG groups
+// of waves share a stage's rows.  PAN: 1, or 2 where blockIdx.y's block has different row and column panels (SP = 256).
+template <typename E, bool WIDE, bool VEC, int SP, int PAN>
+__global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restrict__ G, int64_t ld, OrthoPlan p, float* __restrict__ part,
+                                                             float* __restrict__ part_scale) {
+    constexpr int NP = std::is_same<E, float>::value ? 2 : 1;
+    constexpr int KR = kStage / SP / PAN, WI = SP / 64, WJ = SP == 256 ? 2 : SP / 64, NG = 8 / (WI * WJ), BJ = SP / WJ / 32;
+    constexpr int PIECE = KR * SP, BUF = PAN * NP * PIECE;  // 16-bit elements
+    constexpr int PER = kStage / 4 / kThreads;              // groups of four elements a thread stages
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    _Float16* tile = reinterpret_cast<_Float16*>(smem);     // [2][PAN][NP][KR][SP]
+    __shared__ uint32_t smax[2][8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lx = lane & 31, half = lane >> 5;
+    const int grp = wave / (WI * WJ), wi = (wave % (WI * WJ)) / WJ * 64, wj = (wave % WJ) * (SP / WJ);
+    const int pi = PAN == 2 ? blockIdx.y / p.panels : 0, pj = PAN == 2 ? blockIdx.y % p.panels : 0;
+    const int64_t r0 = blockIdx.x * p.per, r1 = min(p.r, r0 + p.per);
+
+    f32x4 st[PER];
+    auto place = [&](int i, int& pan, int& row, int& col) {
+        const int g = i * kThreads + threadIdx.x;
+        pan = g / (PIECE / 4);
+        const int q = g % (PIECE / 4);
+        if (WIDE)
+            row = q % (KR / 4) * 4, col = q / (KR / 4);
+        else
+            row = q / (SP / 4), col = q % (SP / 4) * 4;
+    };
+    auto fetch = [&](int64_t rb) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int pan, row, col;
+            place(i, pan, row, col);
+            st[i] = load4<E, WIDE, VEC>(G, ld, rb + row, r1, (pan ? pj : pi) * 256 + col, p.s);
+        }
+    };
+    // the stage's largest finite magnitude, over the workgroup
+    auto largest = [&](int b) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t u = __float_as_uint(st[i][e]) & 0x7FFFFFFFu;
+                if (u < 0x7F800000u && u > m) m = u;
+            }
+        m = wave_max_u32(m);
+        if (lane == 0) smax[b][wave] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, smax[b][i]);
+        return m;
+    };
+    auto put = [&](int b, float sc) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int pan, row, col;
+            place(i, pan, row, col);
+            _Float16* t = tile + b * BUF + pan * NP * PIECE;
+            f16x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = st[i][e] * sc;  // (a power of two: exact)
+                h[e] = static_cast<_Float16>(x);
+                l[e] = static_cast<_Float16>(x - static_cast<float>(h[e]));
+            }
+            if (WIDE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    t[lds_at<SP>(row + e, col)] = h[e];
+                    if (NP == 2) t[PIECE + lds_at<SP>(row + e, col)] = l[e];
+                }
+            } else {
+                *reinterpret_cast<f16x4*>(t + lds_at<SP>(row, col)) = h;
+                if (NP == 2) *reinterpret_cast<f16x4*>(t + PIECE + lds_at<SP>(row, col)) = l;
+            }
+        }
+    };
+    // operand: lane = column c0 + lane mod 32 of the stage, elements = its rows k0 + 8 half + (0..7)
+    const int g4 = (lane & 15) >> 2, c4 = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    auto frag = [&](const _Float16* t, int k0, int c0) {
+        auto rd = [&](int row) {
+            return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(t + lds_at<SP>(row, c0 + c4)));
+        };
+        const s16x4 u = rd(k0 + 8 * half + g4), w = rd(k0 + 8 * half + 4 + g4);
+        return __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    f32x16 acc[2][BJ];
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) acc[x][y] = f64x4{0};
-    for (int64_t rb = r0; rb < r1; rb += kGR) {
-        for (int e = threadIdx.x; e < kGR * kGT; e += 256) {
-            const int rr = WIDE ? e % kGR : e / kGT, c = WIDE ? e / kGR : e % kGT;
-            const int64_t r = rb + rr;
-            gi[rr][c] = r < r1 && ib * kGT + c < p.s ? elem<E, WIDE>(G, ld, r, ib * kGT + c) : 0.f;
-            gj[rr][c] = r < r1 && jb * kGT + c < p.s ? elem<E, WIDE>(G, ld, r, jb * kGT + c) : 0.f;
-        }
-        __syncthreads();
+        for (int y = 0; y < BJ; ++y) acc[x][y] = f32x16{0};
+    // scale: 2^(12 - exponent of the reference); a stage's largest may reach 2^15
+    float sc = 1.f;
+    uint32_t limit = 0;  // bits of the largest magnitude the scale stands
+    auto follow = [&](uint32_t m) {
+        if (m <= limit) return;
+        const int e = max(static_cast<int>(m >> 23), 1) - 127;
+        limit = e + 3 > 127 ? 0x7F7FFFFFu : static_cast<uint32_t>(e + 3 + 127) << 23;
+        const float next = __uint_as_float(static_cast<uint32_t>(min(12 - e, 126) + 127) << 23), f = next / sc;
+        sc = next;
 #pragma unroll
-        for (int k = 0; k < kGR; k += 4) {
-            double a[2], b[2];
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                a[x] = static_cast<double>(gi[k + lk][wi + 16 * x + lc]);
-                b[x] = static_cast<double>(gj[k + lk][wj + 16 * x + lc]);
+            for (int y = 0; y < BJ; ++y)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[x][y][i] = acc[x][y][i] * f * f;
+    };
+    fetch(r0);
+    follow(largest(0));
+    put(0, sc);
+    __syncthreads();
+    int b = 0;
+    for (int64_t rb = r0; rb < r1; rb += KR, b ^= 1) {
+        const bool more = rb + KR < r1;
+        if (more) fetch(rb + KR);
+        const _Float16 *ti = tile + b * BUF, *tj = ti + (PAN - 1) * NP * PIECE;
+#pragma unroll
+        for (int k = 0; k < KR / 16 / NG; ++k) {
+            const int k0 = (k * NG + grp) * 16;
+            f16x8 fi[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) fi[x] = frag(ti, k0, wi + 32 * x);
+#pragma unroll
+            for (int y = 0; y < BJ; ++y) {
+                f16x8 j1 = frag(tj, k0, wj + 32 * y);
+                if constexpr (NP == 2) j1 *= static_cast<_Float16>(0.5f);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fi[x], j1, acc[x][y], 0, 0, 0);
+                if constexpr (NP == 2) {
+                    const f16x8 j2 = frag(tj + PIECE, k0, wj + 32 * y);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fi[x], j2, acc[x][y], 0, 0, 0);
+                }
             }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) acc[x][y] = __builtin_amdgcn_mfma_f64_16x16x4f64(a[x], b[y], acc[x][y], 0, 0, 0);
+        }
+        if (more) {
+            follow(largest(b ^ 1));
+            put(b ^ 1, sc);
         }
         __syncthreads();
     }
-    double* o = part + (static_cast<int64_t>(blockIdx.y) * p.pairs + blockIdx.x) * kGT * kGT;
+    if (threadIdx.x == 0) part_scale[blockIdx.y * gridDim.x + blockIdx.x] = sc;
+    // the groups' sums, halving their number through LDS
+    float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int n = NG / 2; n; n /= 2) {
+        float* slot = red + ((grp % n) * (SP * SP)) + ((wave % (WI * WJ)) * 2 * BJ) * 1024;
+        if (grp >= n && grp < 2 * n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < BJ; ++y)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) slot[((x * BJ + y) * 16 + e) * 64 + lane] = acc[x][y][e];
+        __syncthreads();
+        if (grp < n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < BJ; ++y)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[x][y][e] += slot[((x * BJ + y) * 16 + e) * 64 + lane];
+        __syncthreads();
+    }
+    if (grp) return;
+    float* o = part + static_cast<int64_t>(blockIdx.x) * p.sp * p.sp + static_cast<int64_t>(pi * 256) * p.sp + pj * 256;
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < BJ; ++y)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[(wi + 16 * x + 4 * e + lk) * kGT + wj + 16 * y + lc] = acc[x][y][e];
+            for (int e = 0; e < 16; ++e)
+                o[static_cast<int64_t>(wi + 32 * x + 8 * (e / 4) + 4 * half + e % 4) * p.sp + wj + 32 * y + lx] = acc[x][y][e];
 }
 
-// the pieces' sum, in their order, to both triangles
-__global__ __launch_bounds__(256) void ortho_gram_join_kernel(const double* __restrict__ part, OrthoPlan p, double* __restrict__ A) {
+// A0 = sum of the pieces' B + B^T (16-bit tables: their half) in fp64, in the pieces' order; a 16 x 16 block and its
+// mirror per workgroup, four groups of 256 threads share the pieces.
+__global__ __launch_bounds__(1024) void ortho_gram_join_kernel(const float* __restrict__ part, const float* __restrict__ part_scale,
+                                                              OrthoPlan p, double scale, double* __restrict__ A) {
+    __shared__ double sm[2][4][16][17];
     int ib = 0, t = blockIdx.x;
-    while (t > ib) t -= ++ib;
-    const int jb = t;
-    const int e = blockIdx.y * 256 + threadIdx.x;  // element of the tile
-    double s = 0.0;
-    for (int i = 0; i < p.splits; ++i) s += part[(static_cast<int64_t>(i) * p.pairs + blockIdx.x) * kGT * kGT + e];
-    const int i = ib * kGT + e / kGT, j = jb * kGT + e % kGT;
-    if (ib == jb && e / kGT < e % kGT) return;  // a diagonal tile's upper half is its lower half's mirror
-    A[static_cast<int64_t>(i) * p.sp + j] = s;
-    A[static_cast<int64_t>(j) * p.sp + i] = s;
+    while (t > ib) t -= ++ib;  // block t of the lower triangle: row ib, column t
+    const int jb = t, g = threadIdx.x >> 8, i = (threadIdx.x >> 4) & 15, j = threadIdx.x & 15;
+    const float *u = part + static_cast<int64_t>(ib * 16 + i) * p.sp + jb * 16 + j, *v = part + static_cast<int64_t>(jb * 16 + i) * p.sp + ib * 16 + j;
+    const float *us = part_scale + (ib / 16 * p.panels + jb / 16) * p.splits, *vs = part_scale + (jb / 16 * p.panels + ib / 16) * p.splits;
+    const int64_t step = static_cast<int64_t>(p.sp) * p.sp;
+    double su = 0.0, sv = 0.0;
+    const int n0 = p.splits * g / 4, n1 = p.splits * (g + 1) / 4;
+#pragma unroll 8
+    for (int n = n0; n < n1; ++n) {
+        const double a = 1.0 / us[n], b = 1.0 / vs[n];  // (powers of two)
+        su += static_cast<double>(u[n * step]) * (a * a);
+        sv += static_cast<double>(v[n * step]) * (b * b);
+    }
+    sm[0][g][i][j] = su;
+    sm[1][g][i][j] = sv;
+    __syncthreads();
+    if (g) return;
+    auto sum = [&](int w, int x, int y) { return ((sm[w][0][x][y] + sm[w][1][x][y]) + sm[w][2][x][y]) + sm[w][3][x][y]; };
+    const double a = (sum(0, i, j) + sum(1, j, i)) * scale;
+    A[static_cast<int64_t>(ib * 16 + i) * p.sm + jb * 16 + j] = a;
+    if (ib != jb) A[static_cast<int64_t>(jb * 16 + j) * p.sm + ib * 16 + i] = a;
 }
 
-// trace of A0 over a block of 256 threads (the same sum in every block)
+// trace of A0 over a block of N threads (the same sum in every block)
+template <int N>
 __device__ __forceinline__ double block_trace(const double* A0, const OrthoPlan& p) {
-    __shared__ double sm[4];
+    __shared__ double sm[N / 64];
     double t = 0.0;
-    for (int i = threadIdx.x; i < p.s; i += 256) t += A0[static_cast<int64_t>(i) * p.sp + i];
+    for (int i = threadIdx.x; i < p.s; i += N) t += A0[static_cast<int64_t>(i) * p.sm + i];
 #pragma unroll
     for (int o = 32; o; o >>= 1) t += __shfl_xor(t, o);
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = t;
     __syncthreads();
-    t = sm[0] + sm[1] + sm[2] + sm[3];
+    t = 0.0;
+#pragma unroll
+    for (int i = 0; i < N / 64; ++i) t += sm[i];
     __syncthreads();
     return t;
 }
 
-// ---- S x S products of symmetric, commuting matrices: C = X Y, 32 x 32 per workgroup, 16 x 16 per wave --------------
+// ---- S x S products of symmetric, commuting matrices: C = X Y, 16 x 16 per workgroup, its four waves share k --------
 struct ChainArgs {
     OrthoPlan p;
     const double* A0;        // unnormalised Gram matrix
@@ -144,140 +323,309 @@ struct ChainArgs {
 };
 
 __global__ __launch_bounds__(256) void ortho_chain_kernel(ChainArgs q) {
-    const int sp = q.p.sp, z = blockIdx.z;
+    __shared__ double sm[3][4][64];
+    const int sm_ = q.p.sm, z = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 15, lk = lane >> 4;
-    const int i0 = blockIdx.x * 32 + (wave & 1) * 16, j0 = blockIdx.y * 32 + (wave >> 1) * 16;
-    const double *X = q.X[z], *Y = q.Y[z];
-    double inv = 1.0;
-    if (q.normalise && z == 0) {
-        const double tr = block_trace(q.A0, q.p);
-        inv = tr == 0.0 ? 0.0 : 1.0 / tr;
-    }
-    f64x4 acc = f64x4{0};
+    const int i0 = blockIdx.x * 16, j0 = blockIdx.y * 16, kq = sm_ / 4;
     // X and Y are symmetric: both operands are read along rows k
-    for (int k = 0; k < sp; k += 32) {
+    const double *X = q.X[z] + static_cast<int64_t>(wave * kq + lk) * sm_ + i0 + lc, *Y = q.Y[z] + static_cast<int64_t>(wave * kq + lk) * sm_ + j0 + lc;
+    f64x4 acc = f64x4{0};
+    for (int k = 0; k < kq; k += 32) {
         double a[8], b[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            a[u] = X[static_cast<int64_t>(k + 4 * u + lk) * sp + i0 + lc];
-            b[u] = Y[static_cast<int64_t>(k + 4 * u + lk) * sp + j0 + lc];
-        }
+        for (int u = 0; u < 8; ++u)
+            if (k + 4 * u < kq) {
+                a[u] = X[static_cast<int64_t>(k + 4 * u) * sm_];
+                b[u] = Y[static_cast<int64_t>(k + 4 * u) * sm_];
+            }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[u], b[u], acc, 0, 0, 0);
+        for (int u = 0; u < 8; ++u)
+            if (k + 4 * u < kq) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(a[u], b[u], acc, 0, 0, 0);
     }
+    double inv = 1.0;
+    if (q.normalise && z == 0) {
+        const double tr = block_trace<256>(q.A0, q.p);
+        inv = tr == 0.0 ? 0.0 : 1.0 / tr;
+    }
+    if (wave)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sm[wave - 1][e][lane] = acc[e];
+    __syncthreads();
+    if (wave) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int i = i0 + 4 * e + lk, j = j0 + lc;
-        const int64_t at = static_cast<int64_t>(i) * sp + j;
-        double v = acc[e] * inv;
-        if (q.poly && z == 0) v = (i == j ? q.a : 0.0) + q.b * X[at] * inv + q.c * (v * inv);
+        const int64_t at = static_cast<int64_t>(i) * sm_ + j;
+        double v = (((acc[e] + sm[0][e][lane]) + sm[1][e][lane]) + sm[2][e][lane]) * inv;
+        if (q.poly && z == 0) v = (i == j ? q.a : 0.0) + q.b * q.X[0][at] * inv + q.c * (v * inv);
         q.C[z][at] = v;
     }
 }
 
-// ---- X = G T / |G| -------------------------------------------------------------------------------------------------
-// NB: column tiles at most (each workgroup has all columns of its rows)
-template <typename E, bool WIDE, int NB>
-__global__ __launch_bounds__(256) void ortho_apply_kernel(const E* G, int64_t ldg, OrthoPlan p, const double* __restrict__ A0,
-                                                         const double* __restrict__ T, E* X, int64_t ldx) {
-    __shared__ float gs[32][kAR + 1], ts[32][kGT + 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 31, half = lane >> 5;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kAR;
-    const double tr = block_trace(A0, p);
-    const float inv = tr == 0.0 ? 0.f : static_cast<float>(1.0 / sqrt(tr));
-    // every column tile of these rows, their sums kept until all are read: X may be G
-    f32x16 acc[NB][2];
+// The whole chain in one workgroup, its matrices in LDS: SM = 32 (four waves), 64 (sixteen), a 16 x 16 block each.  The
+// steps between products cost a barrier instead of a launch.
+template <int SM>
+__global__ __launch_bounds__(SM * SM / 4) void ortho_small_chain_kernel(OrthoPlan p, const double* A0, double* T, int steps, double a, double b, double c) {
+    constexpr int N = SM * SM / 4, LD = SM + 1;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    double* mat = reinterpret_cast<double*>(smem);  // A, M, U, T of SM x LD
+    double *A = mat, *M = mat + SM * LD, *U = M + SM * LD, *Tl = U + SM * LD;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 15, lk = lane >> 4;
+    const int i0 = wave / (SM / 16) * 16, j0 = wave % (SM / 16) * 16;
+    const double tr = block_trace<N>(A0, p), inv = tr == 0.0 ? 0.0 : 1.0 / tr;
+    for (int e = threadIdx.x; e < SM * SM; e += N) A[e / SM * LD + e % SM] = A0[e] * inv;
+    __syncthreads();
+    auto product = [&](const double* X, const double* Y) {
+        f64x4 acc = f64x4{0};
 #pragma unroll
-    for (int jb = 0; jb < NB; ++jb) acc[jb][0] = acc[jb][1] = f32x16{0};
-    for (int k0 = 0; k0 < p.s; k0 += 32) {
+        for (int k = 0; k < SM; k += 4) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(X[(k + lk) * LD + i0 + lc], Y[(k + lk) * LD + j0 + lc], acc, 0, 0, 0);
+        return acc;
+    };
+    auto write = [&](double* C, f64x4 v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) C[(i0 + 4 * e + lk) * LD + j0 + lc] = v[e];
+    };
+    for (int j = 0; j < steps; ++j) {
+        f64x4 v = product(A, A);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int x = i0 + 4 * e + lk, y = j0 + lc;
+            v[e] = (x == y ? a : 0.0) + b * A[x * LD + y] + c * v[e];
+        }
+        write(M, v);
+        if (j == 0) write(Tl, v);
         __syncthreads();
-        for (int e = threadIdx.x; e < 32 * kAR; e += 256) {
-            const int rr = WIDE ? e % kAR : e / 32, c = WIDE ? e / kAR : e % 32;
-            gs[c][rr] = r0 + rr < p.r && k0 + c < p.s ? elem<E, WIDE>(G, ldg, r0 + rr, k0 + c) : 0.f;
-        }
-#pragma unroll
-        for (int jb = 0; jb < NB; ++jb) {
-            if (jb >= p.nb) break;
-            __syncthreads();
-            for (int e = threadIdx.x; e < 32 * kGT; e += 256)
-                ts[e / kGT][e % kGT] = static_cast<float>(T[static_cast<int64_t>(k0 + e / kGT) * p.sp + jb * kGT + e % kGT]);
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-                const float g = gs[k + half][wave * 32 + lc];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const float t = ts[k + half][32 * y + lc];
-                    // lanes run along the contiguous side of X
-                    acc[jb][y] = WIDE ? __builtin_amdgcn_mfma_f32_32x32x2f32(t, g, acc[jb][y], 0, 0, 0)
-                                      : __builtin_amdgcn_mfma_f32_32x32x2f32(g, t, acc[jb][y], 0, 0, 0);
-                }
-            }
-        }
+        const bool last = j + 1 == steps;
+        f64x4 u = f64x4{0}, t = f64x4{0};
+        if (!last) u = product(A, M);
+        if (j) t = product(Tl, M);
+        if (!last) write(U, u);
+        __syncthreads();
+        if (j) write(Tl, t);
+        if (!last) v = product(U, M), write(A, v);
+        __syncthreads();
     }
-#pragma unroll
-    for (int jb = 0; jb < NB; ++jb)
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int row = 8 * (e / 4) + 4 * half + e % 4;
-                const int64_t r = r0 + wave * 32 + (WIDE ? lc : row);
-                const int j = jb * kGT + 32 * y + (WIDE ? row : lc);
-                if (r < p.r && j < p.s) X[WIDE ? j * ldx + r : r * ldx + j] = static_cast<E>(acc[jb][y][e] * inv);
-            }
+    for (int e = threadIdx.x; e < SM * SM; e += N) T[e] = Tl[e / SM * LD + e % SM];
 }
 
-template <typename E, bool WIDE>
+// T as two fp16 pieces, each row (T is symmetric: each column) scaled by a power of two to below 2^14; scale[j] takes an
+// element of G T back and divides by |G|, scale[sp] is the power of two that brings G below 2^14.  A wave per row.
+__global__ __launch_bounds__(64) void ortho_pack_kernel(OrthoPlan p, const double* __restrict__ A0, const double* __restrict__ T,
+                                                       _Float16* __restrict__ tp, float* __restrict__ scale) {
+    const int j = blockIdx.x, lane = threadIdx.x;
+    double tr = 0.0;
+    for (int i = lane; i < p.s; i += 64) tr += A0[static_cast<int64_t>(i) * p.sm + i];
+#pragma unroll
+    for (int o = 32; o; o >>= 1) tr += __shfl_xor(tr, o);
+    const double norm = sqrt(tr);
+    auto power = [](int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); };
+    int eg = 0;
+    if (norm > 0.0 && norm < 1e300) eg = 13 - ilogb(norm);
+    eg = min(max(eg, -126), 126);
+    double m = 0.0;
+    if (j < p.sm)
+        for (int i = lane; i < p.sm; i += 64) m = fmax(m, fabs(T[static_cast<int64_t>(j) * p.sm + i]));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmax(m, __shfl_xor(m, o));
+    int et = 0;
+    if (m > 0.0 && m < 1e300) et = 13 - ilogb(m);
+    et = min(max(et, -120), 120);
+    const double st = ldexp(1.0, et);
+    for (int i = lane; i < p.sp; i += 64) {
+        const double v = j < p.sm && i < p.sm ? T[static_cast<int64_t>(j) * p.sm + i] * st : 0.0;
+        const _Float16 h = static_cast<_Float16>(static_cast<float>(v));
+        tp[static_cast<int64_t>(j) * p.sp + i] = h;
+        tp[static_cast<int64_t>(p.sp + j) * p.sp + i] = static_cast<_Float16>(static_cast<float>(v - static_cast<double>(static_cast<float>(h))));
+    }
+    if (lane == 0) {
+        // G = 0: X = 0.  The product of the two powers and 1 / |G| is near 1 / (2^13 2^13): formed in fp64.
+        scale[j] = norm == 0.0 ? 0.f : static_cast<float>(ldexp(1.0, -et - eg) / norm);
+        if (j == 0) scale[p.sp] = power(eg);
+    }
+}
+
+// ---- X = G T / |G| -------------------------------------------------------------------------------------------------
+// Each wave keeps 32 columns of T in registers (both pieces) for all its rows of G; a tile of G passes through LDS as fp16
+// (fp32: pairs) that all waves read: the table is read once from memory and X written once.  Products: hi T1 + hi T2
+// + lo T1.  SP: short side; KS = SP / 16 steps; WC waves cover the columns of a workgroup (all of them up to 256).
+template <typename E, bool WIDE, bool VEC, int SP, int THREADS>
+__global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_t ldg, OrthoPlan p, const _Float16* __restrict__ tp,
+                                                             const float* __restrict__ scale, E* X, int64_t ldx) {
+    constexpr int NP = std::is_same<E, float>::value ? 2 : 1;
+    constexpr int WAVES = THREADS / 64, WC = SP / 32 < WAVES ? SP / 32 : WAVES, NG = WAVES / WC, KS = SP / 16;
+    constexpr int TR = 32 * NG, PIECE = TR * SP, PER = PIECE / 4 / THREADS;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    _Float16* tile = reinterpret_cast<_Float16*>(smem);  // [2][NP][TR][SP]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lx = lane & 31, half = lane >> 5;
+    const int grp = wave / WC, j0 = blockIdx.y * (WC * 32) + wave % WC * 32;
+    const float gscale = scale[p.sp];
+    f16x8 t[2][KS];
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) t[q][k] = *reinterpret_cast<const f16x8*>(tp + (static_cast<int64_t>(q) * SP + j0 + lx) * SP + k * 16 + half * 8);
+    f32x4 st[PER];
+    auto place = [&](int i, int& row, int& col) {
+        const int g = i * THREADS + threadIdx.x;
+        if (WIDE)
+            row = g % (TR / 4) * 4, col = g / (TR / 4);
+        else
+            row = g / (SP / 4), col = g % (SP / 4) * 4;
+    };
+    auto fetch = [&](int64_t r0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int row, col;
+            place(i, row, col);
+            st[i] = load4<E, WIDE, VEC>(G, ldg, r0 + row, p.r, col, p.s);
+        }
+    };
+    auto put = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int row, col;
+            place(i, row, col);
+            _Float16* d = tile + b * NP * PIECE;
+            f16x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = st[i][e] * gscale;  // (a power of two: exact)
+                h[e] = static_cast<_Float16>(x);
+                l[e] = static_cast<_Float16>(x - static_cast<float>(h[e]));
+            }
+            if (WIDE) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    d[lds_at<SP>(row + e, col)] = h[e];
+                    if (NP == 2) d[PIECE + lds_at<SP>(row + e, col)] = l[e];
+                }
+            } else {
+                *reinterpret_cast<f16x4*>(d + lds_at<SP>(row, col)) = h;
+                if (NP == 2) *reinterpret_cast<f16x4*>(d + PIECE + lds_at<SP>(row, col)) = l;
+            }
+        }
+    };
+    const int64_t tiles = (p.r + TR - 1) / TR;
+    int64_t it = blockIdx.x;
+    if (it < tiles) fetch(it * TR), put(0);
+    __syncthreads();
+    int b = 0;
+    for (; it < tiles; it += gridDim.x, b ^= 1) {
+        const bool more = it + gridDim.x < tiles;
+        if (more) fetch((it + gridDim.x) * TR);
+        const _Float16* d = tile + b * NP * PIECE;
+        f32x16 acc = f32x16{0};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            f16x8 g[NP];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) g[q] = *reinterpret_cast<const f16x8*>(d + q * PIECE + lds_at<SP>(grp * 32 + lx, k * 16 + half * 8));
+            // lanes run along the contiguous side of X
+            auto mm = [&](f16x8 u, f16x8 v) {
+                acc = WIDE ? __builtin_amdgcn_mfma_f32_32x32x16_f16(v, u, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(u, v, acc, 0, 0, 0);
+            };
+            mm(g[0], t[0][k]);
+            mm(g[0], t[1][k]);
+            if constexpr (NP == 2) mm(g[1], t[0][k]);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int o = 8 * (e / 4) + 4 * half + e % 4;
+            const int64_t r = it * TR + grp * 32 + (WIDE ? lx : o);
+            const int j = j0 + (WIDE ? o : lx);
+            if (r < p.r && j < p.s) X[WIDE ? j * ldx + r : r * ldx + j] = static_cast<E>(acc[e] * scale[j]);
+        }
+        if (more) put(b ^ 1);
+        __syncthreads();
+    }
+}
+
+template <typename K, typename... A>
+void launch_lds(K kern, dim3 grid, int threads, int lds, hipStream_t st, A... args) {
+    if (lds > 64 * 1024)
+        RS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    kern<<<grid, threads, lds, st>>>(args...);
+    RS_HIP(hipGetLastError());
+}
+
+template <typename E, bool WIDE, bool VEC>
 void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, double b, double c, E* X, int64_t ldx, char* ws,
          hipStream_t st) {
-    double* part = reinterpret_cast<double*>(ws + p.o_part);
+    constexpr bool kF32 = std::is_same<E, float>::value;
+    float* part = reinterpret_cast<float*>(ws + p.o_part);
+    float* part_scale = reinterpret_cast<float*>(ws + p.o_pscale);
     double* mat[6];
     for (int i = 0; i < 6; ++i) mat[i] = reinterpret_cast<double*>(ws + p.o_mat[i]);
     double *A0 = mat[0], *M = mat[2], *U = mat[3], *T = mat[4], *T2 = mat[5];
-    ortho_gram_kernel<E, WIDE><<<dim3(p.pairs, p.splits), 256, 0, st>>>(G, ldg, p, part);
-    RS_HIP(hipGetLastError());
-    ortho_gram_join_kernel<<<dim3(p.pairs, kGT * kGT / 256), 256, 0, st>>>(part, p, A0);
-    RS_HIP(hipGetLastError());
-    const uint32_t t = static_cast<uint32_t>(p.sp / 32);
-    ChainArgs q{};
-    q.p = p, q.A0 = A0, q.a = a, q.b = b, q.c = c;
-    const double* A = A0;
-    for (int j = 0; j < steps; ++j) {
-        const bool last = j + 1 == steps;
-        q.normalise = j == 0;
-        double* Mj = j == 0 ? T : M;  // T = M_0
-        q.poly = 1;
-        q.X[0] = q.Y[0] = A, q.C[0] = Mj;
-        ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
-        RS_HIP(hipGetLastError());
-        q.poly = 0;
-        // A M (not after the last step) and T M (not in the first)
-        int z = 0;
-        if (!last) q.X[z] = A, q.Y[z] = Mj, q.C[z] = U, ++z;
-        if (j) q.X[z] = T, q.Y[z] = Mj, q.C[z] = T2, ++z;
-        if (z) ortho_chain_kernel<<<dim3(t, t, static_cast<uint32_t>(z)), 256, 0, st>>>(q);
-        RS_HIP(hipGetLastError());
-        if (j) std::swap(T, T2);
-        if (last) break;
-        q.normalise = 0;
-        q.X[0] = U, q.Y[0] = Mj, q.C[0] = mat[1];
-        ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
-        RS_HIP(hipGetLastError());
-        A = mat[1];
-    }
-    auto apply = [&](auto nb) {
-        ortho_apply_kernel<E, WIDE, decltype(nb)::value><<<static_cast<uint32_t>(ceil_div(p.r, kAR)), 256, 0, st>>>(G, ldg, p, A0, T, X, ldx);
-    };
-    if (p.nb <= 1)
-        apply(std::integral_constant<int, 1>{});
-    else if (p.nb <= 2)
-        apply(std::integral_constant<int, 2>{});
-    else if (p.nb <= 4)
-        apply(std::integral_constant<int, 4>{});
+    _Float16* tp = reinterpret_cast<_Float16*>(ws + p.o_t);
+    float* scale = reinterpret_cast<float*>(ws + p.o_scale);
+
+    const int glds = 2 * (kF32 ? 2 : 1) * kStage * 2;
+    const dim3 ggrid(static_cast<uint32_t>(p.splits), static_cast<uint32_t>(p.panels * p.panels));
+    // (the groups' sums take up to 64 KB of the same LDS)
+    if (p.sp == 64)
+        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 64, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
+    else if (p.sp == 128)
+        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 128, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
+    else if (p.sp == 256)
+        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 1>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
     else
-        apply(std::integral_constant<int, 8>{});
+        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 2>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
+    const uint32_t t = static_cast<uint32_t>(p.sm / 16);
+    ortho_gram_join_kernel<<<t * (t + 1) / 2, 1024, 0, st>>>(part, part_scale, p, kF32 ? 1.0 : 0.5, A0);
     RS_HIP(hipGetLastError());
+
+    if (p.sm == 32) {
+        launch_lds(ortho_small_chain_kernel<32>, dim3(1), 256, 4 * 32 * 33 * 8, st, p, static_cast<const double*>(A0), T, steps, a, b, c);
+    } else if (p.sm == 64) {
+        launch_lds(ortho_small_chain_kernel<64>, dim3(1), 1024, 4 * 64 * 65 * 8, st, p, static_cast<const double*>(A0), T, steps, a, b, c);
+    } else {
+        ChainArgs q{};
+        q.p = p, q.A0 = A0, q.a = a, q.b = b, q.c = c;
+        const double* A = A0;
+        for (int j = 0; j < steps; ++j) {
+            const bool last = j + 1 == steps;
+            q.normalise = j == 0;
+            double* Mj = j == 0 ? T : M;  // T = M_0
+            q.poly = 1;
+            q.X[0] = q.Y[0] = A, q.C[0] = Mj;
+            ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
+            RS_HIP(hipGetLastError());
+            q.poly = 0;
+            // A M (not after the last step) and T M (not in the first)
+            int z = 0;
+            if (!last) q.X[z] = A, q.Y[z] = Mj, q.C[z] = U, ++z;
+            if (j) q.X[z] = T, q.Y[z] = Mj, q.C[z] = T2, ++z;
+            if (z) ortho_chain_kernel<<<dim3(t, t, static_cast<uint32_t>(z)), 256, 0, st>>>(q);
+            RS_HIP(hipGetLastError());
+            if (j) std::swap(T, T2);
+            if (last) break;
+            q.normalise = 0;
+            q.X[0] = U, q.Y[0] = Mj, q.C[0] = mat[1];
+            ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
+            RS_HIP(hipGetLastError());
+            A = mat[1];
+        }
+    }
+    ortho_pack_kernel<<<static_cast<uint32_t>(p.sp), 64, 0, st>>>(p, A0, T, tp, scale);
+    RS_HIP(hipGetLastError());
+
+    auto apply = [&](auto sp, auto threads) {
+        constexpr int SP = decltype(sp)::value, N = decltype(threads)::value;
+        constexpr int WC = SP / 32 < N / 64 ? SP / 32 : N / 64, TR = 32 * (N / 64 / WC);
+        const uint32_t blocks = static_cast<uint32_t>(std::min<int64_t>(ceil_div(p.r, TR), SP == 512 ? 64 : 256));
+        launch_lds(ortho_apply_kernel<E, WIDE, VEC, SP, N>, dim3(blocks, SP / (WC * 32)), N, 2 * (kF32 ? 2 : 1) * TR * SP * 2, st, G, ldg, p,
+                   static_cast<const _Float16*>(tp), static_cast<const float*>(scale), X, ldx);
+    };
+    using std::integral_constant;
+    if (p.sp == 64)
+        apply(integral_constant<int, 64>{}, integral_constant<int, 512>{});
+    else if (p.sp == 128)
+        apply(integral_constant<int, 128>{}, integral_constant<int, 512>{});
+    else if (p.sp == 256)
+        apply(integral_constant<int, 256>{}, integral_constant<int, 512>{});
+    else
+        apply(integral_constant<int, 512>{}, integral_constant<int, 256>{});
 }
 
 std::string check_sizes(int64_t rows, int64_t cols) {
@@ -313,6 +661,7 @@ extern "C" int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t
     for (const std::string& m : {check_matrix("G", G, cols, ldg, type_size(type)), check_matrix("X", X, cols, ldx, type_size(type))})
         if (!m.empty()) return set_error(ctx, RS_ERR_INVALID, m);
     if (G == X && ldg != ldx) return set_error(ctx, RS_ERR_INVALID, "X is G with another row stride");
+    if (G == X && std::min(rows, cols) > 256) return set_error(ctx, RS_ERR_UNSUPPORTED, "X may be G only where the shorter side is at most 256");
     const OrthoPlan p = make_plan(rows, cols);
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");
     if (ws_bytes < p.bytes)
@@ -321,13 +670,16 @@ extern "C" int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t
         const hipStream_t st = pick_stream(ctx, stream);
         with_type(type, [&](auto e) {
             using E = typename decltype(e)::type;
-            auto go = [&](auto wide) {
-                run<E, decltype(wide)::value>(p, static_cast<const E*>(G), ldg, steps, a, b, c, static_cast<E*>(X), ldx, static_cast<char*>(ws), st);
+            // four elements at once where every row starts on a multiple of four
+            const bool vec = reinterpret_cast<uintptr_t>(G) % (4 * sizeof(E)) == 0 && ldg % 4 == 0;
+            auto go = [&](auto wide, auto v) {
+                run<E, decltype(wide)::value, decltype(v)::value>(p, static_cast<const E*>(G), ldg, steps, a, b, c, static_cast<E*>(X), ldx,
+                                                                  static_cast<char*>(ws), st);
             };
             if (rows >= cols)
-                go(std::false_type{});
+                vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
             else
-                go(std::true_type{});
+                vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
         });
         return RS_OK;
     });

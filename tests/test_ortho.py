@@ -1,9 +1,15 @@
 """Orthogonalised updates (rs_orthogonalize): refusals on the CPU, values against the steps in 64 bits on the GPU.
 
-X = G T / |G| with T the product of the steps' polynomials on the short side, formed in fp64 and rounded to fp32 (u32 of
-each entry), the table's rows times T summed in fp32 over the short side S, then 1 / |G| (two roundings): an element is
-off by at most (S + 4) u32 (|G| |T| / |G|_F) and half a step of its type; T's own fp64 error is below 1e-9 of its
-largest entry for the singular values used here.
+X = G T / |G| with T = f(A), A = G^T G / |G|^2 (or G G^T), f the steps' polynomials over s, formed in fp64.  Three errors:
+- the Gram matrix: fp16 pairs leave 3 u32 of each product of two elements (2^-24 of each element, the dropped lo lo),
+  and the fp32 sums of a piece of the long side take a rounding for each of its at most 2 (512 / 16) products of 16 and
+  at most 16 inside each: 83 roundings, each at most u32 of (|G|^T |G|)_ij / |G|^2.  They are independent: an entry of
+  dA has a variance of at most v_ij = 83 u32^2 (|G|^T |G|)_ij^2 / |G|^4.  T moves by V (D o V^T dA V) V^T, V the
+  eigenvectors of A and D the divided differences of f on its eigenvalues (f' on the diagonal), to first order, so an
+  element of X by a sum of variance ((G V)^2 (D^2 o (V^2)^T v V^2) (V^2)^T) / |G|^2, squares taken of each entry; 8 of its
+  standard deviations are allowed.  (The worst case of all roundings at once is no use as a bound: it passes X itself.)
+- T as pairs (2^-24 of an element), the table's too, the dropped lo lo, and S sums in fp32: (S + 6) u32 |G| |T| / |G|.
+- the factor 1 / |G| and half a step of X's own type.
 """
 import ctypes as C
 import math
@@ -20,7 +26,7 @@ COEF = (3.4445, -4.7750, 2.0315)
 
 
 def reference(G, steps=5, coef=COEF):
-    """(X, bound): the steps in 64 bits, and |G| |T| / |G|_F."""
+    """(X, bound): the steps in 64 bits, and what an element may be off before its own type's rounding."""
     G = G.double().cpu()
     norm = torch.linalg.vector_norm(G)
     if norm == 0:
@@ -39,17 +45,31 @@ def reference(G, steps=5, coef=COEF):
         p = a + b * s ** 2 + c * s ** 4
         amp, s = amp * p, s * p
     Tm = V @ torch.diag(amp) @ V.T
-    bound = Y0.abs() @ (Tm.abs() + 1e-9 * 2 ** 24 * Tm.abs().max() / (Y0.shape[1] + 4))
+    # f'(w) by f = amp: d log amp, accumulated along the steps
+    w0 = w.clamp(min=0)
+    s, val, der = w0.clone(), torch.ones_like(w0), torch.zeros_like(w0)  # s^2, f and f' at w0
+    ds = torch.ones_like(w0)
+    for _ in range(steps):
+        p, dp = a + b * s + c * s * s, (b + 2 * c * s) * ds
+        val, der = val * p, der * p + val * dp
+        s, ds = s * p * p, ds * p * p + s * 2 * p * dp
+    gap = w0[:, None] - w0[None, :]
+    near = gap.abs() < 1e-7 * w0.max().clamp(min=1e-300)
+    D = torch.where(near, torch.maximum(der.abs()[:, None], der.abs()[None, :]), ((val[:, None] - val[None, :]) / torch.where(near, torch.ones_like(gap), gap)).abs())
+    v = 83 * U32 ** 2 * (Y0.abs().T @ Y0.abs()) ** 2
+    V2 = V ** 2
+    move = 8 * ((Y0 @ V) ** 2 @ (D ** 2 * (V2.T @ v @ V2)) @ V2.T).sqrt()
+    S = Y0.shape[1]
+    bound = (S + 6) * U32 * (Y0.abs() @ Tm.abs()) + move
     return (Y.T, bound.T) if flip else (Y, bound)
 
 
 def check(X, G, steps=5, coef=COEF):
     ref, bound = reference(G, steps, coef)
-    S = min(G.shape)
     ut = torch.finfo(X.dtype).eps / 2
     tiny = torch.finfo(X.dtype).smallest_normal * torch.finfo(X.dtype).eps
     err = (X.double().cpu() - ref).abs()
-    lim = (S + 4) * U32 * bound * (1 + ut) + ut * ref.abs() + tiny
+    lim = bound * (1 + ut) + (ut + 2 * U32) * ref.abs() + tiny
     assert (err <= lim).all(), (float((err - lim).max()), float((err / lim.clamp(min=1e-300)).max()))
 
 
