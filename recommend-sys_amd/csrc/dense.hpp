@@ -98,6 +98,12 @@ inline std::string check_matrix(const char* name, const void* p, int64_t cols, i
     return std::string();
 }
 
+// LDS written by lanes of a wave before this is read by its other lanes after it
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // maximum over the wave (64 lanes)
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 #pragma unroll

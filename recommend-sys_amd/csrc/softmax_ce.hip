@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
             for (int j = 0; j < 4; ++j) {
                 const f32x4 ls = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
                 const f32x4 wv = *reinterpret_cast<const f32x4*>(mt + kTileY + 8 * j + 4 * half);
-                const i32x4 tg = *reinterpret_cast<const i32x4*>(mt + 2 * kTileY + 8 * j + 4 * half);
+                const i32x4 tg = __builtin_bit_cast(i32x4, *reinterpret_cast<const f32x4*>(mt + 2 * kTileY + 8 * j + 4 * half));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     // a row that takes no part has lse2 = +inf and weight 0

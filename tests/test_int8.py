@@ -117,7 +117,8 @@ def test_quantize_strided_leaves_the_rest(ctx):
 
 
 SHAPES = [(1, 1, 1), (1, 3706, 100), (2, 17, 16), (16, 64, 64), (16, 1000, 250), (17, 33, 65), (5, 40, 4096), (5, 40, 4100),
-          (33, 129, 128), (128, 128, 64), (129, 257, 300), (300, 70, 31), (200, 513, 1040), (64, 256, 128), (257, 640, 96)]
+          (33, 129, 128), (128, 128, 64), (129, 257, 300), (300, 70, 31), (200, 513, 1040), (64, 256, 128), (257, 640, 96), (20, 90, 1024), (50, 33, 900), (50, 33, 1100), (65, 20, 64),
+          (3000, 4100, 72), (4097, 4096, 20)]
 
 
 @pytest.mark.gpu
