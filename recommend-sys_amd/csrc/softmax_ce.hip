@@ -25,9 +25,9 @@
 namespace rs {
 namespace {
 
-constexpr int kTileX = 128;      // stationary rows of a workgroup (4 waves of 32)
+constexpr int kTileX = 256;      // stationary rows of a workgroup: a multiple of what its waves hold
 constexpr int kTileY = 32;       // streamed rows of a step
-constexpr int kMaxBlocks = 256;  // blocks of the maxima pass, per matrix
+constexpr int kMaxBlocks = 1024;  // blocks of the maxima pass at most, per matrix
 constexpr float kShift = 14.f;   // p is held as 2^14 p: fp16's range below 1 is short
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -114,8 +114,26 @@ __device__ __forceinline__ bool item_there(const CeArgs& a, int64_t v) {
     return v < a.p.v && !(a.bias && a.bias[v] == -INFINITY);
 }
 
+// Eight elements of a row from column c on as fp32, zeros past column k.  VEC: rows start at 16-byte addresses.
+template <typename E, bool VEC>
+__device__ __forceinline__ void load8(const E* row, int c, int k, float (&v)[8]) {
+    constexpr int V = 16 / sizeof(E);
+    typedef __attribute__((ext_vector_type(V))) E vec;
+    if (VEC && c + 8 <= k) {
+#pragma unroll
+        for (int h = 0; h < 8 / V; ++h) {
+            const vec w = *reinterpret_cast<const vec*>(row + c + h * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[h * V + e] = static_cast<float>(w[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c + e < k ? static_cast<float>(row[c + e]) : 0.f;
+    }
+}
+
 // ---- largest finite magnitudes of H, W and the weights (blockIdx.y = 0, 1, 2), one value per block ----------------
-template <typename E>
+template <typename E, bool VEC>
 __global__ __launch_bounds__(256) void ce_max_kernel(CeArgs a) {
     const int which = blockIdx.y;
     uint32_t m = 0;
@@ -126,13 +144,16 @@ __global__ __launch_bounds__(256) void ce_max_kernel(CeArgs a) {
     if (which < 2) {
         const E* X = static_cast<const E*>(which ? a.W : a.H);
         const int64_t rows = which ? a.p.v : a.p.n, ld = which ? a.ldw : a.ldh;
-        // a wave per row
-        for (int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4) {
-            if (!(which ? item_there(a, r) : row_known(a, r))) continue;
-            for (int c = threadIdx.x & 63; c < a.p.k; c += 64) see(static_cast<float>(X[r * ld + c]));
+        const int lanes = a.p.kp / 8, at = threadIdx.x / lanes, c = threadIdx.x % lanes * 8, step = 256 / lanes;
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * step + at; r < rows; r += static_cast<int64_t>(gridDim.x) * step) {
+            if (c >= a.p.k || !(which ? item_there(a, r) : row_known(a, r))) continue;
+            float v[8];
+            load8<E, VEC>(X + r * ld, c, a.p.k, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) see(v[e]);
         }
     } else if (a.weight) {
-        for (int64_t r = blockIdx.x * 256 + threadIdx.x; r < a.p.n; r += gridDim.x * 256)
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < a.p.n; r += static_cast<int64_t>(gridDim.x) * 256)
             if (row_known(a, r)) see(a.weight[r]);
     }
     m = wave_max_u32(m);
@@ -152,8 +173,8 @@ __device__ __forceinline__ float scale_for(uint32_t max_bits) {
     return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// ---- packing -------------------------------------------------------------------------------------------------------
-template <typename E, int NP>
+// ---- packing: a thread per eight columns ---------------------------------------------------------------------------
+template <typename E, int NP, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) {
     __shared__ uint32_t sm[3];
     if (threadIdx.x < 192) {
@@ -177,10 +198,8 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         s.inv_cs = 1.f / cs;
         *a.at<Scal>(a.p.o_scal) = s;
     }
-    const int64_t per_row = a.p.kp / 8, chunks = (a.p.n_pad + a.p.v_pad) * per_row;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < chunks; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t row = i / per_row;
-        const int c0 = static_cast<int>(i % per_row) * 8;
+    const int lanes = a.p.kp / 8, at = threadIdx.x / lanes, c0 = threadIdx.x % lanes * 8, step = 256 / lanes;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * step + at; row < a.p.n_pad + a.p.v_pad; row += static_cast<int64_t>(gridDim.x) * step) {
         const bool w = row >= a.p.n_pad;
         const int64_t r = w ? row - a.p.n_pad : row;
         const bool there = w ? item_there(a, r) : row_known(a, r);
@@ -190,11 +209,12 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         }
         const E* src = static_cast<const E*>(w ? a.W : a.H) + (there ? r * (w ? a.ldw : a.ldh) : 0);
         const float sc = w ? wsc : hs;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (there) load8<E, VEC>(src, c0, a.p.k, v);
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = there && c0 + e < a.p.k ? static_cast<float>(src[c0 + e]) : 0.f;
-            const float y = x * sc;  // (a power of two: exact)
+            const float y = v[e] * sc;  // (a power of two: exact)
             hi[e] = static_cast<_Float16>(y);
             if (NP == 2) lo[e] = static_cast<_Float16>(y - static_cast<float>(hi[e]));
         }
@@ -208,51 +228,60 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
 __device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // 16-byte chunk c of row r of an LDS tile sits at chunk c ^ (r mod 16) of the row (fewer where a row has fewer
-// chunks): the row-wise and the transposing reads both spread over the banks.
+// chunks): the row-wise and the transposing reads both spread over the banks.  Byte offset: what a lane adds is one
+// base, the constant part of c goes in by XOR (bits the rows do not reach: by addition), so a few registers hold all
+// the addresses of a tile.
 template <int KP>
-__device__ __forceinline__ int lds_chunk(int row, int c) {
-    constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;
-    return row * C + (c ^ (row & M));
-}
+struct LdsTile {
+    static constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;
+    static __device__ __forceinline__ int base(int row, int c) { return row * (KP * 2) + ((c ^ (row & M)) & M) * 16 + (c & ~M) * 16; }
+    // base(row, c) with the constant dc joined to c (no common bits)
+    static __device__ __forceinline__ int at(int base, int dc) { return (base ^ ((dc & M) * 16)) + (dc & ~M) * 16; }
+};
 
+// A wave holds XB blocks of 32 stationary rows: each fragment of Y read from LDS feeds XB products (one block reads 1 KB of
+// LDS per 32-cycle MFMA in each of the four SIMDs: all that LDS gives).
 // MODE kLoss / kLossGrad: x = users' rows, y = items; kItems: x = items, y = users' rows.
-template <typename E, int NP, int KP, int MODE>
-__global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
+template <typename E, int NP, int KP, int MODE, int XB, int WAVES, int OCC>
+__global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
 #pragma clang fp contract(fast)
-    constexpr int OC = KP < 256 ? KP : 256, NB = OC / 32, KS = KP / 16, C = KP / 8;
+    constexpr int THREADS = WAVES * 64;
+    constexpr int OC = KP < 256 ? KP : 256, NB = MODE == kLoss ? 1 : OC / 32, KS = KP / 16, C = KP / 8;
     constexpr int PIECE = kTileY * KP;                     // elements of one piece of a tile
-    constexpr int CHUNKS = kTileY * C * NP, PER = (CHUNKS + 255) / 256;
+    constexpr int CHUNKS = kTileY * C * NP, PER = (CHUNKS + THREADS - 1) / THREADS;
     constexpr int NM = MODE == kItems ? 3 : 1;             // values per streamed row
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    _Float16* tile = reinterpret_cast<_Float16*>(smem);          // [2][NP][kTileY][KP]
+    // smem: [2][NP][kTileY][KP] fp16
     float* meta = reinterpret_cast<float*>(smem + 2 * NP * PIECE * 2);       // [2][NM][kTileY]
 
     const CePlan& p = a.p;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lx = lane & 31, half = lane >> 5;
-    const bool items = MODE == kItems;
+    constexpr bool items = MODE == kItems;
     const int64_t x_pad = items ? p.v_pad : p.n_pad, y_pad = items ? p.n_pad : p.v_pad;
     const _Float16* X = a.at<_Float16>(items ? p.o_w : p.o_h);
     const _Float16* Y = a.at<_Float16>(items ? p.o_h : p.o_w);
     const int per = items ? p.tiles_w : p.tiles_f;
     const int split = blockIdx.y, oc0 = blockIdx.z * OC;
-    const int64_t x = static_cast<int64_t>(blockIdx.x) * kTileX + wave * 32 + lx;
+    const int64_t x0 = (static_cast<int64_t>(blockIdx.x) * WAVES + wave) * (32 * XB);  // the wave's first row
     const int t0 = split * per, t1 = static_cast<int>(min<int64_t>(y_pad / kTileY, t0 + per));
     const Scal sc = *a.at<Scal>(p.o_scal);
 
-    f16x8 xf[NP][KS];
+    f16x8 xf[XB][NP][KS];
 #pragma unroll
-    for (int q = 0; q < NP; ++q)
+    for (int u = 0; u < XB; ++u)
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
-            xf[q][s] = *reinterpret_cast<const f16x8*>(X + (q * x_pad + x) * KP + s * 16 + half * 8);
+        for (int q = 0; q < NP; ++q)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                xf[u][q][s] = *reinterpret_cast<const f16x8*>(X + (q * x_pad + x0 + 32 * u + lx) * KP + s * 16 + half * 8);
 
     f16x8 stage[PER];
     float stage_meta = 0.f;
     auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int ch = i * 256 + threadIdx.x;
-            if (CHUNKS % 256 == 0 || ch < CHUNKS) {
+            const int ch = i * THREADS + threadIdx.x;
+            if (CHUNKS % THREADS == 0 || ch < CHUNKS) {
                 const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
                 stage[i] = *reinterpret_cast<const f16x8*>(Y + (q * y_pad + static_cast<int64_t>(t) * kTileY + r) * KP + c * 8);
             }
@@ -266,21 +295,32 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
     auto put = [&](int b) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int ch = i * 256 + threadIdx.x;
-            if (CHUNKS % 256 == 0 || ch < CHUNKS) {
+            const int ch = i * THREADS + threadIdx.x;
+            if (CHUNKS % THREADS == 0 || ch < CHUNKS) {
                 const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
-                *reinterpret_cast<f16x8*>(tile + (b * NP + q) * PIECE + lds_chunk<KP>(r, c) * 8) = stage[i];
+                *reinterpret_cast<f16x8*>(smem + (b * NP + q) * PIECE * 2 + LdsTile<KP>::base(r, c)) = stage[i];
             }
         }
         if (threadIdx.x < NM * kTileY) meta[b * NM * kTileY + threadIdx.x] = stage_meta;
     };
 
-    f32x16 acc[MODE == kLoss ? 1 : NB];
+    f32x16 acc[NB][XB];
 #pragma unroll
-    for (int b = 0; b < (MODE == kLoss ? 1 : NB); ++b) acc[b] = f32x16{0};
-    float m_run = -INFINITY, sum = 0.f;
-    float bias_x = 0.f;
-    if (items) bias_x = a.at<float>(p.o_bias)[x];
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int u = 0; u < XB; ++u) acc[b][u] = f32x16{0};
+    float m_run[XB], sum[XB], bias_x[XB];
+#pragma unroll
+    for (int u = 0; u < XB; ++u) {
+        m_run[u] = -INFINITY, sum[u] = 0.f;
+        bias_x[u] = items ? a.at<float>(p.o_bias)[x0 + 32 * u + lx] : 0.f;
+    }
+
+    // row-wise reads: row lx, chunk half + 2 ks.  Transposing reads hand lane i of a group of 16 the column i of the
+    // 4 x 16 block whose rows its lanes address: row 4 half + (i / 4) of 8, chunk 2 (group mod 2) + (i mod 4) / 2.
+    const int g4 = lane & 15, row_base = LdsTile<KP>::base(lx, half);
+    const int tr_row = 4 * half + (g4 >> 2), tr_chunk = oc0 / 8 + 2 * ((lane >> 4) & 1) + ((g4 & 3) >> 1);
+    const int tr_base[2] = {LdsTile<KP>::base(tr_row, tr_chunk) + (g4 & 1) * 8, LdsTile<KP>::base(tr_row + 8, tr_chunk) + (g4 & 1) * 8};
 
     fetch(t0);
     put(0);
@@ -288,104 +328,140 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
     for (int t = t0; t < t1; ++t) {
         const int b = (t - t0) & 1;
         if (t + 1 < t1) fetch(t + 1);
-        const _Float16* tl = tile + b * NP * PIECE;
+        const char* tl = smem + b * NP * PIECE * 2;
         const float* mt = meta + b * NM * kTileY;
 
-        f32x16 s = f32x16{0};
+        f32x16 s[XB];
+#pragma unroll
+        for (int u = 0; u < XB; ++u) s[u] = f32x16{0};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const f16x8 y0 = *reinterpret_cast<const f16x8*>(tl + lds_chunk<KP>(lx, ks * 2 + half) * 8);
-            s = mfma16(y0, xf[0][ks], s);
+            const f16x8 y0 = *reinterpret_cast<const f16x8*>(tl + LdsTile<KP>::at(row_base, ks * 2));
+#pragma unroll
+            for (int u = 0; u < XB; ++u) s[u] = mfma16(y0, xf[u][0][ks], s[u]);
             if constexpr (NP == 2) {
-                const f16x8 y1 = *reinterpret_cast<const f16x8*>(tl + PIECE + lds_chunk<KP>(lx, ks * 2 + half) * 8);
-                s = mfma16(y0, xf[1][ks], s);
-                s = mfma16(y1, xf[0][ks], s);
+                const f16x8 y1 = *reinterpret_cast<const f16x8*>(tl + PIECE * 2 + LdsTile<KP>::at(row_base, ks * 2));
+#pragma unroll
+                for (int u = 0; u < XB; ++u) s[u] = mfma16(y0, xf[u][1][ks], s[u]);
+#pragma unroll
+                for (int u = 0; u < XB; ++u) s[u] = mfma16(y1, xf[u][0][ks], s[u]);
             }
         }
         // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the tile
-        if constexpr (MODE != kItems) {
-            float top = -INFINITY;
+        if constexpr (!items) {
+            f32x4 bv[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 bv = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
+            for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
+            float top[XB];
+            bool grows = false;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+            for (int u = 0; u < XB; ++u) {
+                top[u] = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     // a withdrawn item's row is zeros: 0 + (-inf)
-                    s[4 * j + e] = s[4 * j + e] * sc.logit + bv[e];
-                    top = fmaxf(top, s[4 * j + e]);
+                    s[u][i] = s[u][i] * sc.logit + bv[i / 4][i % 4];
+                    top[u] = fmaxf(top[u], s[u][i]);
+                }
+                top[u] = fmaxf(top[u], __shfl_xor(top[u], 32));
+                grows |= top[u] > m_run[u];
+            }
+            if (__any(grows)) {  // rare after the first tiles: the maximum of a column grows about log(items) times
+#pragma unroll
+                for (int u = 0; u < XB; ++u) {
+                    const float m_new = fmaxf(m_run[u], top[u]);
+                    const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[u] - m_new);
+                    m_run[u] = m_new;
+                    sum[u] *= f;
+                    if constexpr (MODE == kLossGrad) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[nb][u][i] *= f;
+                    }
                 }
             }
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m_run)) {  // rare after the first tiles: the maximum of a column grows about log(items) times
-                const float m_new = fmaxf(m_run, top);
-                const float f = m_new == -INFINITY ? 1.f : exp2f(m_run - m_new);
-                m_run = m_new;
-                sum *= f;
-                if constexpr (MODE == kLossGrad) {
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+            for (int u = 0; u < XB; ++u) {
+                const float off = m_run[u] == -INFINITY ? 0.f : m_run[u] - kShift;
+                float part = 0.f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                for (int i = 0; i < 16; ++i) {
+                    s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - off);
+                    part += s[u][i];
                 }
+                sum[u] += part;
             }
-            const float off = m_run == -INFINITY ? 0.f : m_run - kShift;
-            float part = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[i] = exp2f(s[i] - off);
-                part += s[i];
-            }
-            sum += part;
         } else {
-            float part = 0.f;
+            // which of the tile's rows have their target among the wave's columns (few: one in items / (32 XB))
+            const int tg = __float_as_int(mt[2 * kTileY + lx]) - static_cast<int>(x0);
+            const bool here = __any(static_cast<uint32_t>(tg) < 32u * XB);
+            f32x4 ls[4], wv[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const f32x4 ls = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
-                const f32x4 wv = *reinterpret_cast<const f32x4*>(mt + kTileY + 8 * j + 4 * half);
-                const i32x4 tg = __builtin_bit_cast(i32x4, *reinterpret_cast<const f32x4*>(mt + 2 * kTileY + 8 * j + 4 * half));
+                ls[j] = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
+                wv[j] = *reinterpret_cast<const f32x4*>(mt + kTileY + 8 * j + 4 * half);
+            }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // a row that takes no part has lse2 = +inf and weight 0
-                    const float pr = exp2f(s[4 * j + e] * sc.logit + bias_x - ls[e]);
-                    s[4 * j + e] = wv[e] * (pr - (tg[e] == static_cast<int32_t>(x) ? 1.f : 0.f));
-                    part += s[4 * j + e];
+            for (int u = 0; u < XB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)  // a row that takes no part has lse2 = +inf and weight 0
+                    s[u][i] = __builtin_amdgcn_exp2f(s[u][i] * sc.logit + bias_x[u] - ls[i / 4][i % 4]);
+            if (here) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int at = __shfl(tg, 8 * (i / 4) + 4 * half + i % 4);
+#pragma unroll
+                    for (int u = 0; u < XB; ++u)
+                        if (at == 32 * u + lx) s[u][i] -= 1.f;
                 }
             }
-            sum += part;
+#pragma unroll
+            for (int u = 0; u < XB; ++u) {
+                float part = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[u][i] *= wv[i / 4][i % 4];
+                    part += s[u][i];
+                }
+                sum[u] += part;
+            }
         }
         if constexpr (MODE != kLoss) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                f16x8 c0, c1;
+                f16x8 c[XB][NP];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float f = s[8 * j + e];
-                    // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
-                    // product before it would round to another hi now and then
-                    if (NP == 2) asm("" : "+v"(f));
-                    c0[e] = static_cast<_Float16>(f);
-                    if (NP == 2) c1[e] = static_cast<_Float16>(f - static_cast<float>(c0[e]));
-                }
-                // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c0's.  A transposing
-                // read hands lane i of a group of 16 the column i of the 4 x 16 block whose rows its lanes address.
-                const int g = lane & 15, row = 16 * j + 4 * half + (g >> 2), col = oc0 + 16 * ((lane >> 4) & 1) + 4 * (g & 3);
+                for (int u = 0; u < XB; ++u)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float f = s[u][8 * j + e];
+                        // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
+                        // product before it would round to another hi now and then
+                        if (NP == 2) asm("" : "+v"(f));
+                        c[u][0][e] = static_cast<_Float16>(f);
+                        if (NP == 2) c[u][NP - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[u][0][e]));
+                    }
+                // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c's
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                     f16x8 yt[NP];
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
-                        const int cc = col + nb * 32;
-                        auto rd = [&](int r) {
+                        auto rd = [&](int h) {
                             return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                                tl + q * PIECE + lds_chunk<KP>(r, cc >> 3) * 8 + (cc & 7)));
+                                tl + q * PIECE * 2 + j * (32 * KP) + LdsTile<KP>::at(tr_base[h], nb * 4)));
                         };
-                        const s16x4 u = rd(row), w = rd(row + 8);
+                        const s16x4 u = rd(0), w = rd(1);
                         yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
                     }
-                    acc[nb] = mfma16(yt[0], c0, acc[nb]);
+#pragma unroll
+                    for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[0], c[u][0], acc[nb][u]);
                     if constexpr (NP == 2) {
-                        acc[nb] = mfma16(yt[0], c1, acc[nb]);
-                        acc[nb] = mfma16(yt[1], c0, acc[nb]);
+#pragma unroll
+                        for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[0], c[u][1], acc[nb][u]);
+#pragma unroll
+                        for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[1], c[u][0], acc[nb][u]);
                     }
                 }
             }
@@ -394,46 +470,77 @@ __global__ __launch_bounds__(256) void ce_main_kernel(CeArgs a) {
         __syncthreads();
     }
 
-    sum += __shfl_xor(sum, 32);
-    if constexpr (MODE != kItems) {
-        if (blockIdx.z == 0 && half == 0) {
-            a.at<float>(p.o_m)[split * p.n_pad + x] = m_run;
-            a.at<float>(p.o_s)[split * p.n_pad + x] = sum;
-        }
-        if constexpr (MODE == kLossGrad) {
-            float* O = a.at<float>(p.o_part) + (split * p.n_pad + x) * KP + oc0;
+#pragma unroll
+    for (int u = 0; u < XB; ++u) {
+        const int64_t x = x0 + 32 * u + lx;
+        const float total = sum[u] + __shfl_xor(sum[u], 32);
+        // four columns of row x of a split's sums at a time
+        auto partial = [&](int64_t rows) {
+            float* O = a.at<float>(p.o_part) + (split * rows + x) * KP + oc0;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     f32x4 o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * j + e];
+                    for (int e = 0; e < 4; ++e) o[e] = acc[nb][u][4 * j + e];
                     *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * j + 4 * half) = o;
                 }
+        };
+        if constexpr (!items) {
+            if (blockIdx.z == 0 && half == 0) {
+                a.at<float>(p.o_m)[split * p.n_pad + x] = m_run[u];
+                a.at<float>(p.o_s)[split * p.n_pad + x] = total;
+            }
+            if constexpr (MODE == kLossGrad) partial(p.n_pad);
+        } else if (p.splits_w > 1) {
+            if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = total;
+            partial(p.v_pad);
+        } else if (x < p.v) {
+            if (blockIdx.z == 0 && half == 0) a.dbias[x] = total * sc.inv_cs;
         }
-    } else if (p.splits_w > 1) {
-        if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = sum;
-        float* O = a.at<float>(p.o_part) + (split * p.v_pad + x) * KP + oc0;
+        if constexpr (items) {
+            if (p.splits_w == 1) {
+                // through LDS, so that a row's stores are contiguous: OW columns at a time, 16-byte chunk c of row r at
+                // chunk c ^ (r mod the row's chunks)
+                constexpr int OW = OC < 128 / static_cast<int>(sizeof(E)) ? OC : 128 / static_cast<int>(sizeof(E));
+                constexpr int kRow = OW * static_cast<int>(sizeof(E)), CH = kRow / 16, V = 16 / sizeof(E), ROWS = 64 / CH;
+                typedef __attribute__((ext_vector_type(4))) E e4;
+                typedef __attribute__((ext_vector_type(sizeof(E)))) int words;
+                typedef __attribute__((ext_vector_type(V))) E ev;
+                char* mine = smem + wave * 32 * kRow;
+                const bool aligned = (reinterpret_cast<uintptr_t>(a.dW) | static_cast<uintptr_t>(a.lddw * static_cast<int64_t>(sizeof(E)))) % 16 == 0;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+                for (int w0 = 0; w0 < OC; w0 += OW) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f32x4 o;
+                    for (int q = 0; q < OW / 8; ++q) {
+                        e4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * j + e];
-                *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * j + 4 * half) = o;
+                        for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][u][4 * (q % 4) + e] * sc.inv_dw);
+                        const int byte = (8 * q + 4 * half) * static_cast<int>(sizeof(E));
+                        *reinterpret_cast<words*>(mine + lx * kRow + (((byte >> 4) ^ (lx & (CH - 1))) << 4) + (byte & 15)) = __builtin_bit_cast(words, v);
+                    }
+                    wave_lds_fence();
+#pragma unroll
+                    for (int r = 0; r < 32; r += ROWS) {
+                        const int row = r + lane / CH, ch = lane % CH, col = oc0 + w0 + ch * V;
+                        const i32x4 w = *reinterpret_cast<const i32x4*>(mine + row * kRow + ((ch ^ (row & (CH - 1))) << 4));
+                        const int64_t item = x0 + 32 * u + row;
+                        if (item >= p.v) continue;
+                        E* o = static_cast<E*>(a.dW) + item * a.lddw + col;
+                        if (aligned && col + V <= p.k) {
+                            *reinterpret_cast<i32x4*>(o) = w;
+                        } else {
+                            const ev y = __builtin_bit_cast(ev, w);
+#pragma unroll
+                            for (int e = 0; e < V; ++e)
+                                if (col + e < p.k) o[e] = y[e];
+                        }
+                    }
+                    wave_lds_fence();
+                }
             }
-    } else if (x < p.v) {
-        if (blockIdx.z == 0 && half == 0) a.dbias[x] = sum * sc.inv_cs;
-        E* O = static_cast<E*>(a.dW) + x * a.lddw;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int col = oc0 + nb * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                if (col < p.k) O[col] = static_cast<E>(acc[nb][i] * sc.inv_dw);
-            }
+        }
     }
 }
 
@@ -447,24 +554,24 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     if (n >= rows) return;
     const Scal sc = *a.at<Scal>(p.o_scal);
     const bool known = row_known(a, n);
+    const float *pm = a.at<float>(p.o_m) + n, *ps = a.at<float>(p.o_s) + n;
     float m = -INFINITY, s = 0.f;
     if (known)
-        for (int i = lane; i < p.splits_f; i += 64) m = fmaxf(m, a.at<float>(p.o_m)[i * p.n_pad + n]);
+        for (int i = lane; i < p.splits_f; i += 64) m = fmaxf(m, pm[i * p.n_pad]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (known)
         for (int i = lane; i < p.splits_f; i += 64) {
-            const float mi = a.at<float>(p.o_m)[i * p.n_pad + n], si = a.at<float>(p.o_s)[i * p.n_pad + n];
-            s += m == -INFINITY ? si : si * exp2f(mi - m);
+            const float mi = pm[i * p.n_pad], si = ps[i * p.n_pad];
+            s += m == -INFINITY ? si : si * __builtin_amdgcn_exp2f(mi - m);
         }
     s = wave_sum_f32(s);
     const int32_t tg = known ? a.target[n] : 0;
     const bool there = known && item_there(a, tg);
+    const E *h = static_cast<const E*>(a.H) + n * a.ldh, *wt = static_cast<const E*>(a.W) + tg * a.ldw;
     float lt = 0.f;
     if (there)
-        for (int c = lane; c < p.k; c += 64)
-            lt = fmaf(static_cast<float>(static_cast<const E*>(a.H)[n * a.ldh + c]),
-                      static_cast<float>(static_cast<const E*>(a.W)[tg * a.ldw + c]), lt);
+        for (int c = lane; c < p.k; c += 64) lt = fmaf(static_cast<float>(h[c]), static_cast<float>(wt[c]), lt);
     lt = wave_sum_f32(lt);
     if (there && a.bias) lt += a.bias[tg];
     // every item withdrawn: m stays -inf and s is 0
@@ -486,64 +593,102 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     if (n >= p.n) return;
     E* out = static_cast<E*>(a.dH) + n * a.lddh;
     const float inv = sc.inv_w / s;
-    for (int c = lane; c < p.k; c += 64) {
-        float g = 0.f;
-        if (live) {
-            float o = 0.f;
-            for (int i = 0; i < p.splits_f; ++i)
-                o += a.at<float>(p.o_part)[(i * p.n_pad + n) * p.kp + c] * exp2f(a.at<float>(p.o_m)[i * p.n_pad + n] - m);
-            g = w * (o * inv - static_cast<float>(static_cast<const E*>(a.W)[tg * a.ldw + c]));
-        }
-        out[c] = static_cast<E>(g);
+    // four columns a lane; where a row has fewer than 256, groups of lanes share the splits
+    const int quads = p.kp / 4, lanes = quads < 64 ? quads : 64, groups = 64 / lanes, grp = lane / lanes;
+    const float* O = a.at<float>(p.o_part) + n * p.kp;
+    const int64_t step = p.n_pad * p.kp;
+    for (int c = lane % lanes * 4; c < p.kp; c += 256) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        if (live)
+#pragma unroll 8
+            for (int i = grp; i < p.splits_f; i += groups) {
+                const float f = __builtin_amdgcn_exp2f(pm[i * p.n_pad] - m);
+                const f32x4 x = *reinterpret_cast<const f32x4*>(O + i * step + c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+            }
+        for (int g = lanes; g < 64; g <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], g);
+        if (grp == 0)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < p.k) out[c + e] = static_cast<E>(live ? w * (o[e] * inv - static_cast<float>(wt[c + e])) : 0.f);
     }
 }
 
-// dW and dbias from the splits of the users' rows, in their order
+// dW and dbias from the splits of the users' rows, in their order; a thread per four columns
 template <typename E>
 __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
     const Scal sc = *a.at<Scal>(p.o_scal);
-    const int64_t total = p.v * p.k;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t v = i / p.k;
-        const int c = static_cast<int>(i % p.k);
-        float o = 0.f;
-        for (int s = 0; s < p.splits_w; ++s) o += a.at<float>(p.o_part)[(s * p.v_pad + v) * p.kp + c];
-        static_cast<E*>(a.dW)[v * a.lddw + c] = static_cast<E>(o * sc.inv_dw);
-        if (c == 0) {
-            float d = 0.f;
-            for (int s = 0; s < p.splits_w; ++s) d += a.at<float>(p.o_db)[s * p.v_pad + v];
-            a.dbias[v] = d * sc.inv_cs;
-        }
+    const int quads = p.kp / 4;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, v = i / quads;
+    const int c = static_cast<int>(i % quads) * 4;
+    if (v >= p.v || c >= p.k) return;
+    const float* O = a.at<float>(p.o_part) + v * p.kp + c;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < p.splits_w; ++s) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(O + s * p.v_pad * p.kp);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += x[e];
     }
+    E* out = static_cast<E*>(a.dW) + v * a.lddw;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c + e < p.k) out[c + e] = static_cast<E>(o[e] * sc.inv_dw);
+    if (c == 0) {
+        float d = 0.f;
+        for (int s = 0; s < p.splits_w; ++s) d += a.at<float>(p.o_db)[s * p.v_pad + v];
+        a.dbias[v] = d * sc.inv_cs;
+    }
+}
+
+template <typename E, int NP, int KP, int MODE, int XB, int WAVES, int OCC>
+void launch_tile(const CeArgs& a, hipStream_t st) {
+    const CePlan& p = a.p;
+    constexpr int NM = MODE == kItems ? 3 : 1;
+    constexpr int OC = KP < 256 ? KP : 256, row = OC * static_cast<int>(sizeof(E)) < 128 ? OC * static_cast<int>(sizeof(E)) : 128;
+    // the tiles and their rows' values; dW leaves through the same memory
+    constexpr int tiles = 2 * NP * kTileY * KP * 2 + 2 * NM * kTileY * 4, out = MODE == kItems ? WAVES * 32 * row : 0;
+    constexpr int lds = tiles > out ? tiles : out, kTileX = WAVES * 32 * XB;
+    auto kern = ce_main_kernel<E, NP, KP, MODE, XB, WAVES, OCC>;
+    if (lds > 64 * 1024)
+        RS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    const dim3 grid(static_cast<uint32_t>(ceil_div(MODE == kItems ? p.v : p.n, kTileX)),
+                    static_cast<uint32_t>(MODE == kItems ? p.splits_w : p.splits_f), MODE == kLoss ? 1u : static_cast<uint32_t>(p.z));
+    kern<<<grid, WAVES * 64, lds, st>>>(a);
+    RS_HIP(hipGetLastError());
 }
 
 template <typename E, int NP, int KP, int MODE>
 void launch_main(const CeArgs& a, hipStream_t st) {
-    const CePlan& p = a.p;
-    constexpr int NM = MODE == kItems ? 3 : 1;
-    constexpr int lds = 2 * NP * kTileY * KP * 2 + 2 * NM * kTileY * 4;
-    auto kern = ce_main_kernel<E, NP, KP, MODE>;
-    if (lds > 64 * 1024)
-        RS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    const dim3 grid(static_cast<uint32_t>((MODE == kItems ? p.v_pad : p.n_pad) / kTileX),
-                    static_cast<uint32_t>(MODE == kItems ? p.splits_w : p.splits_f), MODE == kLoss ? 1u : static_cast<uint32_t>(p.z));
-    kern<<<grid, 256, lds, st>>>(a);
-    RS_HIP(hipGetLastError());
+    constexpr int XB = KP <= (NP == 2 ? 64 : 256) ? 2 : 1;
+    launch_tile<E, NP, KP, MODE, XB, XB == 2 ? 4 : 8, 1>(a, st);
 }
 
 template <typename E, int NP>
 void launch_all(const CeArgs& a, hipStream_t st) {
     const CePlan& p = a.p;
-    int blocks = 0;
-    if (!std::is_same<E, _Float16>::value || (p.grad && a.weight)) {
-        blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), 4)));
-        ce_max_kernel<E><<<dim3(static_cast<uint32_t>(blocks), 3), 256, 0, st>>>(a);
+    const bool vec = (reinterpret_cast<uintptr_t>(a.H) | reinterpret_cast<uintptr_t>(a.W) |
+                      static_cast<uintptr_t>((a.ldh | a.ldw) * static_cast<int64_t>(sizeof(E)))) % 16 == 0;
+    auto prepare = [&](auto v) {
+        constexpr bool VEC = decltype(v)::value;
+        const int64_t step = 256 / (p.kp / 8);  // rows of a block at a time
+        int blocks = 0;
+        if (!std::is_same<E, _Float16>::value || (p.grad && a.weight)) {
+            blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), 4 * step)));
+            ce_max_kernel<E, VEC><<<dim3(static_cast<uint32_t>(blocks), 3), 256, 0, st>>>(a);
+            RS_HIP(hipGetLastError());
+        }
+        ce_pack_kernel<E, NP, VEC><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(p.n_pad + p.v_pad, step), 8192)), 256, 0, st>>>(a, blocks);
         RS_HIP(hipGetLastError());
-    }
-    const int64_t chunks = (p.n_pad + p.v_pad) * (p.kp / 8);
-    ce_pack_kernel<E, NP><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(chunks, 256), 4096)), 256, 0, st>>>(a, blocks);
-    RS_HIP(hipGetLastError());
+    };
+    if (vec)
+        prepare(std::true_type{});
+    else
+        prepare(std::false_type{});
     auto mode = [&](auto m) {
         constexpr int M = decltype(m)::value;
         switch (p.kp) {
@@ -563,7 +708,7 @@ void launch_all(const CeArgs& a, hipStream_t st) {
     if (!p.grad) return;
     mode(std::integral_constant<int, kItems>{});
     if (p.splits_w > 1) {
-        ce_items_join_kernel<E><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(p.v * p.k, 256), 8192)), 256, 0, st>>>(a);
+        ce_items_join_kernel<E><<<static_cast<uint32_t>(ceil_div(p.v * (p.kp / 4), 256)), 256, 0, st>>>(a);
         RS_HIP(hipGetLastError());
     }
 }
