@@ -42,9 +42,10 @@ extern "C" {
  *     loss, lse and its row of dH are zero.
  *   Every item withdrawn: lse -inf, loss 0, no gradient.  target withdrawn, others not: lse as defined, loss +inf,
  *     no gradient from that row.
+ *   Finite biases are held to +-2^120: the type's lowest value is no withdrawal.
  * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
- * (hi + lo), so an element keeps 2^-24 of itself or 2^-39 of the matrix's largest element, whichever is more;
- * RS_TYPE_BF16 exactly down to 2^-28 of the largest, and to 2^-39 of it below.
+ * (hi + lo), so an element keeps 2^-24 of itself or 2^-38 of the matrix's largest element, whichever is more;
+ * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below.
  * n_items < 2^31, n_rows < 2^31. */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);

@@ -4,7 +4,7 @@
 //   forward: x = users' rows, y = items.  S[y, x] = W_y . H_x; a running maximum m_x and sum s_x of 2^(l2 - m_x), l2 the
 //     logit in base 2, and (for the gradient) O_x = sum_y 2^(l2 - m_x) W_y, all three rescaled when m_x grows.  So one
 //     pass over the catalogue gives lse and dH = weight (O / s - W_target).
-//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - lse2) - [target]) and dW_x += sum_y c H_y.
+//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - m_y) / s_y - [target]) and dW_x += sum_y c H_y.
 // Both are one kernel: S = Y X^T, then acc[k, x] += Y^T f(S).  S comes out of the matrix unit with x over lanes and y
 // over registers, which is (up to an order of y, the same for both operands) what the second product takes as its
 // second operand: f(S) never leaves the registers.  Its first operand Y^T comes from the same LDS tile as Y by
@@ -25,13 +25,36 @@
 namespace rs {
 namespace {
 
-constexpr int kTileX = 256;      // stationary rows of a workgroup: a multiple of what its waves hold
-constexpr int kTileY = 32;       // streamed rows of a step
+constexpr int kPad = 256;        // rows are padded to this: a multiple of what a workgroup holds or a stage streams
+constexpr int kTileY = 128;      // streamed rows are split over workgroups in multiples of this
 constexpr int kMaxBlocks = 1024;  // blocks of the maxima pass at most, per matrix
-constexpr float kShift = 14.f;   // p is held as 2^14 p: fp16's range below 1 is short
+// p = 2^(l2 - m) is held as 2^shift_of(m) p (fp16's range below 1 is short; beside a large m the shift would be lost in
+// the difference), and m may lag the maximum by kLag: moving it at each new maximum costs a pass over the sums in most
+// tiles (32 columns a wave, each with its own records)
+constexpr float kLag = 8.f;
+__device__ __forceinline__ float shift_of(float m) { return fabsf(m) < 32768.f ? 7.f : 0.f; }
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 enum Mode { kLoss = 0, kLossGrad = 1, kItems = 2 };
+
+// Shape of a workgroup: waves of 32 stationary rows each, streamed rows of a stage (between two barriers) in blocks of
+// 32, waves per SIMD asked of the compiler.  Measured on 8192 x 26744 x 128 and 1024 x 1e6 x 256 (bf16), 4096 x 3706 x 100
+// (fp32), times of the two passes (users / items):
+//   KP = 128, one piece: 8 waves 148 / 196 us, 4 waves 161 / 184; stages of 4 blocks 135 for the users' pass, 2 for the
+//     items' (4 spill)
+//   KP = 256, one piece: 8 waves 1255 / 1536 us, 4 waves 1444 / 1617 (8 waves read the streamed tile once for 256 rows)
+//   KP = 128, two pieces: 4 waves 39 / 41 us, 8 waves 42 / 45
+//   wider: the row and its sums take more than half the registers: one wave per SIMD
+struct Shape {
+    int waves, blocks, occ;
+};
+constexpr Shape shape_for(int np, int kp, int mode) {
+    if (np * kp >= 512) return {4, 1, 1};
+    if (np * kp == 256) return np == 1 ? Shape{8, 1, 2} : Shape{4, 1, 2};
+    if (np * kp == 128) return np == 2 ? Shape{4, 2, 2} : mode == kItems ? Shape{4, 2, 2} : Shape{8, 4, 2};
+    return {4, 2, 2};
+}
+
 
 // Device scalars (ws): the powers of two that scale H, W and the weights, and what undoes them.
 struct Scal {
@@ -46,7 +69,7 @@ struct CePlan {
     int64_t n, v, n_pad, v_pad;
     int32_t k, kp, np, oc, z, type, grad;
     int32_t splits_f, tiles_f, splits_w, tiles_w;  // splits of the streamed rows and their tiles each
-    int64_t o_max, o_scal, o_h, o_w, o_bias, o_m, o_s, o_lse2, o_wv, o_tgt, o_part, o_db, bytes;
+    int64_t o_max, o_scal, o_h, o_w, o_bias, o_m, o_s, o_row, o_part, o_db, bytes;
 };
 
 CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
@@ -56,16 +79,32 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
     p.np = type == RS_TYPE_F32 ? 2 : 1;
     p.oc = std::min(p.kp, 256);
     p.z = p.kp / p.oc;
-    p.n_pad = round_up(n, kTileX);
-    p.v_pad = round_up(v, kTileX);
-    auto split = [](int64_t tx, int64_t ty, int32_t* splits, int32_t* tiles) {
-        const int64_t want = std::max<int64_t>(1, ceil_div(512, tx));        // two workgroups per CU
-        int64_t per = std::max<int64_t>(ceil_div(ty, want), std::min<int64_t>(ty, 2));
-        *tiles = static_cast<int32_t>(per);
-        *splits = static_cast<int32_t>(ceil_div(ty, per));
+    p.n_pad = round_up(n, kPad);
+    p.v_pad = round_up(v, kPad);
+    // Splits of the streamed rows: enough to fill the chip, against the sums that every split writes and the join reads.
+    // In microseconds, by the measured rates of the passes: a tile of kTileY rows at 3.4 TFLOP/s a CU where one
+    // workgroup has it (whole rounds of 256 workgroups), 2.4 where two share it (they end at different times: half a
+    // workgroup's time is lost at the end), 3 for a workgroup's start and end, the sums at 8 TB/s.
+    auto split = [&](int64_t rows_x, int64_t rows_y, int mode, int32_t* splits, int32_t* tiles) {
+        const Shape sh = shape_for(p.np, p.kp, mode);
+        const int64_t tx = ceil_div(rows_x, 32 * sh.waves) * p.z, ty = ceil_div(rows_y, kTileY);
+        const bool alone = sh.waves == 8 || sh.occ == 1;
+        const double tile = static_cast<double>(kTileY) * 32 * sh.waves * (p.kp + p.oc) * 2 * (p.np == 2 ? 3 : 1) / (alone ? 3.4e6 : 2.4e6);
+        const double sums = static_cast<double>(rows_x) * p.kp * 8 / 8e6;
+        double best = 0.0;
+        for (int64_t s = 1; s <= ty && (s == 1 || tx * s <= 4096); ++s) {
+            const int64_t per = ceil_div(ty, s);
+            if (ceil_div(ty, per) != s) continue;
+            const double one = static_cast<double>(per) * tile;
+            double cost = alone ? static_cast<double>(ceil_div(tx * s, 256)) * (one + 3.0)
+                                : static_cast<double>(std::max<int64_t>(tx * s, 256)) / 256 * (one + 2.0) + 0.5 * one;
+            if (s > 1 || mode != kItems) cost += static_cast<double>(s) * sums;
+            if (s > 1 && mode == kItems) cost += 5.0;  // the join's launch
+            if (s == 1 || cost < best) best = cost, *splits = static_cast<int32_t>(s), *tiles = static_cast<int32_t>(per);
+        }
     };
-    split(p.n_pad / kTileX, p.v_pad / kTileY, &p.splits_f, &p.tiles_f);
-    split(p.v_pad / kTileX, p.n_pad / kTileY, &p.splits_w, &p.tiles_w);
+    split(n, v, kLossGrad, &p.splits_f, &p.tiles_f);
+    split(v, n, kItems, &p.splits_w, &p.tiles_w);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -80,9 +119,7 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
     p.o_m = take(p.splits_f * p.n_pad * 4);
     p.o_s = take(p.splits_f * p.n_pad * 4);
     if (grad) {
-        p.o_lse2 = take(p.n_pad * 4);
-        p.o_wv = take(p.n_pad * 4);
-        p.o_tgt = take(p.n_pad * 4);
+        p.o_row = take(4 * p.n_pad * 4);
         const int64_t of = p.splits_f * p.n_pad * p.kp * 4, ow = p.splits_w > 1 ? p.splits_w * p.v_pad * p.kp * 4 : 0;
         p.o_part = take(std::max(of, ow));  // O partials, read before dW's are written
         p.o_db = take(p.splits_w > 1 ? p.splits_w * p.v_pad * 4 : 0);
@@ -110,6 +147,9 @@ struct CeArgs {
 __device__ __forceinline__ bool row_known(const CeArgs& a, int64_t n) {
     return n < a.p.n && static_cast<uint64_t>(static_cast<int64_t>(a.target[n])) < static_cast<uint64_t>(a.p.v);
 }
+__device__ __forceinline__ float bounded_bias(float b) {
+    return fabsf(b) < INFINITY ? fminf(fmaxf(b, -0x1p120f), 0x1p120f) : b;
+}
 __device__ __forceinline__ bool item_there(const CeArgs& a, int64_t v) {
     return v < a.p.v && !(a.bias && a.bias[v] == -INFINITY);
 }
@@ -132,85 +172,90 @@ __device__ __forceinline__ void load8(const E* row, int c, int k, float (&v)[8])
     }
 }
 
+// 2^e with max * 2^e in [2^13, 2^14), e bounded so that the power and its inverse are normal numbers
+__device__ __forceinline__ float scale_for(uint32_t max_bits) {
+    if (max_bits == 0) return 1.f;
+    const int e = 13 + 127 - static_cast<int>(max_bits >> 23);
+    return __uint_as_float(static_cast<uint32_t>(min(max(e, -100), 100) + 127) << 23);
+}
+
+__device__ __forceinline__ Scal scales(float hs, float wsc, float cs) {
+    Scal s;
+    s.hs = hs, s.wsc = wsc, s.cs = cs;
+    s.logit = kLog2e / hs / wsc;
+    s.inv_w = 1.f / wsc;
+    s.inv_dw = 1.f / cs / hs;
+    s.inv_cs = 1.f / cs;
+    return s;
+}
+
+__device__ __forceinline__ void see_largest(uint32_t& m, float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+    if (b < 0x7F800000u && b > m) m = b;
+}
+
 // ---- largest finite magnitudes of H, W and the weights (blockIdx.y = 0, 1, 2), one value per block ----------------
 template <typename E, bool VEC>
 __global__ __launch_bounds__(256) void ce_max_kernel(CeArgs a) {
+    const CePlan& p = a.p;
     const int which = blockIdx.y;
     uint32_t m = 0;
-    auto see = [&](float x) {
-        const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-        if (b < 0x7F800000u && b > m) m = b;
-    };
     if (which < 2) {
         const E* X = static_cast<const E*>(which ? a.W : a.H);
-        const int64_t rows = which ? a.p.v : a.p.n, ld = which ? a.ldw : a.ldh;
-        const int lanes = a.p.kp / 8, at = threadIdx.x / lanes, c = threadIdx.x % lanes * 8, step = 256 / lanes;
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * step + at; r < rows; r += static_cast<int64_t>(gridDim.x) * step) {
-            if (c >= a.p.k || !(which ? item_there(a, r) : row_known(a, r))) continue;
+        const int64_t rows = which ? p.v : p.n, ld = which ? a.ldw : a.ldh;
+        const int lanes = p.kp / 8, at = threadIdx.x / lanes, c = threadIdx.x % lanes * 8;
+        const int64_t step = static_cast<int64_t>(gridDim.x) * (256 / lanes);
+#pragma unroll 4
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / lanes) + at; r < rows; r += step) {
+            if (c >= p.k) continue;
             float v[8];
-            load8<E, VEC>(X + r * ld, c, a.p.k, v);
+            load8<E, VEC>(X + r * ld, c, p.k, v);
+            uint32_t t = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) see(v[e]);
+            for (int e = 0; e < 8; ++e) see_largest(t, v[e]);
+            if (t > m && (which ? item_there(a, r) : row_known(a, r))) m = t;  // (looked up for new records only)
         }
     } else if (a.weight) {
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < a.p.n; r += static_cast<int64_t>(gridDim.x) * 256)
-            if (row_known(a, r)) see(a.weight[r]);
+        for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < p.n; r += static_cast<int64_t>(gridDim.x) * 256)
+            if (row_known(a, r)) see_largest(m, a.weight[r]);
     }
     m = wave_max_u32(m);
     __shared__ uint32_t sm[4];
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0)
-        a.at<uint32_t>(a.p.o_max)[which * kMaxBlocks + blockIdx.x] = max(max(sm[0], sm[1]), max(sm[2], sm[3]));
-}
-
-// 2^e with max * 2^e in [2^13, 2^14), e bounded so that the power and its inverse are normal numbers
-__device__ __forceinline__ float scale_for(uint32_t max_bits) {
-    if (max_bits == 0) return 1.f;
-    int e = static_cast<int>(max_bits >> 23) - 127;
-    e = 13 - e;
-    e = min(max(e, -100), 100);
-    return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+    if (threadIdx.x == 0) a.at<uint32_t>(p.o_max)[which * kMaxBlocks + blockIdx.x] = max(max(sm[0], sm[1]), max(sm[2], sm[3]));
 }
 
 // ---- packing: a thread per eight columns ---------------------------------------------------------------------------
 template <typename E, int NP, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) {
+    constexpr bool kScaled = !std::is_same<E, _Float16>::value;
+    const CePlan& p = a.p;
     __shared__ uint32_t sm[3];
     if (threadIdx.x < 192) {
         const int which = threadIdx.x >> 6;
         uint32_t m = 0;
-        for (int i = threadIdx.x & 63; i < max_blocks; i += 64) m = max(m, a.at<uint32_t>(a.p.o_max)[which * kMaxBlocks + i]);
+        for (int i = threadIdx.x & 63; i < max_blocks; i += 64) m = max(m, a.at<uint32_t>(p.o_max)[which * kMaxBlocks + i]);
         m = wave_max_u32(m);
         if ((threadIdx.x & 63) == 0) sm[which] = m;
     }
     __syncthreads();
-    constexpr bool kScaled = !std::is_same<E, _Float16>::value;
     const float hs = kScaled ? scale_for(sm[0]) : 1.f, wsc = kScaled ? scale_for(sm[1]) : 1.f;
     // coefficients c = weight (p - [target]): |c| <= |weight| cs < 2^14
-    const float cs = scale_for(a.weight ? sm[2] : 0x3F800000u);
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        Scal s;
-        s.hs = hs, s.wsc = wsc, s.cs = cs;
-        s.logit = kLog2e / hs / wsc;
-        s.inv_w = 1.f / wsc;
-        s.inv_dw = 1.f / cs / hs;
-        s.inv_cs = 1.f / cs;
-        *a.at<Scal>(a.p.o_scal) = s;
-    }
-    const int lanes = a.p.kp / 8, at = threadIdx.x / lanes, c0 = threadIdx.x % lanes * 8, step = 256 / lanes;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * step + at; row < a.p.n_pad + a.p.v_pad; row += static_cast<int64_t>(gridDim.x) * step) {
-        const bool w = row >= a.p.n_pad;
-        const int64_t r = w ? row - a.p.n_pad : row;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.at<Scal>(p.o_scal) = scales(hs, wsc, scale_for(a.weight ? sm[2] : 0x3F800000u));
+    const int lanes = p.kp / 8, at = threadIdx.x / lanes, c0 = threadIdx.x % lanes * 8, step = 256 / lanes;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * step + at; row < p.n_pad + p.v_pad; row += static_cast<int64_t>(gridDim.x) * step) {
+        const bool w = row >= p.n_pad;
+        const int64_t r = w ? row - p.n_pad : row;
         const bool there = w ? item_there(a, r) : row_known(a, r);
         if (w && c0 == 0) {
-            const float b = r < a.p.v ? (a.bias ? a.bias[r] : 0.f) : -INFINITY;
-            a.at<float>(a.p.o_bias)[r] = b * kLog2e;
+            // base-2 biases.  Finite ones are held to +-2^120: the type's lowest value is no withdrawal.
+            const float b = r < p.v ? (a.bias ? a.bias[r] : 0.f) : -INFINITY;
+            a.at<float>(p.o_bias)[r] = bounded_bias(b) * kLog2e;
         }
-        const E* src = static_cast<const E*>(w ? a.W : a.H) + (there ? r * (w ? a.ldw : a.ldh) : 0);
-        const float sc = w ? wsc : hs;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (there) load8<E, VEC>(src, c0, a.p.k, v);
+        if (there) load8<E, VEC>(static_cast<const E*>(w ? a.W : a.H) + r * (w ? a.ldw : a.ldh), c0, p.k, v);
+        const float sc = w ? wsc : hs;
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -218,103 +263,96 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
             hi[e] = static_cast<_Float16>(y);
             if (NP == 2) lo[e] = static_cast<_Float16>(y - static_cast<float>(hi[e]));
         }
-        _Float16* dst = a.at<_Float16>(w ? a.p.o_w : a.p.o_h) + r * a.p.kp + c0;
+        _Float16* dst = a.at<_Float16>(w ? p.o_w : p.o_h) + r * p.kp + c0;
         *reinterpret_cast<f16x8*>(dst) = hi;
-        if (NP == 2) *reinterpret_cast<f16x8*>(dst + (w ? a.p.v_pad : a.p.n_pad) * a.p.kp) = lo;
+        if (NP == 2) *reinterpret_cast<f16x8*>(dst + (w ? p.v_pad : p.n_pad) * p.kp) = lo;
     }
 }
 
 // ---- the products --------------------------------------------------------------------------------------------------
 __device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// 16-byte chunk c of row r of an LDS tile sits at chunk c ^ (r mod 16) of the row (fewer where a row has fewer
-// chunks): the row-wise and the transposing reads both spread over the banks.  Byte offset: what a lane adds is one
-// base, the constant part of c goes in by XOR (bits the rows do not reach: by addition), so a few registers hold all
-// the addresses of a tile.
+// 16-byte chunk c of row r of an LDS tile sits at chunk c ^ mix(r), the row's low three bits rotated.  A row-wise read (8
+// rows, one chunk at a time) and a transposing one (4 rows, two neighbouring chunks) then both meet every bank once; c ^ (r mod 16) had neighbouring rows share their chunk pairs
+// (half of the LDS cycles were conflicts).  Byte offset: what a lane adds is one base, the constant part of c goes in
+// by XOR (bits the rows do not reach: by addition), so a few registers hold all the addresses of a tile.
 template <int KP>
 struct LdsTile {
     static constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;
-    static __device__ __forceinline__ int base(int row, int c) { return row * (KP * 2) + ((c ^ (row & M)) & M) * 16 + (c & ~M) * 16; }
+    static __device__ __forceinline__ int mix(int row) {
+        return KP == 32 ? (row & 2) | ((row >> 2) & 1) : (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & M;
+    }
+    static __device__ __forceinline__ int base(int row, int c) { return row * (KP * 2) + ((c ^ mix(row)) & M) * 16 + (c & ~M) * 16; }
     // base(row, c) with the constant dc joined to c (no common bits)
     static __device__ __forceinline__ int at(int base, int dc) { return (base ^ ((dc & M) * 16)) + (dc & ~M) * 16; }
 };
-
-// A wave holds XB blocks of 32 stationary rows: each fragment of Y read from LDS feeds XB products (one block reads 1 KB of
-// LDS per 32-cycle MFMA in each of the four SIMDs: all that LDS gives).
+// Each wave holds 32 stationary rows; a stage of streamed rows passes through LDS, the next one on its way in registers.
 // MODE kLoss / kLossGrad: x = users' rows, y = items; kItems: x = items, y = users' rows.
-template <typename E, int NP, int KP, int MODE, int XB, int WAVES, int OCC>
+template <typename E, int NP, int KP, int MODE, int WAVES, int SUB, int OCC>
 __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
 #pragma clang fp contract(fast)
+    constexpr bool items = MODE == kItems;
     constexpr int THREADS = WAVES * 64;
     constexpr int OC = KP < 256 ? KP : 256, NB = MODE == kLoss ? 1 : OC / 32, KS = KP / 16, C = KP / 8;
-    constexpr int PIECE = kTileY * KP;                     // elements of one piece of a tile
-    constexpr int CHUNKS = kTileY * C * NP, PER = (CHUNKS + THREADS - 1) / THREADS;
-    constexpr int NM = MODE == kItems ? 3 : 1;             // values per streamed row
+    constexpr int ROWS = 32 * SUB;                         // rows of a stage
+    constexpr int PIECE = ROWS * KP;                       // elements of one piece of a stage
+    constexpr int CHUNKS = ROWS * C * NP, PER = (CHUNKS + THREADS - 1) / THREADS;
+    constexpr int NM = items ? 4 : 1;                      // values per streamed row: bias, or m, weight / s, target, weight
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    // smem: [2][NP][kTileY][KP] fp16
-    float* meta = reinterpret_cast<float*>(smem + 2 * NP * PIECE * 2);       // [2][NM][kTileY]
+    // smem: [2][NP][ROWS][KP] fp16
+    float* meta = reinterpret_cast<float*>(smem + 2 * NP * PIECE * 2);  // [2][NM][ROWS]
 
     const CePlan& p = a.p;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lx = lane & 31, half = lane >> 5;
-    constexpr bool items = MODE == kItems;
     const int64_t x_pad = items ? p.v_pad : p.n_pad, y_pad = items ? p.n_pad : p.v_pad;
     const _Float16* X = a.at<_Float16>(items ? p.o_w : p.o_h);
     const _Float16* Y = a.at<_Float16>(items ? p.o_h : p.o_w);
-    const int per = items ? p.tiles_w : p.tiles_f;
+    const int per = (items ? p.tiles_w : p.tiles_f) * (kTileY / ROWS);
     const int split = blockIdx.y, oc0 = blockIdx.z * OC;
-    const int64_t x0 = (static_cast<int64_t>(blockIdx.x) * WAVES + wave) * (32 * XB);  // the wave's first row
-    const int t0 = split * per, t1 = static_cast<int>(min<int64_t>(y_pad / kTileY, t0 + per));
+    const int64_t x0 = (static_cast<int64_t>(blockIdx.x) * WAVES + wave) * 32, x = x0 + lx;  // the wave's first row, the lane's
+    const int t0 = split * per, t1 = static_cast<int>(min<int64_t>(((items ? p.n : p.v) + ROWS - 1) / ROWS, t0 + per));
     const Scal sc = *a.at<Scal>(p.o_scal);
 
-    f16x8 xf[XB][NP][KS];
+    f16x8 xf[NP][KS];
 #pragma unroll
-    for (int u = 0; u < XB; ++u)
+    for (int q = 0; q < NP; ++q)
 #pragma unroll
-        for (int q = 0; q < NP; ++q)
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-                xf[u][q][s] = *reinterpret_cast<const f16x8*>(X + (q * x_pad + x0 + 32 * u + lx) * KP + s * 16 + half * 8);
+        for (int s = 0; s < KS; ++s) xf[q][s] = *reinterpret_cast<const f16x8*>(X + (q * x_pad + x) * KP + s * 16 + half * 8);
 
+    // A stage is contiguous in memory, piece by piece: chunk i THREADS + thread of it is this thread's i-th.
+    static_assert(CHUNKS % THREADS == 0 && (ROWS * C) % THREADS == 0, "a thread's i-th chunk is in one piece for all threads");
     f16x8 stage[PER];
     float stage_meta = 0.f;
     auto fetch = [&](int t) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int ch = i * THREADS + threadIdx.x;
-            if (CHUNKS % THREADS == 0 || ch < CHUNKS) {
-                const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
-                stage[i] = *reinterpret_cast<const f16x8*>(Y + (q * y_pad + static_cast<int64_t>(t) * kTileY + r) * KP + c * 8);
-            }
+            constexpr int per_piece = ROWS * C / THREADS;
+            const char* src = reinterpret_cast<const char*>(Y + (i / per_piece * y_pad + static_cast<int64_t>(t) * ROWS) * KP) + i % per_piece * (THREADS * 16);
+            stage[i] = *reinterpret_cast<const f16x8*>(src + threadIdx.x * 16u);
         }
-        if (threadIdx.x < NM * kTileY) {
-            const int64_t y = static_cast<int64_t>(t) * kTileY + (threadIdx.x & 31);
-            const int which = threadIdx.x >> 5;
-            stage_meta = a.at<float>(!items ? p.o_bias : which == 0 ? p.o_lse2 : which == 1 ? p.o_wv : p.o_tgt)[y];
+        if (threadIdx.x < NM * ROWS) {
+            const int64_t y = static_cast<int64_t>(t) * ROWS + threadIdx.x % ROWS;
+            const int which = threadIdx.x / ROWS;
+            stage_meta = a.at<float>(!items ? p.o_bias : p.o_row + which * p.n_pad * 4)[y];
         }
     };
+    constexpr int LINES_T = THREADS / C;  // rows that the threads' chunks cover
+    const int put_base = LdsTile<KP>::base(threadIdx.x / C, threadIdx.x % C);
     auto put = [&](int b) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int ch = i * THREADS + threadIdx.x;
-            if (CHUNKS % THREADS == 0 || ch < CHUNKS) {
-                const int q = ch / (kTileY * C), r = ch / C % kTileY, c = ch % C;
-                *reinterpret_cast<f16x8*>(smem + (b * NP + q) * PIECE * 2 + LdsTile<KP>::base(r, c)) = stage[i];
-            }
+            // rows a multiple of 16 further have the same chunk order
+            const int r = i * LINES_T, at = LINES_T % 16 == 0 ? put_base + r * KP * 2 : LdsTile<KP>::base(r + threadIdx.x / C, threadIdx.x % C);
+            *reinterpret_cast<f16x8*>(smem + b * NP * PIECE * 2 + at) = stage[i];
         }
-        if (threadIdx.x < NM * kTileY) meta[b * NM * kTileY + threadIdx.x] = stage_meta;
+        if (threadIdx.x < NM * ROWS) meta[b * NM * ROWS + threadIdx.x] = stage_meta;
     };
 
-    f32x16 acc[NB][XB];
+    f32x16 acc[NB];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int u = 0; u < XB; ++u) acc[b][u] = f32x16{0};
-    float m_run[XB], sum[XB], bias_x[XB];
-#pragma unroll
-    for (int u = 0; u < XB; ++u) {
-        m_run[u] = -INFINITY, sum[u] = 0.f;
-        bias_x[u] = items ? a.at<float>(p.o_bias)[x0 + 32 * u + lx] : 0.f;
-    }
+    for (int b = 0; b < NB; ++b) acc[b] = f32x16{0};
+    float m_run = -INFINITY, sum = 0.f;
+    const float bias_x = items ? a.at<float>(p.o_bias)[x] : 0.f;
 
     // row-wise reads: row lx, chunk half + 2 ks.  Transposing reads hand lane i of a group of 16 the column i of the
     // 4 x 16 block whose rows its lanes address: row 4 half + (i / 4) of 8, chunk 2 (group mod 2) + (i mod 4) / 2.
@@ -322,224 +360,203 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     const int tr_row = 4 * half + (g4 >> 2), tr_chunk = oc0 / 8 + 2 * ((lane >> 4) & 1) + ((g4 & 3) >> 1);
     const int tr_base[2] = {LdsTile<KP>::base(tr_row, tr_chunk) + (g4 & 1) * 8, LdsTile<KP>::base(tr_row + 8, tr_chunk) + (g4 & 1) * 8};
 
+    // 32 streamed rows: the byte offset of their LDS tile and their values
+    auto block = [&](int tile, const float* mt) {
+        // the tile's offset has none of the bits that the chunks are mixed in: it joins the bases.  Wide rows take the
+        // addresses anew for every block, or the compiler keeps all of them in registers and spills others (KP = 256: 168
+        // bytes, 1221 / 2067 us against 1072 / 1215); narrow ones keep them (KP = 128: 126 us against 154)
+        int rb = row_base + tile, tb[2] = {tr_base[0] + tile, tr_base[1] + tile};
+        if (KP >= 256) asm volatile("" : "+v"(rb), "+v"(tb[0]), "+v"(tb[1]));
+        f32x16 s = f32x16{0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const f16x8 y0 = *reinterpret_cast<const f16x8*>(smem + LdsTile<KP>::at(rb, ks * 2));
+            s = mfma16(y0, xf[0][ks], s);
+            if constexpr (NP == 2) {
+                const f16x8 y1 = *reinterpret_cast<const f16x8*>(smem + PIECE * 2 + LdsTile<KP>::at(rb, ks * 2));
+                s = mfma16(y0, xf[1][ks], s);
+                s = mfma16(y1, xf[0][ks], s);
+            }
+        }
+        // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the block
+        float off = 0.f;
+        bool here = false;
+        int tg = 0;
+        if constexpr (!items) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 bv = *reinterpret_cast<const f32x4*>(mt + 8 * q + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // a withdrawn item's row is zeros: 0 + (-inf)
+                    s[4 * q + e] = s[4 * q + e] * sc.logit + bv[e];
+                    top = fmaxf(top, s[4 * q + e]);
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m_run + kLag)) {  // the first block, and rarely after it
+                const float m_new = top > m_run + kLag ? top : m_run;
+                const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) + (shift_of(m_new) - shift_of(m_run)));
+                m_run = m_new;
+                sum *= f;
+                if constexpr (MODE == kLossGrad)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+            }
+            off = m_run == -INFINITY ? 0.f : m_run - shift_of(m_run);
+        } else {
+            // which of the rows have their target among the wave's columns (few: one in items / 32)
+            tg = __float_as_int(mt[2 * ROWS + lx]) - static_cast<int>(x0);
+            here = __any(static_cast<uint32_t>(tg) < 32u);
+        }
+        // f(S) and its product.  Wide rows leave few registers: 16 rows of the block at a time (KP = 256: the items'
+        // pass 2001 -> 1536 us); otherwise all 32, which gives the scheduler more to run beside the products (KP = 128:
+        // 145 us against 166)
+        constexpr int HALVES = NP * KP >= 256 ? 2 : 1, Q = 4 / HALVES;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+            if constexpr (items) {
+#pragma unroll
+                for (int q = Q * h; q < Q * h + Q; ++q) {
+                    const f32x4 m = *reinterpret_cast<const f32x4*>(mt + 8 * q + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)  // a row that takes no part has m = +inf and weight 0
+                        s[4 * q + e] = __builtin_amdgcn_exp2f((s[4 * q + e] * sc.logit + bias_x) - m[e]);  // (rounded as the users' pass rounds it)
+                }
+#pragma unroll
+                for (int q = Q * h; q < Q * h + Q; ++q) {
+                    const f32x4 ws = *reinterpret_cast<const f32x4*>(mt + ROWS + 8 * q + 4 * half);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * q + e] *= ws[e];
+                }
+                if (here) {
+#pragma unroll
+                    for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) {
+                        const int row = 8 * (i / 4) + 4 * half + i % 4;
+                        if (__shfl(tg, row) == lx) s[i] -= mt[3 * ROWS + row];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - off);
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) part += s[i];
+            sum += part;
+            if constexpr (MODE != kLoss) {
+#pragma unroll
+                for (int j = 2 * h / HALVES; j < 2 * (h + 1) / HALVES; ++j) {
+                    f16x8 c[NP];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float f = s[8 * j + e];
+                        // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
+                        // product before it would round to another hi now and then
+                        if (NP == 2) asm("" : "+v"(f));
+                        c[0][e] = static_cast<_Float16>(f);
+                        if (NP == 2) c[NP - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[0][e]));
+                    }
+                    // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c's
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        f16x8 yt[NP];
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) {
+                            auto rd = [&](int k) {
+                                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+                                    smem + q * PIECE * 2 + j * (32 * KP) + LdsTile<KP>::at(tb[k], nb * 4)));
+                            };
+                            const s16x4 u = rd(0), w = rd(1);
+                            yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
+                        }
+                        acc[nb] = mfma16(yt[0], c[0], acc[nb]);
+                        if constexpr (NP == 2) {
+                            acc[nb] = mfma16(yt[0], c[1], acc[nb]);
+                            acc[nb] = mfma16(yt[1], c[0], acc[nb]);
+                        }
+                    }
+                }
+            }
+        }
+    };
+
     fetch(t0);
     put(0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int b = (t - t0) & 1;
         if (t + 1 < t1) fetch(t + 1);
-        const char* tl = smem + b * NP * PIECE * 2;
-        const float* mt = meta + b * NM * kTileY;
-
-        f32x16 s[XB];
 #pragma unroll
-        for (int u = 0; u < XB; ++u) s[u] = f32x16{0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const f16x8 y0 = *reinterpret_cast<const f16x8*>(tl + LdsTile<KP>::at(row_base, ks * 2));
-#pragma unroll
-            for (int u = 0; u < XB; ++u) s[u] = mfma16(y0, xf[u][0][ks], s[u]);
-            if constexpr (NP == 2) {
-                const f16x8 y1 = *reinterpret_cast<const f16x8*>(tl + PIECE * 2 + LdsTile<KP>::at(row_base, ks * 2));
-#pragma unroll
-                for (int u = 0; u < XB; ++u) s[u] = mfma16(y0, xf[u][1][ks], s[u]);
-#pragma unroll
-                for (int u = 0; u < XB; ++u) s[u] = mfma16(y1, xf[u][0][ks], s[u]);
-            }
-        }
-        // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the tile
-        if constexpr (!items) {
-            f32x4 bv[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
-            float top[XB];
-            bool grows = false;
-#pragma unroll
-            for (int u = 0; u < XB; ++u) {
-                top[u] = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    // a withdrawn item's row is zeros: 0 + (-inf)
-                    s[u][i] = s[u][i] * sc.logit + bv[i / 4][i % 4];
-                    top[u] = fmaxf(top[u], s[u][i]);
-                }
-                top[u] = fmaxf(top[u], __shfl_xor(top[u], 32));
-                grows |= top[u] > m_run[u];
-            }
-            if (__any(grows)) {  // rare after the first tiles: the maximum of a column grows about log(items) times
-#pragma unroll
-                for (int u = 0; u < XB; ++u) {
-                    const float m_new = fmaxf(m_run[u], top[u]);
-                    const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[u] - m_new);
-                    m_run[u] = m_new;
-                    sum[u] *= f;
-                    if constexpr (MODE == kLossGrad) {
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[nb][u][i] *= f;
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < XB; ++u) {
-                const float off = m_run[u] == -INFINITY ? 0.f : m_run[u] - kShift;
-                float part = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - off);
-                    part += s[u][i];
-                }
-                sum[u] += part;
-            }
-        } else {
-            // which of the tile's rows have their target among the wave's columns (few: one in items / (32 XB))
-            const int tg = __float_as_int(mt[2 * kTileY + lx]) - static_cast<int>(x0);
-            const bool here = __any(static_cast<uint32_t>(tg) < 32u * XB);
-            f32x4 ls[4], wv[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                ls[j] = *reinterpret_cast<const f32x4*>(mt + 8 * j + 4 * half);
-                wv[j] = *reinterpret_cast<const f32x4*>(mt + kTileY + 8 * j + 4 * half);
-            }
-#pragma unroll
-            for (int u = 0; u < XB; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)  // a row that takes no part has lse2 = +inf and weight 0
-                    s[u][i] = __builtin_amdgcn_exp2f(s[u][i] * sc.logit + bias_x[u] - ls[i / 4][i % 4]);
-            if (here) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int at = __shfl(tg, 8 * (i / 4) + 4 * half + i % 4);
-#pragma unroll
-                    for (int u = 0; u < XB; ++u)
-                        if (at == 32 * u + lx) s[u][i] -= 1.f;
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < XB; ++u) {
-                float part = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[u][i] *= wv[i / 4][i % 4];
-                    part += s[u][i];
-                }
-                sum[u] += part;
-            }
-        }
-        if constexpr (MODE != kLoss) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                f16x8 c[XB][NP];
-#pragma unroll
-                for (int u = 0; u < XB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float f = s[u][8 * j + e];
-                        // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
-                        // product before it would round to another hi now and then
-                        if (NP == 2) asm("" : "+v"(f));
-                        c[u][0][e] = static_cast<_Float16>(f);
-                        if (NP == 2) c[u][NP - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[u][0][e]));
-                    }
-                // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c's
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    f16x8 yt[NP];
-#pragma unroll
-                    for (int q = 0; q < NP; ++q) {
-                        auto rd = [&](int h) {
-                            return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                                tl + q * PIECE * 2 + j * (32 * KP) + LdsTile<KP>::at(tr_base[h], nb * 4)));
-                        };
-                        const s16x4 u = rd(0), w = rd(1);
-                        yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
-                    }
-#pragma unroll
-                    for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[0], c[u][0], acc[nb][u]);
-                    if constexpr (NP == 2) {
-#pragma unroll
-                        for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[0], c[u][1], acc[nb][u]);
-#pragma unroll
-                        for (int u = 0; u < XB; ++u) acc[nb][u] = mfma16(yt[1], c[u][0], acc[nb][u]);
-                    }
-                }
-            }
-        }
+        for (int sub = 0; sub < SUB; ++sub) block(b * NP * PIECE * 2 + sub * (64 * KP), meta + b * NM * ROWS + sub * 32);
         if (t + 1 < t1) put(b ^ 1);
         __syncthreads();
     }
 
+    const float total = sum + __shfl_xor(sum, 32);
+    // a split's sums: four columns of row x at a time
+    auto partial = [&](int64_t rows) {
+        float* O = a.at<float>(p.o_part) + (split * rows + x) * KP + oc0;
 #pragma unroll
-    for (int u = 0; u < XB; ++u) {
-        const int64_t x = x0 + 32 * u + lx;
-        const float total = sum[u] + __shfl_xor(sum[u], 32);
-        // four columns of row x of a split's sums at a time
-        auto partial = [&](int64_t rows) {
-            float* O = a.at<float>(p.o_part) + (split * rows + x) * KP + oc0;
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+            for (int q = 0; q < 4; ++q) {
+                f32x4 o;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f32x4 o;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = acc[nb][u][4 * j + e];
-                    *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * j + 4 * half) = o;
-                }
-        };
-        if constexpr (!items) {
-            if (blockIdx.z == 0 && half == 0) {
-                a.at<float>(p.o_m)[split * p.n_pad + x] = m_run[u];
-                a.at<float>(p.o_s)[split * p.n_pad + x] = total;
+                for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * q + e];
+                *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * q + 4 * half) = o;
             }
-            if constexpr (MODE == kLossGrad) partial(p.n_pad);
-        } else if (p.splits_w > 1) {
-            if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = total;
-            partial(p.v_pad);
-        } else if (x < p.v) {
-            if (blockIdx.z == 0 && half == 0) a.dbias[x] = total * sc.inv_cs;
+    };
+    if constexpr (!items) {
+        if (blockIdx.z == 0 && half == 0) {
+            a.at<float>(p.o_m)[split * p.n_pad + x] = m_run;
+            a.at<float>(p.o_s)[split * p.n_pad + x] = total;
         }
-        if constexpr (items) {
-            if (p.splits_w == 1) {
-                // through LDS, so that a row's stores are contiguous: OW columns at a time, 16-byte chunk c of row r at
-                // chunk c ^ (r mod the row's chunks)
-                constexpr int OW = OC < 128 / static_cast<int>(sizeof(E)) ? OC : 128 / static_cast<int>(sizeof(E));
-                constexpr int kRow = OW * static_cast<int>(sizeof(E)), CH = kRow / 16, V = 16 / sizeof(E), ROWS = 64 / CH;
-                typedef __attribute__((ext_vector_type(4))) E e4;
-                typedef __attribute__((ext_vector_type(sizeof(E)))) int words;
-                typedef __attribute__((ext_vector_type(V))) E ev;
-                char* mine = smem + wave * 32 * kRow;
-                const bool aligned = (reinterpret_cast<uintptr_t>(a.dW) | static_cast<uintptr_t>(a.lddw * static_cast<int64_t>(sizeof(E)))) % 16 == 0;
+        if constexpr (MODE == kLossGrad) partial(p.n_pad);
+    } else if (p.splits_w > 1) {
+        if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = total;
+        partial(p.v_pad);
+    } else {
+        if (x < p.v && blockIdx.z == 0 && half == 0) a.dbias[x] = total * sc.inv_cs;
+        // dW through LDS, so that a row's stores are contiguous: OW columns at a time, 16-byte chunk c of row r at
+        // chunk c ^ (r mod the row's chunks)
+        constexpr int OW = OC < 128 / static_cast<int>(sizeof(E)) ? OC : 128 / static_cast<int>(sizeof(E));
+        constexpr int kRow = OW * static_cast<int>(sizeof(E)), CH = kRow / 16, V = 16 / sizeof(E), LINES = 64 / CH;
+        typedef __attribute__((ext_vector_type(4))) E e4;
+        typedef __attribute__((ext_vector_type(sizeof(E)))) int words;  // (stored as it is read: integers)
+        typedef __attribute__((ext_vector_type(V))) E ev;
+        char* mine = smem + wave * 32 * kRow;
+        const bool aligned = (reinterpret_cast<uintptr_t>(a.dW) | static_cast<uintptr_t>(a.lddw * static_cast<int64_t>(sizeof(E)))) % 16 == 0;
 #pragma unroll
-                for (int w0 = 0; w0 < OC; w0 += OW) {
+        for (int w0 = 0; w0 < OC; w0 += OW) {
 #pragma unroll
-                    for (int q = 0; q < OW / 8; ++q) {
-                        e4 v;
+            for (int q = 0; q < OW / 8; ++q) {
+                e4 v;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][u][4 * (q % 4) + e] * sc.inv_dw);
-                        const int byte = (8 * q + 4 * half) * static_cast<int>(sizeof(E));
-                        *reinterpret_cast<words*>(mine + lx * kRow + (((byte >> 4) ^ (lx & (CH - 1))) << 4) + (byte & 15)) = __builtin_bit_cast(words, v);
-                    }
-                    wave_lds_fence();
+                for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][4 * (q % 4) + e] * sc.inv_dw);
+                const int byte = (8 * q + 4 * half) * static_cast<int>(sizeof(E));
+                *reinterpret_cast<words*>(mine + lx * kRow + (((byte >> 4) ^ (lx & (CH - 1))) << 4) + (byte & 15)) = __builtin_bit_cast(words, v);
+            }
+            wave_lds_fence();
 #pragma unroll
-                    for (int r = 0; r < 32; r += ROWS) {
-                        const int row = r + lane / CH, ch = lane % CH, col = oc0 + w0 + ch * V;
-                        const i32x4 w = *reinterpret_cast<const i32x4*>(mine + row * kRow + ((ch ^ (row & (CH - 1))) << 4));
-                        const int64_t item = x0 + 32 * u + row;
-                        if (item >= p.v) continue;
-                        E* o = static_cast<E*>(a.dW) + item * a.lddw + col;
-                        if (aligned && col + V <= p.k) {
-                            *reinterpret_cast<i32x4*>(o) = w;
-                        } else {
-                            const ev y = __builtin_bit_cast(ev, w);
+            for (int r = 0; r < 32; r += LINES) {
+                const int row = r + lane / CH, ch = lane % CH, col = oc0 + w0 + ch * V;
+                const i32x4 w = *reinterpret_cast<const i32x4*>(mine + row * kRow + ((ch ^ (row & (CH - 1))) << 4));
+                if (x0 + row >= p.v) continue;
+                E* o = static_cast<E*>(a.dW) + (x0 + row) * a.lddw + col;
+                if (aligned && col + V <= p.k) {
+                    *reinterpret_cast<i32x4*>(o) = w;
+                } else {
+                    const ev y = __builtin_bit_cast(ev, w);
 #pragma unroll
-                            for (int e = 0; e < V; ++e)
-                                if (col + e < p.k) o[e] = y[e];
-                        }
-                    }
-                    wave_lds_fence();
+                    for (int e = 0; e < V; ++e)
+                        if (col + e < p.k) o[e] = y[e];
                 }
             }
+            wave_lds_fence();
         }
     }
 }
@@ -563,7 +580,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     if (known)
         for (int i = lane; i < p.splits_f; i += 64) {
             const float mi = pm[i * p.n_pad], si = ps[i * p.n_pad];
-            s += m == -INFINITY ? si : si * __builtin_amdgcn_exp2f(mi - m);
+            s += m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi));
         }
     s = wave_sum_f32(s);
     const int32_t tg = known ? a.target[n] : 0;
@@ -573,22 +590,23 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     if (there)
         for (int c = lane; c < p.k; c += 64) lt = fmaf(static_cast<float>(h[c]), static_cast<float>(wt[c]), lt);
     lt = wave_sum_f32(lt);
-    if (there && a.bias) lt += a.bias[tg];
     // every item withdrawn: m stays -inf and s is 0
     const bool empty = m == -INFINITY && s == 0.f;
-    const float l2 = m + (log2f(s) - kShift);
-    const float lse = empty ? -INFINITY : m * kLn2 + logf(s) - kShift * kLn2;
+    // lse2 = m + log2 s, in two parts: where m is large they must not be joined before the target's logit goes
+    const float ls = log2f(s), lt2 = there ? lt * kLog2e + a.at<float>(p.o_bias)[tg] : 0.f;
     if (lane == 0 && n < p.n) {
-        a.lse[n] = known ? lse : 0.f;
-        a.loss[n] = !known || empty ? 0.f : there ? lse - lt : INFINITY;
+        a.lse[n] = !known ? 0.f : empty ? -INFINITY : fmaf(m, kLn2, ls * kLn2);
+        a.loss[n] = !known || empty ? 0.f : there ? ((m - lt2) + ls) * kLn2 : INFINITY;
     }
     if (!p.grad) return;
     const bool live = there && !empty;
     const float w = live ? (a.weight ? a.weight[n] : 1.f) : 0.f;
     if (lane == 0) {
-        a.at<float>(p.o_lse2)[n] = live ? l2 : INFINITY;
-        a.at<float>(p.o_wv)[n] = w * sc.cs;
-        a.at<int32_t>(p.o_tgt)[n] = live ? tg : -1;
+        float* row = a.at<float>(p.o_row) + n;
+        row[0] = live ? m : INFINITY;
+        row[p.n_pad] = live ? w * sc.cs / s : 0.f;
+        row[2 * p.n_pad] = __int_as_float(live ? tg : -1);
+        row[3 * p.n_pad] = w * sc.cs;
     }
     if (n >= p.n) return;
     E* out = static_cast<E*>(a.dH) + n * a.lddh;
@@ -600,12 +618,21 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     for (int c = lane % lanes * 4; c < p.kp; c += 256) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         if (live)
+            for (int i0 = 0; i0 < p.splits_f; i0 += 64) {
+                // the factors of 64 splits, one a lane
+                float f = 0.f;
+                if (i0 + lane < p.splits_f) {
+                    const float mi = pm[(i0 + lane) * p.n_pad];
+                    f = __builtin_amdgcn_exp2f((mi - m) - shift_of(mi));
+                }
+                const int count = min(64, p.splits_f - i0);
 #pragma unroll 8
-            for (int i = grp; i < p.splits_f; i += groups) {
-                const float f = __builtin_amdgcn_exp2f(pm[i * p.n_pad] - m);
-                const f32x4 x = *reinterpret_cast<const f32x4*>(O + i * step + c);
+                for (int i = grp; i < count; i += groups) {
+                    const float fi = __shfl(f, i);
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(O + (i0 + i) * step + c);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], f, o[e]);
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], fi, o[e]);
+                }
             }
         for (int g = lanes; g < 64; g <<= 1)
 #pragma unroll
@@ -645,27 +672,23 @@ __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     }
 }
 
-template <typename E, int NP, int KP, int MODE, int XB, int WAVES, int OCC>
-void launch_tile(const CeArgs& a, hipStream_t st) {
+template <typename E, int NP, int KP, int MODE>
+void launch_main(const CeArgs& a, hipStream_t st) {
     const CePlan& p = a.p;
-    constexpr int NM = MODE == kItems ? 3 : 1;
-    constexpr int OC = KP < 256 ? KP : 256, row = OC * static_cast<int>(sizeof(E)) < 128 ? OC * static_cast<int>(sizeof(E)) : 128;
-    // the tiles and their rows' values; dW leaves through the same memory
-    constexpr int tiles = 2 * NP * kTileY * KP * 2 + 2 * NM * kTileY * 4, out = MODE == kItems ? WAVES * 32 * row : 0;
-    constexpr int lds = tiles > out ? tiles : out, kTileX = WAVES * 32 * XB;
-    auto kern = ce_main_kernel<E, NP, KP, MODE, XB, WAVES, OCC>;
+    constexpr Shape sh = shape_for(NP, KP, MODE);
+    constexpr int NM = MODE == kItems ? 4 : 1, OC = KP < 256 ? KP : 256;
+    constexpr int row = OC * static_cast<int>(sizeof(E)) < 128 ? OC * static_cast<int>(sizeof(E)) : 128;
+    // two stages and their rows' values; dW leaves through the same memory
+    constexpr int rows = 32 * sh.blocks, tiles = 2 * NP * rows * KP * 2 + 2 * NM * rows * 4, out = MODE == kItems ? sh.waves * 32 * row : 0;
+    constexpr int lds = tiles > out ? tiles : out, kTileX = sh.waves * 32;
+    static_assert(lds <= 160 * 1024 && kPad % kTileX == 0 && kTileY % rows == 0, "the shape fits the LDS and the padding");
+    auto kern = ce_main_kernel<E, NP, KP, MODE, sh.waves, sh.blocks, sh.occ>;
     if (lds > 64 * 1024)
         RS_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const dim3 grid(static_cast<uint32_t>(ceil_div(MODE == kItems ? p.v : p.n, kTileX)),
                     static_cast<uint32_t>(MODE == kItems ? p.splits_w : p.splits_f), MODE == kLoss ? 1u : static_cast<uint32_t>(p.z));
-    kern<<<grid, WAVES * 64, lds, st>>>(a);
+    kern<<<grid, sh.waves * 64, lds, st>>>(a);
     RS_HIP(hipGetLastError());
-}
-
-template <typename E, int NP, int KP, int MODE>
-void launch_main(const CeArgs& a, hipStream_t st) {
-    constexpr int XB = KP <= (NP == 2 ? 64 : 256) ? 2 : 1;
-    launch_tile<E, NP, KP, MODE, XB, XB == 2 ? 4 : 8, 1>(a, st);
 }
 
 template <typename E, int NP>

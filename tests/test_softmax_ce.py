@@ -5,7 +5,7 @@ Tolerances.  u = eps / 2 is half a step of a type.  A logit is a sum of k produc
 (k + 4) u32 sum |h w| plus, for the base-2 exponent, 3 u32 |l| (one rounding each for the scale, the sum with the
 bias and the difference); fp16 pairs leave 3 u32 |h w| of a product more.  With L the largest
 sum |h w| + |bias| of a row, e_l = (k + 10) u32 (L + 1) bounds a logit's error, the loss and lse take 2 e_l, and a
-probability is off by 2 e_l of itself.  A coefficient c = weight (p - [target]) is then rounded to the product's type:
+probability is off by 2 e_l and 4 u32 of itself (its exponential, the sum, the division and a product).  A coefficient c = weight (p - [target]) is then rounded to the product's type:
 u16 of itself (fp32: a pair, 2 u32), and the sum over the rows or items adds (terms) u32 of the sum of magnitudes.
 Outputs add half a step of their type.  (exp2 and log2 are good to 2 units, inside the 10.)
 """
@@ -49,12 +49,12 @@ def reference(H, W, target, bias=None, weight=None):
         loss[known & gone[tt]] = math.inf
     lse = torch.where(known, lse, torch.zeros_like(lse))
     p = torch.where(live[:, None], torch.exp(z - lse[:, None]), torch.zeros_like(z))
+    prob = p.clone()
     p[torch.arange(n)[live], tt[live]] -= 1
     gl = torch.where(live, g, torch.zeros_like(g))
     c = p * gl[:, None]
-    absp = p.clone().abs()
     L = (Hm.abs() @ Wm.abs().T + torch.where(gone, torch.zeros_like(b), b).abs()).amax(1) if v else torch.zeros(n)
-    return dict(loss=loss, lse=lse, dH=c @ Wm, dW=c.T @ Hm, db=c.sum(0), L=L, live=live, c=c, Hm=Hm, Wm=Wm, g=gl, absp=absp)
+    return dict(loss=loss, lse=lse, dH=c @ Wm, dW=c.T @ Hm, db=c.sum(0), L=L, live=live, c=c, Hm=Hm, Wm=Wm, g=gl, p=prob)
 
 
 def make(n, v, k, ty, seed=0, spread=1.5, bias=False, gone=0.0, unknown=0.0, weight=True, dev="cuda"):
@@ -88,12 +88,12 @@ def check(out, ref, ty, k, grad=True):
         return
     u_c = 2 * U32 if ty == "f32" else half_step(t)
     n, v = ref["c"].shape
-    # error of a coefficient: its probability's, then its rounding; a rounded fp16 coefficient keeps at least 2^-25 of
+    # error of a coefficient: its probability's, then its rounding; an fp16 coefficient of any type keeps at least 2^-25 of
     # 2^-13 of the largest weight (it is held scaled to below 2^14)
     gmax = ref["g"].abs().max() if n else 0.0
-    floor = float(gmax) * 2.0 ** -37 if ty != "bf16" else 0.0
-    p = ref["absp"]
-    ec = ref["g"].abs()[:, None] * (2 * e_l[:, None] * (p + (p > 0.5)) + 2 * U32) * ref["live"][:, None] + u_c * ref["c"].abs() + floor * ref["live"][:, None]
+    floor = float(gmax) * 2.0 ** -38
+    p = ref["p"]
+    ec = ref["g"].abs()[:, None] * (2 * e_l[:, None] + 4 * U32) * p + u_c * ref["c"].abs() + floor * ref["live"][:, None]
     bound_H = ec @ ref["Wm"].abs() + (v + 4) * U32 * (ref["c"].abs() @ ref["Wm"].abs())
     bound_W = ec.T @ ref["Hm"].abs() + (n + 4) * U32 * (ref["c"].abs().T @ ref["Hm"].abs())
     # db sums the coefficients before they are rounded
@@ -177,6 +177,46 @@ def test_bias_of_the_lowest_value(ctx):
     ref = reference(H, W, target, b, w)
     ref["L"] = ref["L"] * 0 + (H.double().abs() @ W.double().abs().T).max().cpu() + 5  # the lowest values' logits decide nothing
     check(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), ref, "f32", 24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v", [(5, 33), (200, 3000)])
+def test_every_bias_of_the_lowest_value(ctx, n, v):
+    """Every logit is the type's lowest value (the products vanish beside it): each item has the probability 1 / v."""
+    H, W, target, b, w = make(n, v, 16, "f32", seed=15, bias=True)
+    b[:] = torch.finfo(torch.float32).min
+    loss, lse, dH, dW, db = (x.double().cpu() for x in ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True))
+    assert torch.isfinite(lse).all() and (lse < -1e35).all()
+    u = 16 * U32
+    assert ((loss - math.log(v)).abs() <= u * math.log(v)).all()
+    c = torch.full((n, v), 1.0 / v, dtype=torch.float64)
+    c[torch.arange(n), target.cpu().long()] -= 1
+    c *= w.double().cpu()[:, None]
+    Hd, Wd = H.double().cpu(), W.double().cpu()
+    assert ((dH - c @ Wd).abs() <= (u + v * U32) * (c.abs() @ Wd.abs())).all()
+    assert ((dW - c.T @ Hd).abs() <= (u + n * U32) * (c.abs().T @ Hd.abs())).all()
+    assert ((db - c.sum(0)).abs() <= (u + n * U32) * c.abs().sum(0)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("where", ["late", "zeros", "huge", "tiny"])
+def test_scales_from_a_sample(ctx, ty, where):
+    """Tables too large to be looked through before they are scaled: the sampled rows mislead about the rest."""
+    n, v, k = 700, 4000, 64
+    H, W, target, b, w = make(n, v, k, ty, seed=16, bias=True)
+    if where == "late":  # one row far above the others, which no sample of every 30th row meets
+        W[1237] *= 300.0
+        H[333] *= 0.01
+    elif where == "zeros":
+        W[::31] = 0
+        H[::5] = 0
+    elif where == "huge":
+        H *= 1e-18
+        W *= 1e18
+    else:
+        W *= 1e-25
+    check(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), ty, k)
 
 
 @pytest.mark.gpu
