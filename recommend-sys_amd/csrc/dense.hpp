@@ -98,6 +98,22 @@ inline std::string check_matrix(const char* name, const void* p, int64_t cols, i
     return std::string();
 }
 
+// LDS tile of rows of KP 16-bit values: 16-byte chunk c of row r sits at chunk c ^ mix(r), the row's low three bits rotated.  A row-wise read (8
+// rows, one chunk at a time) and a transposing one (4 rows, two neighbouring chunks) then both meet every bank once; c ^ (r mod 16) had neighbouring rows share their chunk pairs
+// (half of the LDS cycles were
+// conflicts).  Byte offset: what a lane adds is one base, the constant part of c goes in
+// by XOR (bits the rows do not reach: by addition), so a few registers hold all the addresses of a tile.
+template <int KP>
+struct LdsTile {
+    static constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;
+    static __device__ __forceinline__ int mix(int row) {
+        return KP == 32 ? (row & 2) | ((row >> 2) & 1) : (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & M;
+    }
+    static __device__ __forceinline__ int base(int row, int c) { return row * (KP * 2) + ((c ^ mix(row)) & M) * 16 + (c & ~M) * 16; }
+    // base(row, c) with the constant dc joined to c (no common bits)
+    static __device__ __forceinline__ int at(int base, int dc) { return (base ^ ((dc & M) * 16)) + (dc & ~M) * 16; }
+};
+
 // LDS written by lanes of a wave before this is read by its other lanes after it
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

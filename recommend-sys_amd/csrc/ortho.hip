@@ -75,12 +75,10 @@ __device__ __forceinline__ f32x4 load4(const E* G, int64_t ld, int64_t r, int64_
     return v;
 }
 
-// 16-byte chunk c of row r of an LDS tile of W 16-bit columns sits at chunk c ^ (r mod 16) of its row (fewer where a
-// row has fewer): element offset
+// element offset of a value in an LDS tile of W 16-bit columns
 template <int W>
 __device__ __forceinline__ int lds_at(int row, int col) {
-    constexpr int C = W / 8, M = C < 16 ? C - 1 : 15;
-    return (row * C + ((col >> 3) ^ (row & M))) * 8 + (col & 7);
+    return LdsTile<W>::base(row, col >> 3) / 2 + (col & 7);
 }
 
 // ---- Gram matrix of a piece of the long side -----------------------------------------------------------------------
@@ -106,7 +104,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
     const int pi = PAN == 2 ? blockIdx.y / p.panels : 0, pj = PAN == 2 ? blockIdx.y % p.panels : 0;
     const int64_t r0 = blockIdx.x * p.per, r1 = min(p.r, r0 + p.per);
 
-    f32x4 st[PER];
+    f32x4 sa[PER], sb[PER];  // two stages on their way: one is too little to cover memory's latency
     auto place = [&](int i, int& pan, int& row, int& col) {
         const int g = i * kThreads + threadIdx.x;
         pan = g / (PIECE / 4);
@@ -116,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
         else
             row = q / (SP / 4), col = q % (SP / 4) * 4;
     };
-    auto fetch = [&](int64_t rb) {
+    auto fetch = [&](f32x4 (&st)[PER], int64_t rb) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int pan, row, col;
@@ -125,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
         }
     };
     // the stage's largest finite magnitude, over the workgroup
-    auto largest = [&](int b) {
+    auto largest = [&](const f32x4 (&st)[PER], int b) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
@@ -141,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
         for (int i = 0; i < 8; ++i) m = max(m, smax[b][i]);
         return m;
     };
-    auto put = [&](int b, float sc) {
+    auto put = [&](const f32x4 (&st)[PER], int b, float sc) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int pan, row, col;
@@ -196,14 +194,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[x][y][i] = acc[x][y][i] * f * f;
     };
-    fetch(r0);
-    follow(largest(0));
-    put(0, sc);
-    __syncthreads();
-    int b = 0;
-    for (int64_t rb = r0; rb < r1; rb += KR, b ^= 1) {
-        const bool more = rb + KR < r1;
-        if (more) fetch(rb + KR);
+    auto multiply = [&](int b) {
         const _Float16 *ti = tile + b * BUF, *tj = ti + (PAN - 1) * NP * PIECE;
 #pragma unroll
         for (int k = 0; k < KR / 16 / NG; ++k) {
@@ -224,11 +215,25 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
                 }
             }
         }
-        if (more) {
-            follow(largest(b ^ 1));
-            put(b ^ 1, sc);
+    };
+    // a stage in LDS, the next one in `ready`, the one after it fetched into `other`
+    auto step = [&](int64_t rb, int b, f32x4 (&ready)[PER], f32x4 (&other)[PER]) {
+        if (rb + 2 * KR < r1) fetch(other, rb + 2 * KR);
+        multiply(b);
+        if (rb + KR < r1) {
+            follow(largest(ready, b ^ 1));
+            put(ready, b ^ 1, sc);
         }
         __syncthreads();
+    };
+    fetch(sa, r0);
+    if (r0 + KR < r1) fetch(sb, r0 + KR);
+    follow(largest(sa, 0));
+    put(sa, 0, sc);
+    __syncthreads();
+    for (int64_t rb = r0; rb < r1; rb += 2 * KR) {
+        step(rb, 0, sb, sa);
+        if (rb + KR < r1) step(rb + KR, 1, sa, sb);
     }
     if (threadIdx.x == 0) part_scale[blockIdx.y * gridDim.x + blockIdx.x] = sc;
     // the groups' sums, halving their number through LDS
@@ -464,7 +469,8 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
     for (int q = 0; q < 2; ++q)
 #pragma unroll
         for (int k = 0; k < KS; ++k) t[q][k] = *reinterpret_cast<const f16x8*>(tp + (static_cast<int64_t>(q) * SP + j0 + lx) * SP + k * 16 + half * 8);
-    f32x4 st[PER];
+    constexpr bool kTwo = SP <= 256;  // two tiles on their way; SP = 512: T takes the registers, one
+    f32x4 sa[PER], sb[kTwo ? PER : 1];
     auto place = [&](int i, int& row, int& col) {
         const int g = i * THREADS + threadIdx.x;
         if (WIDE)
@@ -472,7 +478,7 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
         else
             row = g / (SP / 4), col = g % (SP / 4) * 4;
     };
-    auto fetch = [&](int64_t r0) {
+    auto fetch = [&](f32x4 (&st)[PER], int64_t r0) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int row, col;
@@ -480,7 +486,7 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
             st[i] = load4<E, WIDE, VEC>(G, ldg, r0 + row, p.r, col, p.s);
         }
     };
-    auto put = [&](int b) {
+    auto put = [&](const f32x4 (&st)[PER], int b) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int row, col;
@@ -505,21 +511,22 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
             }
         }
     };
-    const int64_t tiles = (p.r + TR - 1) / TR;
-    int64_t it = blockIdx.x;
-    if (it < tiles) fetch(it * TR), put(0);
-    __syncthreads();
-    int b = 0;
-    for (; it < tiles; it += gridDim.x, b ^= 1) {
-        const bool more = it + gridDim.x < tiles;
-        if (more) fetch((it + gridDim.x) * TR);
-        const _Float16* d = tile + b * NP * PIECE;
+    const int64_t tiles = (p.r + TR - 1) / TR, hop = gridDim.x;
+    const float back = scale[j0 + lx];  // what takes a column's sums back
+    // a tile in LDS, the next one in `ready`, the one after it fetched into `other`
+    auto step = [&](int64_t it, int b, f32x4 (&ready)[PER], f32x4 (&other)[PER]) {
+        const int64_t ahead = it + (kTwo ? 2 : 1) * hop;
+        if (ahead < tiles) fetch(other, ahead * TR);
+        // (both bases taken anew for every tile: kept for all 16 stores and the reads they would cost the registers of T)
+        int rb = LdsTile<SP>::base(grp * 32 + lx, half) + b * NP * PIECE * 2;
+        E* out = X + (WIDE ? (j0 + 4 * half) * ldx + it * TR + grp * 32 + lx : (it * TR + grp * 32 + 4 * half) * ldx + j0 + lx);
+        asm volatile("" : "+v"(rb), "+v"(out));
         f32x16 acc = f32x16{0};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             f16x8 g[NP];
 #pragma unroll
-            for (int q = 0; q < NP; ++q) g[q] = *reinterpret_cast<const f16x8*>(d + q * PIECE + lds_at<SP>(grp * 32 + lx, k * 16 + half * 8));
+            for (int q = 0; q < NP; ++q) g[q] = *reinterpret_cast<const f16x8*>(smem + q * PIECE * 2 + LdsTile<SP>::at(rb, 2 * k));
             // lanes run along the contiguous side of X
             auto mm = [&](f16x8 u, f16x8 v) {
                 acc = WIDE ? __builtin_amdgcn_mfma_f32_32x32x16_f16(v, u, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(u, v, acc, 0, 0, 0);
@@ -528,15 +535,30 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
             mm(g[0], t[1][k]);
             if constexpr (NP == 2) mm(g[1], t[0][k]);
         }
+        if (it + hop < tiles) put(ready, b ^ 1);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int o = 8 * (e / 4) + 4 * half + e % 4;
-            const int64_t r = it * TR + grp * 32 + (WIDE ? lx : o);
-            const int j = j0 + (WIDE ? o : lx);
-            if (r < p.r && j < p.s) X[WIDE ? j * ldx + r : r * ldx + j] = static_cast<E>(acc[e] * scale[j]);
+            const int o = 8 * (e / 4) + e % 4;  // rows (WIDE: columns) past the first of the lane's
+            const int64_t r = it * TR + grp * 32 + (WIDE ? lx : 4 * half + o);
+            const int j = j0 + (WIDE ? 4 * half + o : lx);
+            if (r < p.r && j < p.s) out[o * ldx] = static_cast<E>(acc[e] * (WIDE ? scale[j] : back));
         }
-        if (more) put(b ^ 1);
         __syncthreads();
+    };
+    const int64_t first = blockIdx.x;
+    if (first < tiles) fetch(sa, first * TR);
+    if constexpr (kTwo)
+        if (first + hop < tiles) fetch(sb, (first + hop) * TR);
+    if (first < tiles) put(sa, 0);
+    __syncthreads();
+    for (int64_t it = first; it < tiles; it += 2 * hop) {
+        if constexpr (kTwo) {
+            step(it, 0, sb, sa);
+            if (it + hop < tiles) step(it + hop, 1, sa, sb);
+        } else {
+            step(it, 0, sa, sa);
+            if (it + hop < tiles) step(it + hop, 1, sa, sa);
+        }
     }
 }
 

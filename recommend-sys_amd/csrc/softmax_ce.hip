@@ -272,20 +272,6 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
 // ---- the products --------------------------------------------------------------------------------------------------
 __device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-// 16-byte chunk c of row r of an LDS tile sits at chunk c ^ mix(r), the row's low three bits rotated.  A row-wise read (8
-// rows, one chunk at a time) and a transposing one (4 rows, two neighbouring chunks) then both meet every bank once; c ^ (r mod 16) had neighbouring rows share their chunk pairs
-// (half of the LDS cycles were conflicts).  Byte offset: what a lane adds is one base, the constant part of c goes in
-// by XOR (bits the rows do not reach: by addition), so a few registers hold all the addresses of a tile.
-template <int KP>
-struct LdsTile {
-    static constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;
-    static __device__ __forceinline__ int mix(int row) {
-        return KP == 32 ? (row & 2) | ((row >> 2) & 1) : (((row & 3) << 1) | ((row >> 2) & 1) | (row & 8)) & M;
-    }
-    static __device__ __forceinline__ int base(int row, int c) { return row * (KP * 2) + ((c ^ mix(row)) & M) * 16 + (c & ~M) * 16; }
-    // base(row, c) with the constant dc joined to c (no common bits)
-    static __device__ __forceinline__ int at(int base, int dc) { return (base ^ ((dc & M) * 16)) + (dc & ~M) * 16; }
-};
 // Each wave holds 32 stationary rows; a stage of streamed rows passes through LDS, the next one on its way in registers.
 // MODE kLoss / kLossGrad: x = users' rows, y = items; kItems: x = items, y = users' rows.
 template <typename E, int NP, int KP, int MODE, int WAVES, int SUB, int OCC>
