@@ -8,6 +8,7 @@
 #include <string>
 
 #include "common.hpp"
+#include "wave.hpp"
 #include "rsgpu_dense.h"
 
 namespace rs {
@@ -120,14 +121,18 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// maximum over the wave (64 lanes)
+// maximum over the wave (64 lanes): inside rows of 16 lanes by DPP, the four rows by scalar reads
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const uint32_t w = __shfl_xor(v, o);
+    auto step = [&](auto ctrl) {
+        const uint32_t w = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xF, 0xF, false));
         v = v > w ? v : w;
-    }
-    return v;
+    };
+    step(std::integral_constant<int, DPP_QUAD_XOR1>{});
+    step(std::integral_constant<int, DPP_QUAD_XOR2>{});
+    step(std::integral_constant<int, DPP_ROW_HALF_MIRROR>{});
+    step(std::integral_constant<int, DPP_ROW_MIRROR>{});
+    auto lane = [&](int l) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); };
+    return max(max(lane(0), lane(16)), max(lane(32), lane(48)));
 }
 __device__ __forceinline__ float wave_sum_f32(float v) {
 #pragma unroll

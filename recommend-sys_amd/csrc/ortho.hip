@@ -17,6 +17,8 @@ namespace {
 
 constexpr int kThreads = 512;     // the two passes over the table: 8 waves
 constexpr int kStage = 8192;      // table elements of one stage of the Gram pass (per panel)
+constexpr int kJoinGroups = 8;    // groups that many pieces of the Gram matrix are summed in first
+constexpr int kJoinDirect = 24;   // up to so many pieces are joined at once
 
 struct OrthoPlan {
     int64_t r;       // long side
@@ -25,7 +27,7 @@ struct OrthoPlan {
     int32_t panels;  // the Gram matrix is panels x panels blocks of at most 256 x 256
     int32_t splits;  // pieces of the long side, one per workgroup
     int64_t per;     // long-side rows of a piece
-    int64_t o_part, o_pscale, o_mat[6], o_t, o_scale, bytes;  // A0, A, M, U, Ta, Tb; T's fp16 pieces and their scales
+    int64_t o_part, o_sum, o_pscale, o_mat[6], o_t, o_scale, bytes;  // A0, A, M, U, Ta, Tb; T's fp16 pieces and their scales
 };
 
 OrthoPlan make_plan(int64_t rows, int64_t cols) {
@@ -36,8 +38,10 @@ OrthoPlan make_plan(int64_t rows, int64_t cols) {
     p.sm = p.s <= 32 ? 32 : p.sp;
     p.panels = p.sp > 256 ? 2 : 1;
     const int64_t kr = kStage / std::min(p.sp, 256) / p.panels, stages = ceil_div(p.r, kr);
-    // one workgroup per CU, and a few stages each: the pieces' sums are written and read again
-    p.splits = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(256 / (p.panels * p.panels), ceil_div(stages, 4))));
+    // One workgroup per CU at most; eight stages each, because the pieces' sums are written and read again, fewer where that
+    // leaves only few pieces.
+    const int64_t want = std::max<int64_t>(ceil_div(stages, 8), std::min<int64_t>(stages, kJoinDirect));
+    p.splits = static_cast<int32_t>(std::min<int64_t>(256 / (p.panels * p.panels), want));
     p.per = ceil_div(stages, p.splits) * kr;
     p.splits = static_cast<int32_t>(ceil_div(p.r, p.per));
     int64_t at = 0;
@@ -47,6 +51,7 @@ OrthoPlan make_plan(int64_t rows, int64_t cols) {
         return o;
     };
     p.o_part = take(static_cast<int64_t>(p.splits) * p.sp * p.sp * 4);
+    p.o_sum = take(p.splits > kJoinDirect ? static_cast<int64_t>(kJoinGroups) * p.sp * p.sp * 8 : 0);
     p.o_pscale = take(static_cast<int64_t>(p.splits) * p.panels * p.panels * 4);
     for (int64_t& o : p.o_mat) o = take(static_cast<int64_t>(p.sm) * p.sm * 8);
     p.o_t = take(static_cast<int64_t>(2) * p.sp * p.sp * 2);
@@ -92,6 +97,7 @@ __device__ __forceinline__ int lds_at(int row, int col) {
 template <typename E, bool WIDE, bool VEC, int SP, int PAN>
 __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restrict__ G, int64_t ld, OrthoPlan p, float* __restrict__ part,
                                                              float* __restrict__ part_scale) {
+#pragma clang fp contract(fast)
     constexpr int NP = std::is_same<E, float>::value ? 2 : 1;
     constexpr int KR = kStage / SP / PAN, WI = SP / 64, WJ = SP == 256 ? 2 : SP / 64, NG = 8 / (WI * WJ), BJ = SP / WJ / 32;
     constexpr int PIECE = KR * SP, BUF = PAN * NP * PIECE;  // 16-bit elements
@@ -122,21 +128,20 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
             st[i] = load4<E, WIDE, VEC>(G, ld, rb + row, r1, (pan ? pj : pi) * 256 + col, p.s);
         }
     };
-    // the stage's largest finite magnitude, over the workgroup
-    auto largest = [&](const f32x4 (&st)[PER], int b) {
-        uint32_t m = 0;
+    // a stage's largest magnitude: each wave's share noted, and (a barrier later) the workgroup's
+    auto note = [&](const f32x4 (&st)[PER], int slot) {
+        float top = 0.f;  // (NaN passes by, an infinity makes the result one or NaN whatever the scale)
 #pragma unroll
         for (int i = 0; i < PER; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t u = __float_as_uint(st[i][e]) & 0x7FFFFFFFu;
-                if (u < 0x7F800000u && u > m) m = u;
-            }
-        m = wave_max_u32(m);
-        if (lane == 0) smax[b][wave] = m;
-        __syncthreads();
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(st[i][e]));
+        const uint32_t m = wave_max_u32(__float_as_uint(top));
+        if (lane == 0) smax[slot][wave] = m;
+    };
+    auto largest = [&](int slot) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, smax[b][i]);
+        for (int i = 0; i < 8; ++i) m = max(m, smax[slot][i]);
         return m;
     };
     auto put = [&](const f32x4 (&st)[PER], int b, float sc) {
@@ -148,7 +153,7 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
             f16x4 h, l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = st[i][e] * sc;  // (a power of two: exact)
+                const float x = st[i][e] * sc;  // (a power of two: exact, fused or not)
                 h[e] = static_cast<_Float16>(x);
                 l[e] = static_cast<_Float16>(x - static_cast<float>(h[e]));
             }
@@ -178,21 +183,17 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
     for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int y = 0; y < BJ; ++y) acc[x][y] = f32x16{0};
-    // scale: 2^(12 - exponent of the reference); a stage's largest may reach 2^15
+    // scale: 2^(12 - exponent of the reference); a stage's largest may reach 2^15.  Returns what the sums so far are to be
+    // multiplied by (twice: they are products of two).
     float sc = 1.f;
     uint32_t limit = 0;  // bits of the largest magnitude the scale stands
     auto follow = [&](uint32_t m) {
-        if (m <= limit) return;
+        if (m <= limit) return 1.f;
         const int e = max(static_cast<int>(m >> 23), 1) - 127;
         limit = e + 3 > 127 ? 0x7F7FFFFFu : static_cast<uint32_t>(e + 3 + 127) << 23;
         const float next = __uint_as_float(static_cast<uint32_t>(min(12 - e, 126) + 127) << 23), f = next / sc;
         sc = next;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int y = 0; y < BJ; ++y)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[x][y][i] = acc[x][y][i] * f * f;
+        return f;
     };
     auto multiply = [&](int b) {
         const _Float16 *ti = tile + b * BUF, *tj = ti + (PAN - 1) * NP * PIECE;
@@ -216,20 +217,33 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
             }
         }
     };
-    // a stage in LDS, the next one in `ready`, the one after it fetched into `other`
+    // Stage i in LDS, i + 1 in `ready` (its largest noted), i + 2 on its way in `other`: one barrier a stage.
     auto step = [&](int64_t rb, int b, f32x4 (&ready)[PER], f32x4 (&other)[PER]) {
-        if (rb + 2 * KR < r1) fetch(other, rb + 2 * KR);
-        multiply(b);
+        float f = 1.f;
         if (rb + KR < r1) {
-            follow(largest(ready, b ^ 1));
+            f = follow(largest(b ^ 1));
             put(ready, b ^ 1, sc);
+            if (rb + 3 * KR < r1) fetch(ready, rb + 3 * KR);
         }
+        multiply(b);
+        if (f != 1.f)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < BJ; ++y)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[x][y][i] = acc[x][y][i] * f * f;
+        if (rb + 2 * KR < r1) note(other, b);
         __syncthreads();
     };
     fetch(sa, r0);
     if (r0 + KR < r1) fetch(sb, r0 + KR);
-    follow(largest(sa, 0));
+    note(sa, 0);
+    __syncthreads();
+    follow(largest(0));
     put(sa, 0, sc);
+    if (r0 + 2 * KR < r1) fetch(sa, r0 + 2 * KR);
+    if (r0 + KR < r1) note(sb, 1);
     __syncthreads();
     for (int64_t rb = r0; rb < r1; rb += 2 * KR) {
         step(rb, 0, sb, sa);
@@ -269,22 +283,44 @@ __global__ __launch_bounds__(kThreads) void ortho_gram_kernel(const E* __restric
                 o[static_cast<int64_t>(wi + 32 * x + 8 * (e / 4) + 4 * half + e % 4) * p.sp + wj + 32 * y + lx] = acc[x][y][e];
 }
 
+// Sums of groups of the pieces in fp64, where there are many: a thread per four entries, blockIdx.y a group.
+__global__ __launch_bounds__(256) void ortho_gram_sum_kernel(const float* __restrict__ part, const float* __restrict__ part_scale, OrthoPlan p,
+                                                            double* __restrict__ out) {
+    const int64_t step = static_cast<int64_t>(p.sp) * p.sp, at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+    const int i = static_cast<int>(at / p.sp), j = static_cast<int>(at % p.sp);
+    const float* sc = part_scale + (i / 256 * p.panels + j / 256) * p.splits;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    const int n0 = p.splits * static_cast<int>(blockIdx.y) / kJoinGroups, n1 = p.splits * (static_cast<int>(blockIdx.y) + 1) / kJoinGroups;
+#pragma unroll 8
+    for (int n = n0; n < n1; ++n) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(part + n * step + at);
+        const double a = 1.0 / sc[n];  // (a power of two)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += static_cast<double>(x[e]) * (a * a);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[blockIdx.y * step + at + e] = s[e];
+}
+
 // A0 = sum of the pieces' B + B^T (16-bit tables: their half) in fp64, in the pieces' order; a 16 x 16 block and its
-// mirror per workgroup, four groups of 256 threads share the pieces.
-__global__ __launch_bounds__(1024) void ortho_gram_join_kernel(const float* __restrict__ part, const float* __restrict__ part_scale,
-                                                              OrthoPlan p, double scale, double* __restrict__ A) {
+// mirror per workgroup, four groups of 256 threads share the pieces.  P: float pieces with their scales, or the sums of
+// groups of them.
+template <typename P>
+__global__ __launch_bounds__(1024) void ortho_gram_join_kernel(const P* __restrict__ part, const float* __restrict__ part_scale,
+                                                              OrthoPlan p, int pieces, double scale, double* __restrict__ A) {
     __shared__ double sm[2][4][16][17];
     int ib = 0, t = blockIdx.x;
     while (t > ib) t -= ++ib;  // block t of the lower triangle: row ib, column t
     const int jb = t, g = threadIdx.x >> 8, i = (threadIdx.x >> 4) & 15, j = threadIdx.x & 15;
-    const float *u = part + static_cast<int64_t>(ib * 16 + i) * p.sp + jb * 16 + j, *v = part + static_cast<int64_t>(jb * 16 + i) * p.sp + ib * 16 + j;
+    const P *u = part + static_cast<int64_t>(ib * 16 + i) * p.sp + jb * 16 + j, *v = part + static_cast<int64_t>(jb * 16 + i) * p.sp + ib * 16 + j;
     const float *us = part_scale + (ib / 16 * p.panels + jb / 16) * p.splits, *vs = part_scale + (jb / 16 * p.panels + ib / 16) * p.splits;
     const int64_t step = static_cast<int64_t>(p.sp) * p.sp;
     double su = 0.0, sv = 0.0;
-    const int n0 = p.splits * g / 4, n1 = p.splits * (g + 1) / 4;
-#pragma unroll 8
+    const int n0 = pieces * g / 4, n1 = pieces * (g + 1) / 4;
+#pragma unroll 4
     for (int n = n0; n < n1; ++n) {
-        const double a = 1.0 / us[n], b = 1.0 / vs[n];  // (powers of two)
+        double a = 1.0, b = 1.0;
+        if constexpr (std::is_same<P, float>::value) a = 1.0 / us[n], b = 1.0 / vs[n];  // (powers of two)
         su += static_cast<double>(u[n * step]) * (a * a);
         sv += static_cast<double>(v[n * step]) * (b * b);
     }
@@ -456,6 +492,7 @@ __global__ __launch_bounds__(64) void ortho_pack_kernel(OrthoPlan p, const doubl
 template <typename E, bool WIDE, bool VEC, int SP, int THREADS>
 __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_t ldg, OrthoPlan p, const _Float16* __restrict__ tp,
                                                              const float* __restrict__ scale, E* X, int64_t ldx) {
+#pragma clang fp contract(fast)
     constexpr int NP = std::is_same<E, float>::value ? 2 : 1;
     constexpr int WAVES = THREADS / 64, WC = SP / 32 < WAVES ? SP / 32 : WAVES, NG = WAVES / WC, KS = SP / 16;
     constexpr int TR = 32 * NG, PIECE = TR * SP, PER = PIECE / 4 / THREADS;
@@ -495,7 +532,7 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
             f16x4 h, l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = st[i][e] * gscale;  // (a power of two: exact)
+                const float x = st[i][e] * gscale;  // (a power of two: exact, fused or not)
                 h[e] = static_cast<_Float16>(x);
                 l[e] = static_cast<_Float16>(x - static_cast<float>(h[e]));
             }
@@ -594,7 +631,14 @@ void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, d
     else
         launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 2>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
     const uint32_t t = static_cast<uint32_t>(p.sm / 16);
-    ortho_gram_join_kernel<<<t * (t + 1) / 2, 1024, 0, st>>>(part, part_scale, p, kF32 ? 1.0 : 0.5, A0);
+    if (p.splits > kJoinDirect) {
+        double* sums = reinterpret_cast<double*>(ws + p.o_sum);
+        ortho_gram_sum_kernel<<<dim3(static_cast<uint32_t>(p.sp * p.sp / 1024), kJoinGroups), 256, 0, st>>>(part, part_scale, p, sums);
+        RS_HIP(hipGetLastError());
+        ortho_gram_join_kernel<double><<<t * (t + 1) / 2, 1024, 0, st>>>(sums, part_scale, p, kJoinGroups, kF32 ? 1.0 : 0.5, A0);
+    } else {
+        ortho_gram_join_kernel<float><<<t * (t + 1) / 2, 1024, 0, st>>>(part, part_scale, p, p.splits, kF32 ? 1.0 : 0.5, A0);
+    }
     RS_HIP(hipGetLastError());
 
     if (p.sm == 32) {
