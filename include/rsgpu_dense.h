@@ -2,17 +2,18 @@
  * rsgpu_dense.h -- C-ABI of librsgpu's dense operators over factor tables (device pointers).  Contexts, status codes
  * and errors are rsgpu.h's.
  *
- * Not functions of the reference: what a model with the factor tables P, Q above needs to be trained for ranking
+ * Not functions of the reference: what a model with user and item factor tables needs to be trained for ranking
  * over the whole catalogue and to answer with the whole catalogue.
  *
  * All matrices are row-major device memory of ctx's device with a row stride (ld, in elements) of at least their
  * columns; element types RS_TYPE_*.  A call enqueues its kernels on `stream` (NULL: the ctx stream,
- * RS_STREAM_DEFAULT: the device's default stream) and returns without waiting: it synchronises nothing, allocates nothing, keeps nothing, and may be captured into a graph.
+ * RS_STREAM_DEFAULT: the device's default stream) and returns without waiting: it synchronises nothing, allocates
+ * nothing, keeps nothing, and may be captured into a graph.
  * `ws` is device scratch of at least the bytes that the operator's _workspace call gives (16-byte aligned); it is
  * free for other use once the call's kernels have run, and two calls that may overlap need a workspace each.  The
  * caller's current device is put back before a call returns.  Calls whose sizes leave nothing to do return RS_OK
- * without a launch.  Sums are held in fp32, int32 or fp64 and each output is rounded once; results do not depend on timing (no
- * floating-point atomics).  n_factors up to RS_DENSE_MAX_FACTORS. */
+ * without a launch.  Sums are held in fp32, int32 or fp64 and each output is rounded once; results do not depend on
+ * timing (no floating-point atomics).  n_factors up to RS_DENSE_MAX_FACTORS. */
 #ifndef RSGPU_DENSE_H
 #define RSGPU_DENSE_H
 
@@ -55,10 +56,10 @@ int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, in
                   void* ws, int64_t ws_bytes, void* stream);
 
 /* Rows in 8 bits with a scale each: scale_r = max_c |x_rc| * (1/127), both factors and the product in fp32,
- * q_rc = x_rc / scale_r to the nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of zeros has scale 0 and q 0; a
- * row with an infinity or NaN has scale NaN and q 0 (so that all its products are NaN), as has a row whose scale
- * underflows to 0, but with scale 0.  X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as
- * they are.  n_cols >= 1. */
+ * q_rc = x_rc / scale_r to the nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of
+ * zeros, or whose scale underflows to 0, has scale 0 and q 0; a row with an infinity or NaN has scale NaN and q 0, so
+ * that all its products are NaN.  X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as they
+ * are.  n_cols >= 1. */
 int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_cols, const void* X, int64_t ldx, int8_t* q,
                      int64_t ldq, float* scale, void* stream);
 
@@ -77,13 +78,36 @@ int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, 
  * (for rows > cols the same with A_j = X_j^T X_j on the other side): every singular value s of X_0 becomes
  * p(p(..p(s))), p(s) = a s + b s^3 + c s^5; (3.4445, -4.7750, 2.0315) in 5 steps brings all but the smallest near 1.
  * G = 0 gives X = 0.  G and X have the element type `type`; X may be G itself (same pointer and stride; the
- * shorter side at most 256), otherwise they must not overlap.  The shorter side is at most RS_DENSE_MAX_FACTORS, 1 <= steps <= RS_ORTHO_MAX_STEPS.
- * The polynomials are formed on the shorter side's Gram matrix in fp64, so the table is read twice and written once;
- * with t the largest |p(p(..p(s))) / s|, X is off by a few t 2^-24 of itself at most, plus its rounding. */
+ * shorter side at most 256), otherwise they must not overlap.  The shorter side is at most RS_DENSE_MAX_FACTORS,
+ * 1 <= steps <= RS_ORTHO_MAX_STEPS.
+ * The polynomials are formed on the shorter side's Gram matrix, so the table is read twice and written once.  The Gram
+ * matrix is a sum of fp16 products in fp32, joined in fp64 (RS_TYPE_F32: of pairs, so an element keeps 2^-24 of itself
+ * or 2^-37 of the largest element near it, whichever is more); the polynomials are fp64. */
 #define RS_ORTHO_MAX_STEPS 16
 int rs_orthogonalize_workspace(rs_ctx* ctx, int64_t rows, int64_t cols, int64_t* bytes);
 int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, const void* G, int64_t ldg, int32_t steps, double a,
                      double b, double c, void* X, int64_t ldx, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- the operators on a plan's resident factors (host arrays, as rs_svd_plan_predict) -------------------------- */
+
+/* One training step for ranking: n interactions (inner user, inner item; -1 or out of range = unknown, left out), the
+ * loss is the mean over the m known ones of the softmax cross entropy of p_u . q_i + b_i against all items (GlobalBias and
+ * b_u are the same for every item and play no part).  With g the gradient of that mean:
+ *   p_u -= lr (g_pu + reg (c_u / m) p_u) for every user of the batch, c_u its interactions in it (a user may come several
+ *     times: its gradients are added in batch order)
+ *   b_i -= lr g_bi
+ *   Q   -= q_lr (O + reg Q), O = rs_orthogonalize(g_Q) with 5 steps of (3.4445, -4.7750, 2.0315)
+ * *loss (may be NULL): the mean loss before the step; NaN, and nothing changed, where no interaction is known.  The
+ * call waits for the step.  Needs scratch on the device, kept with the plan: about 3 n_items x n_factors floats
+ * and the batch.  A plan joined to a group is refused (RS_ERR_UNSUPPORTED): its factors are replicas.  n <= 2^20. */
+int rs_svd_plan_rank_step(rs_svd_plan* plan, int64_t n, const int32_t* users, const int32_t* items, double lr, double q_lr,
+                          double reg, double* loss);
+
+/* Scores of n users (inner ids, -1 = unknown) against all items, out[r][i] = GlobalBias + b_u + b_i + p_u . q_i in fp32 (n x
+ * n_items, host), the products in 8 bits: p_u and q_i by rs_quantize_rows (their scales s_p, s_q), so a score is off by at
+ * most sum_f (s_p |q_f| + s_q |p_f|) / 2 + s_p s_q / 4 and fp32 rounding.  Unknown users: GlobalBias + b_i (svd.go:39-48).
+ * The item table is quantised once a call. */
+int rs_svd_plan_score_items(rs_svd_plan* plan, int64_t n, const int32_t* users, float* out);
 
 #ifdef __cplusplus
 }

@@ -1087,6 +1087,12 @@ static void sync_item_copies(rs_svd_plan* pl, hipStream_t s, int32_t mode) {
     }
 }
 
+void plan_factors_changed(rs_svd_plan* pl, hipStream_t s) {
+    reset_loss(pl, s);
+    sync_item_copies(pl, s, 1);
+    RS_HIP(hipGetLastError());
+}
+
 // measured at configs[4] (Zipf head of 3.4M ratings in a 1/8 shard): 8 live copies of such an item
 // diverge to NaN within 5 epochs where 52 averaged copies of 65536 ratings train
 constexpr int64_t kAutoItemCap = 65536;

@@ -186,6 +186,7 @@ struct rs_svd_plan {
     rs::DevBuf<float> loss_part;               // per (workgroup, wave): sum of (lr diff)^2 of the last epoch
     rs::DevBuf<double> loss_state;             // last epoch's training MSE (0: none since the factors were set)
     rs::DevBuf<int32_t> guard_flag;            // the guard's own signals (a rising loss, |p| or |q| >= guard bound): redo, not an error
+    rs::DevBuf<char> rank_ws;                  // rank.hip: workspace of the ranking step and the catalogue scores (grown on demand)
     int32_t soft_refits = 0;                   // redos the guard's own signals alone asked for (the grid is restored after them)
     bool tiles_deferred = false;               // a soft redo restored the caller's grid: rebuilt by the next epochs call
     int32_t own_fx_shift = -1, own_tile_wg = -1;  // while joined: the plan's own shift and grid (rs_svd_plan_leave restores them)
@@ -272,6 +273,8 @@ inline int32_t buffer_bytes32(size_t elems, size_t elem_size, const char* what) 
 // sgd.hip
 int32_t fast_ld(int32_t k);            // row stride of the FAST plans (k factors + bias, 64-float lines)
 void plan_sync_last(rs_svd_plan* pl);  // waits for the stream of the last enqueued epochs
+// factors written outside an epoch: the item copies follow, the guard's loss history starts over
+void plan_factors_changed(rs_svd_plan* pl, hipStream_t s);
 bool plan_range_ok(rs_svd_plan* pl);   // P and Q finite and below the guard bound (syncs the stream)
 int32_t* numflag(rs_svd_plan* pl);  // the RS_ERR_NUMERIC device flag (allocated on first use)
 void q_convert(rs_svd_plan* pl, hipStream_t s, int32_t to_fixed);  // Q <-> int32 fixed point in place

@@ -724,6 +724,27 @@ class SvdPlan:
         self.ctx.check(lib().rs_svd_plan_predict(self.h, len(u), _ptr(u), _ptr(i), _ptr(out)))
         return out
 
+    def rank_step(self, users, items, lr=1.0, q_lr=0.02, reg=0.0):
+        """One training step for ranking on the resident factors (rs_svd_plan_rank_step): softmax cross entropy of the
+        interactions (inner ids, -1 = unknown) over the whole catalogue, SGD on the users' rows and the item biases, an
+        orthogonalised update of the item table.  Returns the mean loss before the step (NaN: no known interaction)."""
+        u, i = np.ascontiguousarray(users, np.int32), np.ascontiguousarray(items, np.int32)
+        if u.shape != i.shape or u.ndim != 1:
+            raise ValueError("users and items must be two lists of the same length")
+        loss = _dbl(0)
+        self.ctx.check(lib().rs_svd_plan_rank_step(self.h, len(u), _ptr(u), _ptr(i), lr, q_lr, reg, C.byref(loss)))
+        return loss.value
+
+    def score_items(self, users):
+        """Every item's score for each user (inner ids, -1 = unknown), float32 n x n_items: svd.go:32-51 with the
+        product in 8 bits (rs_svd_plan_score_items)."""
+        u = np.ascontiguousarray(users, np.int32)
+        if u.ndim != 1:
+            raise ValueError("users must be a list of ids")
+        out = np.empty((len(u), self.n_items), np.float32)
+        self.ctx.check(lib().rs_svd_plan_score_items(self.h, len(u), _ptr(u), _ptr(out)))
+        return out
+
     def evaluate(self, users, items, ratings):
         """(RMSE, MAE) over a test set (utils.go:162-180) on the device."""
         u, i = np.ascontiguousarray(users, np.int32), np.ascontiguousarray(items, np.int32)

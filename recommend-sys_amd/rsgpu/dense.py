@@ -24,6 +24,8 @@ SIGNATURES = {
     "rs_i8_matmul": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "rs_orthogonalize_workspace": (C.c_int, [_vp, _i64, _i64, C.POINTER(_i64)]),
     "rs_orthogonalize": (C.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _i32, _dbl, _dbl, _dbl, _vp, _i64, _vp, _i64, _vp]),
+    "rs_svd_plan_rank_step": (C.c_int, [_vp, _i64, _vp, _vp, _dbl, _dbl, _dbl, C.POINTER(_dbl)]),
+    "rs_svd_plan_score_items": (C.c_int, [_vp, _i64, _vp, _vp]),
 }
 
 # torch, the library and the element types, set by the first call (this module imports neither)

@@ -1,0 +1,176 @@
+"""The dense operators on a plan's resident factors: the ranking step (loss, gradient and orthogonalised update together)
+against the same step in 64 bits, the catalogue's scores against the plan's own predictions, and both among epochs."""
+import math
+
+import numpy as np
+import pytest
+
+import rsgpu
+
+COEF = (3.4445, -4.7750, 2.0315)
+U32 = 2.0 ** -24
+
+
+def make_plan(ctx, n_users=60, n_items=90, k=20, nnz=1500, seed=0):
+    rng = np.random.default_rng(seed)
+    u = rng.integers(0, n_users, nnz).astype(np.int32)
+    i = np.minimum(rng.geometric(0.05, nnz) - 1, n_items - 1).astype(np.int32)
+    r = rng.integers(1, 6, nnz).astype(np.float64)
+    plan = ctx.svd_plan(rsgpu.Ratings(u, i, r, n_users, n_items), k)
+    P, Q = rng.normal(0, 0.5, (n_users, k)), rng.normal(0, 0.5, (n_items, k))
+    plan.upload(P.astype(np.float32), Q.astype(np.float32), rng.normal(0, 0.2, n_users).astype(np.float32),
+                rng.normal(0, 0.2, n_items).astype(np.float32), 3.5)
+    return plan
+
+
+def orthogonalized(G):
+    X = G / np.linalg.norm(G)
+    a, b, c = COEF
+    for _ in range(5):
+        A = X.T @ X if X.shape[0] >= X.shape[1] else X @ X.T
+        M = b * A + c * A @ A
+        X = a * X + (X @ M if X.shape[0] >= X.shape[1] else M @ X)
+    return X
+
+
+def reference_step(P, Q, bi, users, items, lr, q_lr, reg):
+    ok = (users >= 0) & (users < len(P)) & (items >= 0) & (items < len(Q))
+    u, t = users[ok], items[ok]
+    m = len(u)
+    H = P[u]
+    z = H @ Q.T + bi
+    z -= z.max(1, keepdims=True)
+    lse = np.log(np.exp(z).sum(1))
+    loss = float((lse - z[np.arange(m), t]).mean())
+    c = np.exp(z - lse[:, None])
+    c[np.arange(m), t] -= 1
+    c /= m
+    gP = np.zeros_like(P)
+    np.add.at(gP, u, c @ Q)
+    cnt = np.bincount(u, minlength=len(P))
+    gQ, gb = c.T @ H, c.sum(0)
+    P1 = P - lr * (gP + reg * (cnt / m)[:, None] * P)
+    return loss, P1, Q - q_lr * (orthogonalized(gQ) + reg * Q), bi - lr * gb, gP, gQ
+
+
+def logit_bound(P, Q, bi):
+    """Logits of up to L, products of k terms and a bias in fp32 (operands rounded from pairs: one more step each)."""
+    k = P.shape[1]
+    return (k + 10) * U32 * (np.abs(P).max() * np.abs(Q).max() * k + np.abs(bi).max() + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [5, 20, 100])
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_step_against_64_bits(ctx, n, k):
+    plan = make_plan(ctx, k=k)
+    rng = np.random.default_rng(n)
+    users, items = rng.integers(0, 60, n).astype(np.int32), rng.integers(0, 90, n).astype(np.int32)
+    if n > 1:
+        users[3], items[5], users[7], items[9] = -1, -1, 60, 90   # unknown
+        users[10:14] = users[10]                                  # one user several times
+    P, Q, bu, bi, gb = plan.download()
+    lr, q_lr, reg = 0.7, 0.05, 0.01
+    loss, P1, Q1, b1, gP, gQ = reference_step(P, Q, bi, users, items, lr, q_lr, reg)
+    got = plan.rank_step(users, items, lr, q_lr, reg)
+    Pg, Qg, bug, big, gbg = plan.download()
+    # logits off by e; a gradient's coefficients by 2 e + 8 u32 of themselves, its sums by their length's roundings, a
+    # row's coefficients sum to at most 2 weight; a step adds four roundings of the row
+    e = logit_bound(P, Q, bi)
+    assert abs(got - loss) <= 2 * e + 4 * U32 * loss
+    rel = 2 * e + (n + 98) * U32
+    assert np.abs(Pg - P1).max() <= lr * rel * 2 * np.abs(Q).max() + 6 * U32 * np.abs(P1).max()
+    assert np.abs(big - b1).max() <= lr * rel * 2 + 6 * U32
+    # the update of the items: its gradient's relative error is carried by the polynomials to at most a^5 of the weakest
+    # direction's share; the errors of the gradient are random, so against its norm they are e-sized
+    O, Og = (Q - Q1) / q_lr - reg * Q, (Q - Qg) / q_lr - reg * Q
+    assert np.linalg.norm(Og - O) <= (COEF[0] ** 5 * rel + 8 * U32 * np.sqrt(O.size) * np.abs(Q).max() / q_lr / np.linalg.norm(O)) * np.linalg.norm(O)
+    assert np.array_equal(bu, bug) and gb == gbg
+    untouched = np.setdiff1d(np.arange(60), users)
+    assert np.array_equal(P[untouched], Pg[untouched])
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_steps_between_epochs(ctx):
+    """Epochs, steps and scores on one plan, as a program mixes them: everything stays finite and each call sees the
+    factors that the one before left."""
+    plan = make_plan(ctx, k=16)
+    rng = np.random.default_rng(3)
+    users, items = rng.integers(0, 60, 200).astype(np.int32), rng.integers(0, 90, 200).astype(np.int32)
+    plan.epochs(2)
+    for _ in range(3):
+        P, Q, bu, bi, gb = plan.download()
+        want = reference_step(P, Q, bi, users, items, 1.0, 0.02, 0.0)[0]
+        got = plan.rank_step(users, items)
+        assert abs(got - want) <= 2 * logit_bound(P, Q, bi) + 4 * U32 * want
+        plan.epochs(1)
+    out = plan.score_items(np.arange(60))
+    assert np.isfinite(out).all()
+    assert all(np.isfinite(x).all() for x in plan.download()[:4])
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_item_copies_follow_a_step(ctx):
+    """The hybrid schedule keeps copies of hot items' rows: after a step they hold the stepped rows (an epoch that learns
+    nothing leaves the factors as they are, up to its fixed point of 2^-24)."""
+    plan = make_plan(ctx, k=12, nnz=4000)
+    plan.set_mode(rsgpu.WB_ATOMIC)
+    plan.set_hot_replicas(16, 4)
+    plan.epochs(1)
+    users = np.arange(40, dtype=np.int32)
+    plan.rank_step(users, (users * 2).astype(np.int32), q_lr=0.5)
+    before = plan.download()
+    plan.epochs(1, lr=0.0, reg=0.0)
+    after = plan.download()
+    for a, b in zip(before[:4], after[:4]):
+        assert np.abs(a - b).max() <= 2.0 ** -24
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_nothing_known(ctx):
+    plan = make_plan(ctx)
+    before = plan.download()
+    assert math.isnan(plan.rank_step([], []))
+    assert math.isnan(plan.rank_step([-1, 60, 3], [4, 4, 90]))
+    for a, b in zip(before, plan.download()):
+        assert np.array_equal(a, b)
+    assert plan.score_items([]).shape == (0, 90)
+    with pytest.raises(ValueError):
+        plan.rank_step([1, 2], [3])
+    with pytest.raises(rsgpu.RsError):
+        plan.rank_step([1], [2], lr=math.nan)
+    with pytest.raises(rsgpu.RsError):
+        plan.rank_step([1], [2], q_lr=1e300)  # finite, but no float
+    with pytest.raises(rsgpu.RsError):
+        plan.rank_step(np.zeros((1 << 20) + 1, np.int32), np.zeros((1 << 20) + 1, np.int32))
+    for a, b in zip(before, plan.download()):
+        assert np.array_equal(a, b)
+    plan.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k", [(1, 20), (30, 7), (200, 100)])
+def test_scores_against_predictions(ctx, n, k):
+    plan = make_plan(ctx, k=k)
+    rng = np.random.default_rng(n)
+    users = rng.integers(-1, 62, n).astype(np.int32)  # some unknown
+    out = plan.score_items(users).astype(np.float64)
+    P, Q, bu, bi, gb = plan.download()
+    want = np.stack([plan.predict(np.full(90, u, np.int32), np.arange(90, dtype=np.int32)) for u in users])
+    known = (users >= 0) & (users < 60)
+    p = np.where(known[:, None], P[np.clip(users, 0, 59)], 0)
+    sp, sq = np.abs(p).max(1) / 127, np.abs(Q).max(1) / 127
+    bound = (sp[:, None] * np.abs(Q).sum(1) + np.abs(p).sum(1)[:, None] * sq) / 2 + k * sp[:, None] * sq / 4
+    bound = bound * (1 + 1e-6) + 8 * U32 * (np.abs(want) + np.abs(p) @ np.abs(Q).T + 5)
+    assert (np.abs(out - want) <= bound).all()
+    assert np.array_equal(out[~known], np.broadcast_to((np.float32(gb) + bi.astype(np.float32)).astype(np.float64), (int((~known).sum()), 90)))
+    plan.close()
+
+
+def test_entry_point_refusals():
+    L = rsgpu.lib()
+    assert L.rs_svd_plan_rank_step(None, 0, None, None, 0.1, 0.1, 0.0, None) == rsgpu.RS_ERR_INVALID
+    assert L.rs_svd_plan_score_items(None, 0, None, None) == rsgpu.RS_ERR_INVALID
