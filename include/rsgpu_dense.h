@@ -13,7 +13,7 @@
  * free for other use once the call's kernels have run, and two calls that may overlap need a workspace each.  The
  * caller's current device is put back before a call returns.  Calls whose sizes leave nothing to do return RS_OK
  * without a launch.  Sums are held in fp32, int32 or fp64 and each output is rounded once; results do not depend on
- * timing (no floating-point atomics).  n_factors up to RS_DENSE_MAX_FACTORS. */
+ * timing (no floating-point atomics).  Outputs and ws overlap neither the inputs nor each other.  n_factors up to RS_DENSE_MAX_FACTORS. */
 #ifndef RSGPU_DENSE_H
 #define RSGPU_DENSE_H
 
@@ -47,7 +47,7 @@ extern "C" {
  * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
  * (hi + lo), so an element keeps 2^-24 of itself or 2^-38 of the matrix's largest element, whichever is more;
  * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below.
- * n_items < 2^31, n_rows < 2^31. */
+ * n_rows and n_items from 1 to 2^31 - 1025 (or both 0). */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);
 int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, const void* H, int64_t ldh,
@@ -82,7 +82,8 @@ int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, 
  * 1 <= steps <= RS_ORTHO_MAX_STEPS.
  * The polynomials are formed on the shorter side's Gram matrix, so the table is read twice and written once.  The Gram
  * matrix is a sum of fp16 products in fp32, joined in fp64 (RS_TYPE_F32: of pairs, so an element keeps 2^-24 of itself
- * or 2^-37 of the largest element near it, whichever is more); the polynomials are fp64. */
+ * or 2^-37 of the largest element near it, whichever is more; fewer bits below 2^-114); the polynomials are fp64.  An
+ * infinity or NaN in G makes all of X NaN. */
 #define RS_ORTHO_MAX_STEPS 16
 int rs_orthogonalize_workspace(rs_ctx* ctx, int64_t rows, int64_t cols, int64_t* bytes);
 int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, const void* G, int64_t ldg, int32_t steps, double a,

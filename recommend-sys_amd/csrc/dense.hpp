@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -48,6 +49,14 @@ void with_type(int32_t type, F&& f) {
 
 __host__ __device__ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 __host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+
+// A launch holds fewer than 2^32 threads along an axis: many workgroups (of up to 1024 threads) are laid over two, and a
+// kernel asks for its number (workgroups past the end find no row and leave).
+inline dim3 wide_grid(int64_t workgroups) {
+    const int64_t x = std::min<int64_t>(workgroups, int64_t{1} << 21);
+    return dim3(static_cast<uint32_t>(x), static_cast<uint32_t>(ceil_div(workgroups, x)));
+}
+__device__ __forceinline__ int64_t wide_block() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 // The caller's current device is put back when an operator returns (its tensors may live on another device than the
 // one that is current in the calling thread).
@@ -99,11 +108,11 @@ inline std::string check_matrix(const char* name, const void* p, int64_t cols, i
     return std::string();
 }
 
-// LDS tile of rows of KP 16-bit values: 16-byte chunk c of row r sits at chunk c ^ mix(r), the row's low three bits rotated.  A row-wise read (8
-// rows, one chunk at a time) and a transposing one (4 rows, two neighbouring chunks) then both meet every bank once; c ^ (r mod 16) had neighbouring rows share their chunk pairs
-// (half of the LDS cycles were
-// conflicts).  Byte offset: what a lane adds is one base, the constant part of c goes in
-// by XOR (bits the rows do not reach: by addition), so a few registers hold all the addresses of a tile.
+// LDS tile of rows of KP 16-bit values: 16-byte chunk c of row r sits at chunk c ^ mix(r), the row's low three bits
+// rotated.  A row-wise read (8 rows, one chunk at a time) and a transposing one (4 rows, two neighbouring chunks) then
+// both meet every bank once; c ^ (r mod 16) had neighbouring rows share their chunk pairs (half of the LDS cycles were
+// conflicts).  Byte offset: what a lane adds is one base, the constant part of c goes in by XOR (bits the rows do not
+// reach: by addition), so a few registers hold all the addresses of a tile.
 template <int KP>
 struct LdsTile {
     static constexpr int C = KP / 8, M = C < 16 ? C - 1 : 15;

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict_
     typedef __attribute__((ext_vector_type(16 / sizeof(E)))) E vec;
     constexpr int V = 16 / sizeof(E);
     const int lane = threadIdx.x & 63;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t r = wide_block() * 4 + (threadIdx.x >> 6);
     if (r >= rows) return;
     const E* x = X + r * ldx;
     int8_t* o = q + r * ldq;
@@ -375,7 +375,7 @@ extern "C" int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64
             using E = typename decltype(e)::type;
             const bool vec = (reinterpret_cast<uintptr_t>(X) | static_cast<uintptr_t>(ldx * static_cast<int64_t>(sizeof(E)))) % 16 == 0 &&
                              (reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ldq)) % 8 == 0;
-            const uint32_t blocks = static_cast<uint32_t>(ceil_div(n_rows, 4));
+            const dim3 blocks = wide_grid(ceil_div(n_rows, 4));
             if (vec)
                 quantize_rows_kernel<E, true><<<blocks, 256, 0, st>>>(static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
             else

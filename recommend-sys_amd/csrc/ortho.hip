@@ -694,6 +694,16 @@ void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, d
         apply(integral_constant<int, 512>{}, integral_constant<int, 256>{});
 }
 
+// whether two matrices share memory (columns of one table beside each other do not)
+bool overlap(const void* G, int64_t ldg, const void* X, int64_t ldx, int64_t rows, int64_t cols, int64_t elem) {
+    const uintptr_t g = reinterpret_cast<uintptr_t>(G), x = reinterpret_cast<uintptr_t>(X);
+    const uintptr_t ge = g + ((rows - 1) * ldg + cols) * elem, xe = x + ((rows - 1) * ldx + cols) * elem;
+    if (g >= xe || x >= ge) return false;
+    if (ldg != ldx) return true;
+    const int64_t m = static_cast<int64_t>((x > g ? x - g : g - x) / elem) % ldg;
+    return m < cols || m > ldg - cols;
+}
+
 std::string check_sizes(int64_t rows, int64_t cols) {
     if (rows < 0 || rows > INT32_MAX - 1024) return "rows out of range";
     if (cols < 0 || cols > INT32_MAX - 1024) return "cols out of range";
@@ -727,6 +737,8 @@ extern "C" int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t
     for (const std::string& m : {check_matrix("G", G, cols, ldg, type_size(type)), check_matrix("X", X, cols, ldx, type_size(type))})
         if (!m.empty()) return set_error(ctx, RS_ERR_INVALID, m);
     if (G == X && ldg != ldx) return set_error(ctx, RS_ERR_INVALID, "X is G with another row stride");
+    if (G != X && overlap(G, ldg, X, ldx, rows, cols, type_size(type)))
+        return set_error(ctx, RS_ERR_INVALID, "X overlaps G");
     if (G == X && std::min(rows, cols) > 256) return set_error(ctx, RS_ERR_UNSUPPORTED, "X may be G only where the shorter side is at most 256");
     const OrthoPlan p = make_plan(rows, cols);
     if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");

@@ -16,7 +16,7 @@ namespace {
 __global__ __launch_bounds__(256) void rank_gather_kernel(const float* __restrict__ P, int32_t ld, int32_t k, int32_t n_users, int64_t n,
                                                          const int32_t* __restrict__ users, float* __restrict__ dst) {
     const int lane = threadIdx.x & 63;
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t r = wide_block() * 4 + (threadIdx.x >> 6);
     if (r >= n) return;
     const int32_t u = users[r];
     const bool known = static_cast<uint32_t>(u) < static_cast<uint32_t>(n_users);
@@ -25,14 +25,14 @@ __global__ __launch_bounds__(256) void rank_gather_kernel(const float* __restric
 
 // the bias column of a table
 __global__ __launch_bounds__(256) void rank_bias_kernel(const float* __restrict__ T, int32_t ld, int32_t k, int64_t rows, float* __restrict__ out) {
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t r = wide_block() * 256 + threadIdx.x;
     if (r < rows) out[r] = T[r * ld + k];
 }
 
 // GlobalBias + b_u (unknown users: GlobalBias)
 __global__ __launch_bounds__(256) void rank_row_bias_kernel(const float* __restrict__ P, int32_t ld, int32_t k, int32_t n_users, int64_t n,
                                                            const int32_t* __restrict__ users, const double* __restrict__ gb, float* __restrict__ out) {
-    const int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t r = wide_block() * 256 + threadIdx.x;
     if (r >= n) return;
     const int32_t u = users[r];
     const bool known = static_cast<uint32_t>(u) < static_cast<uint32_t>(n_users);
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void rank_users_kernel(float* __restrict__ P, 
                                                         const int32_t* __restrict__ seg_user, const int32_t* __restrict__ rows, int64_t n_seg,
                                                         const float* __restrict__ dH, float lr, float decay) {
     const int lane = threadIdx.x & 63;
-    const int64_t s = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t s = wide_block() * 4 + (threadIdx.x >> 6);
     if (s >= n_seg) return;
     const int32_t a = seg[s], b = seg[s + 1];
     float* p = P + static_cast<int64_t>(seg_user[s]) * ld;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void rank_users_kernel(float* __restrict__ P, 
 __global__ __launch_bounds__(256) void rank_items_kernel(float* __restrict__ Q, int32_t ld, int32_t k, int64_t n_items, const float* __restrict__ O,
                                                         const float* __restrict__ db, float lr, float q_lr, float reg) {
     const int lane = threadIdx.x & 63;
-    const int64_t v = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t v = wide_block() * 4 + (threadIdx.x >> 6);
     if (v >= n_items) return;
     float* q = Q + v * ld;
     for (int c = lane; c < k; c += 64) q[c] -= q_lr * (O[v * k + c] + reg * q[c]);
@@ -133,17 +133,17 @@ void rank_step(rs_svd_plan* pl, int64_t n, const int32_t* users, const int32_t* 
     up(o_rows, rows.data(), m * 4);
     up(o_seg, seg.data(), (n_seg + 1) * 4);
     up(o_su, seg_user.data(), n_seg * 4);
-    rank_gather_kernel<<<static_cast<uint32_t>(ceil_div(n, 4)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, n, i32(o_users), f(o_h));
+    rank_gather_kernel<<<wide_grid(ceil_div(n, 4)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, n, i32(o_users), f(o_h));
     RS_HIP(hipGetLastError());
-    rank_bias_kernel<<<static_cast<uint32_t>(ceil_div(V, 256)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_bias));
+    rank_bias_kernel<<<wide_grid(ceil_div(V, 256)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_bias));
     RS_HIP(hipGetLastError());
     check(pl, rs_softmax_ce(pl->ctx, RS_TYPE_F32, n, V, k, f(o_h), k, pl->Q.p, ld, f(o_bias), i32(o_tgt), f(o_w), f(o_loss), f(o_lse), f(o_dh), k,
                             f(o_dw), k, f(o_db), ws + o_ws, ce_bytes, nullptr));
     check(pl, rs_orthogonalize(pl->ctx, RS_TYPE_F32, V, k, f(o_dw), k, 5, 3.4445, -4.7750, 2.0315, f(o_x), k, ws + o_ws, or_bytes, nullptr));
-    rank_users_kernel<<<static_cast<uint32_t>(ceil_div(n_seg, 4)), 256, 0, s>>>(pl->P.p, ld, k, i32(o_seg), i32(o_su), i32(o_rows), n_seg, f(o_dh), lr,
+    rank_users_kernel<<<wide_grid(ceil_div(n_seg, 4)), 256, 0, s>>>(pl->P.p, ld, k, i32(o_seg), i32(o_su), i32(o_rows), n_seg, f(o_dh), lr,
                                                                                reg / static_cast<float>(m));
     RS_HIP(hipGetLastError());
-    rank_items_kernel<<<static_cast<uint32_t>(ceil_div(V, 4)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_x), f(o_db), lr, q_lr, reg);
+    rank_items_kernel<<<wide_grid(ceil_div(V, 4)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_x), f(o_db), lr, q_lr, reg);
     RS_HIP(hipGetLastError());
     plan_factors_changed(pl, s);
     std::vector<float> h(static_cast<size_t>(n));
@@ -169,14 +169,14 @@ void score_items(rs_svd_plan* pl, int64_t n, const int32_t* users, float* out) {
     auto i8 = [&](int64_t o) { return reinterpret_cast<int8_t*>(ws + o); };
     RS_HIP(hipMemcpyAsync(ws + o_users, users, static_cast<size_t>(n) * 4, hipMemcpyHostToDevice, s));
     check(pl, rs_quantize_rows(pl->ctx, RS_TYPE_F32, V, k, pl->Q.p, ld, i8(o_q), ldq, f(o_qs), nullptr));
-    rank_bias_kernel<<<static_cast<uint32_t>(ceil_div(V, 256)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_cb));
+    rank_bias_kernel<<<wide_grid(ceil_div(V, 256)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_cb));
     RS_HIP(hipGetLastError());
     for (int64_t r = 0; r < n; r += batch) {
         const int64_t b = std::min(batch, n - r);
         const int32_t* du = reinterpret_cast<int32_t*>(ws + o_users) + r;
-        rank_gather_kernel<<<static_cast<uint32_t>(ceil_div(b, 4)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, b, du, f(o_h));
+        rank_gather_kernel<<<wide_grid(ceil_div(b, 4)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, b, du, f(o_h));
         RS_HIP(hipGetLastError());
-        rank_row_bias_kernel<<<static_cast<uint32_t>(ceil_div(b, 256)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, b, du, pl->gb.p, f(o_rb));
+        rank_row_bias_kernel<<<wide_grid(ceil_div(b, 256)), 256, 0, s>>>(pl->P.p, ld, k, pl->n_users, b, du, pl->gb.p, f(o_rb));
         RS_HIP(hipGetLastError());
         check(pl, rs_quantize_rows(pl->ctx, RS_TYPE_F32, b, k, f(o_h), k, i8(o_hq), ldq, f(o_hs), nullptr));
         check(pl, rs_i8_matmul(pl->ctx, b, V, k, i8(o_hq), ldq, f(o_hs), i8(o_q), ldq, f(o_qs), f(o_rb), f(o_cb), RS_TYPE_F32, f(o_out), V, nullptr));

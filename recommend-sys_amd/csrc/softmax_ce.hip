@@ -92,15 +92,15 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
         const double tile = static_cast<double>(kTileY) * 32 * sh.waves * (p.kp + p.oc) * 2 * (p.np == 2 ? 3 : 1) / (alone ? 3.4e6 : 2.4e6);
         const double sums = static_cast<double>(rows_x) * p.kp * 8 / 8e6;
         double best = 0.0;
-        for (int64_t s = 1; s <= ty && (s == 1 || tx * s <= 4096); ++s) {
-            const int64_t per = ceil_div(ty, s);
-            if (ceil_div(ty, per) != s) continue;
+        for (int64_t s = 1, per = ty; s == 1 || tx * s <= 4096; s = ceil_div(ty, per)) {  // each length of a split once
             const double one = static_cast<double>(per) * tile;
             double cost = alone ? static_cast<double>(ceil_div(tx * s, 256)) * (one + 3.0)
                                 : static_cast<double>(std::max<int64_t>(tx * s, 256)) / 256 * (one + 2.0) + 0.5 * one;
             if (s > 1 || mode != kItems) cost += static_cast<double>(s) * sums;
             if (s > 1 && mode == kItems) cost += 5.0;  // the join's launch
             if (s == 1 || cost < best) best = cost, *splits = static_cast<int32_t>(s), *tiles = static_cast<int32_t>(per);
+            if (per == 1) break;
+            per = ceil_div(ty, ceil_div(ty, per - 1));
         }
     };
     split(n, v, kLossGrad, &p.splits_f, &p.tiles_f);
@@ -552,7 +552,7 @@ template <typename E>
 __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
     const int lane = threadIdx.x & 63;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int64_t n = wide_block() * 4 + (threadIdx.x >> 6);
     const int64_t rows = p.grad ? p.n_pad : p.n;
     if (n >= rows) return;
     const Scal sc = *a.at<Scal>(p.o_scal);
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
     const Scal sc = *a.at<Scal>(p.o_scal);
     const int quads = p.kp / 4;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, v = i / quads;
+    const int64_t i = wide_block() * 256 + threadIdx.x, v = i / quads;
     const int c = static_cast<int>(i % quads) * 4;
     if (v >= p.v || c >= p.k) return;
     const float* O = a.at<float>(p.o_part) + v * p.kp + c;
@@ -712,12 +712,12 @@ void launch_all(const CeArgs& a, hipStream_t st) {
         mode(std::integral_constant<int, kLossGrad>{});
     else
         mode(std::integral_constant<int, kLoss>{});
-    ce_join_kernel<E><<<static_cast<uint32_t>(ceil_div(p.grad ? p.n_pad : p.n, 4)), 256, 0, st>>>(a);
+    ce_join_kernel<E><<<wide_grid(ceil_div(p.grad ? p.n_pad : p.n, 4)), 256, 0, st>>>(a);
     RS_HIP(hipGetLastError());
     if (!p.grad) return;
     mode(std::integral_constant<int, kItems>{});
     if (p.splits_w > 1) {
-        ce_items_join_kernel<E><<<static_cast<uint32_t>(ceil_div(p.v * (p.kp / 4), 256)), 256, 0, st>>>(a);
+        ce_items_join_kernel<E><<<wide_grid(ceil_div(p.v * (p.kp / 4), 256)), 256, 0, st>>>(a);
         RS_HIP(hipGetLastError());
     }
 }

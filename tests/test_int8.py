@@ -105,6 +105,40 @@ def test_quantize_ties_and_borders(ctx):
 
 
 @pytest.mark.gpu
+def test_quantize_many_rows_and_far_rows(ctx):
+    """More rows than one axis of a launch holds waves for, and rows further apart than 32 bits of elements."""
+    n = 2 ** 26 + 77
+    x = (torch.arange(n, device="cuda") % 255 - 127).to(torch.float16)[:, None]
+    q, s = ctx.quantize_rows(x)
+    assert torch.equal(q, (x > 0).to(torch.int8) * 127 - (x < 0).to(torch.int8) * 127)
+    assert torch.equal(s, x[:, 0].abs().float() * torch.tensor(1 / 127, dtype=torch.float32, device="cuda"))
+    del x, q, s
+    far = torch.empty(2 * (2 ** 31 + 16) + 40, dtype=torch.float16, device="cuda").as_strided((3, 40), (2 ** 31 + 16, 1))
+    far.copy_(torch.randn(3, 40, generator=torch.Generator().manual_seed(1)))
+    q, s = ctx.quantize_rows(far)
+    rq, rs = quantize_reference(far)
+    assert torch.equal(q.cpu().long(), rq) and torch.equal(s.cpu(), rs)
+
+
+@pytest.mark.gpu
+def test_product_of_far_rows(ctx):
+    """Rows of A, B and C further apart than 32 bits of elements."""
+    step = 2 ** 31 + 32
+    big = torch.empty(2 * step + 64, dtype=torch.int8, device="cuda")
+    A = big.as_strided((3, 40), (step, 1))
+    A.copy_(codes(3, 40, 1))
+    sa, sb = scales(3, 2), scales(70, 3)
+    B = codes(70, 40, 4)
+    near = ctx.i8_matmul(A.contiguous(), sa, B, sb)
+    assert torch.equal(ctx.i8_matmul(A, sa, B, sb), near)
+    assert torch.equal(ctx.i8_matmul(B, sb, A, sa), near.T)
+    out = torch.empty(2 * step + 70, dtype=torch.float16, device="cuda").as_strided((3, 70), (step, 1))
+    ctx.check(rsgpu.lib().rs_i8_matmul(ctx.h, 3, 70, 40, A.data_ptr(), step, sa.data_ptr(), B.data_ptr(), 40, sb.data_ptr(), None, None,
+                                       rsgpu.dense.TYPE_F16, out.data_ptr(), step, rsgpu.dense.STREAM_DEFAULT))
+    assert torch.equal(out, near.half())
+
+
+@pytest.mark.gpu
 def test_quantize_strided_leaves_the_rest(ctx):
     x = torch.randn(6, 40, device="cuda")
     q, s = ctx.quantize_rows(x[:, 1:30])

@@ -154,6 +154,29 @@ def test_strided_in_place_and_beside(ctx, rows, cols):
 
 
 @pytest.mark.gpu
+def test_rows_far_apart(ctx):
+    """Rows of G and X further apart than 32 bits of elements."""
+    step = 2 ** 31 + 8
+    big = torch.empty(2 * step + 64, dtype=torch.float16, device="cuda")
+    G, X = big.as_strided((3, 20), (step, 1)), big.as_strided((3, 20), (step, 1), 32)
+    G.copy_(torch.randn(3, 20, generator=torch.Generator().manual_seed(1)))
+    ctx.orthogonalize(G, out=X)
+    assert torch.equal(X, ctx.orthogonalize(G.contiguous()))
+
+
+@pytest.mark.gpu
+def test_columns_beside_and_overlapping(ctx):
+    big = torch.randn(60, 50, device="cuda")
+    G = big[:, :20]
+    want = ctx.orthogonalize(G)
+    assert torch.equal(ctx.orthogonalize(G, out=big[:, 20:40]), want) and torch.equal(ctx.orthogonalize(G, out=big[:, 30:]), want)
+    for bad in (big[:, 1:21], big[:, 19:39], big[1:, :20]):
+        with pytest.raises(rsgpu.RsError):
+            ctx.orthogonalize(G[:len(bad)], out=bad)
+    assert torch.equal(ctx.orthogonalize(big[:30, :20], out=big[30:, :20]), ctx.orthogonalize(big[:30, :20]))
+
+
+@pytest.mark.gpu
 def test_transposed_update(ctx):
     """A tall update and its transpose are the same operator: equal up to the order of the sums."""
     G = update(500, 90, "f32", seed=9)

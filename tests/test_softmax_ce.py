@@ -284,6 +284,53 @@ def test_gradient_against_differences(ctx):
 
 
 @pytest.mark.gpu
+def test_many_rows(ctx):
+    """More rows than one axis of a launch holds waves for.  Two items of one factor: l = h w_v, p = sigmoid.  A few fp32
+    roundings of lse; a coefficient's 2^-11 and half a step of bf16 for dH; the sums of dW and dbias besides by a rounding
+    for each of at most 2^26 / 16 products of a split, which stay below 2^-11 of the sum of magnitudes too."""
+    n = 2 ** 26 + 300
+    h = (torch.randn(n, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) / 4).bfloat16()
+    W = torch.tensor([[0.5], [-1.25]], device="cuda").bfloat16()
+    target = (torch.arange(n, device="cuda") % 3 - 1).int()
+    loss, lse, dH, dW, db = ctx.softmax_ce(h[:, None], W, target, grad=True)
+    dW, db = dW.double(), db.double()
+    w = W.double()[:, 0]
+    gw, gb, mag = torch.zeros(2, dtype=torch.float64, device="cuda"), torch.zeros(2, dtype=torch.float64, device="cuda"), 0.0
+    for a in range(0, n, 1 << 24):
+        x, t = h[a:a + (1 << 24)].double(), target[a:a + (1 << 24)].long()
+        there = t >= 0
+        l = x[:, None] * w
+        z = torch.logsumexp(l, 1)
+        assert ((lse[a:a + (1 << 24)] - z * there).abs() <= 16 * 2.0 ** -24 * (1 + l.abs().amax(1))).all()
+        lt = l.gather(1, t.clamp(min=0)[:, None])[:, 0]
+        assert ((loss[a:a + (1 << 24)] - (z - lt) * there).abs() <= 16 * 2.0 ** -24 * (1 + l.abs().amax(1))).all()
+        c = (torch.exp(l - z[:, None]) - torch.nn.functional.one_hot(t.clamp(min=0), 2)) * there[:, None]
+        d = (c * w).sum(1)
+        assert ((dH[a:a + (1 << 24), 0] - d).abs() <= 2.0 ** -8 * d.abs() + 2.0 ** -10 * w.abs().sum()).all()
+        gw += (x[:, None] * c).sum(0)
+        gb += c.sum(0)
+        mag += float((c.abs() * (1 + x.abs()[:, None])).sum())
+    assert ((dW[:, 0] - gw).abs() <= 2.0 ** -8 * gw.abs() + 2.0 ** -10 * mag).all()
+    assert ((db - gb).abs() <= 2.0 ** -10 * mag).all()
+
+
+@pytest.mark.gpu
+def test_rows_far_apart(ctx):
+    """Rows of H and W further apart than 32 bits of elements."""
+    step = 2 ** 31 + 8
+    big = torch.empty(2 * step + 64, dtype=torch.float16, device="cuda")
+    far = big.as_strided((3, 20), (step, 1))
+    far.copy_(torch.randn(3, 20, generator=torch.Generator().manual_seed(1)))
+    W = torch.randn(70, 20, generator=torch.Generator().manual_seed(2)).half().cuda()
+    target = torch.tensor([4, 69, 0], dtype=torch.int32, device="cuda")
+    for x, y in zip(ctx.softmax_ce(far, W, target, grad=True), ctx.softmax_ce(far.contiguous(), W, target, grad=True)):
+        assert torch.equal(x, y)
+    target = torch.arange(70, dtype=torch.int32, device="cuda") % 3
+    for x, y in zip(ctx.softmax_ce(W, far, target, grad=True), ctx.softmax_ce(W, far.contiguous(), target, grad=True)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
 def test_same_call_same_bits(ctx):
     H, W, target, b, w = make(300, 5000, 48, "f32", seed=13, bias=True)
     one = ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True)
