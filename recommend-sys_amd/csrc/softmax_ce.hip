@@ -367,7 +367,6 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
         // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the block
         float off = 0.f;
         bool here = false;
-        int tg = 0;
         if constexpr (!items) {
             float top = -INFINITY;
 #pragma unroll
@@ -395,8 +394,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             off = m_run == -INFINITY ? 0.f : m_run - shift_of(m_run);
         } else {
             // which of the rows have their target among the wave's columns (few: one in items / 32)
-            tg = __float_as_int(mt[2 * ROWS + lx]) - static_cast<int>(x0);
-            here = __any(static_cast<uint32_t>(tg) < 32u);
+            here = __any(static_cast<uint32_t>(__float_as_int(mt[2 * ROWS + lx]) - static_cast<int>(x0)) < 32u);
         }
         // f(S) and its product.  Wide rows leave few registers: 16 rows of the block at a time (KP = 256: the items'
         // pass 2001 -> 1536 us); otherwise all 32, which gives the scheduler more to run beside the products (KP = 128:
@@ -420,9 +418,11 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                 }
                 if (here) {
 #pragma unroll
-                    for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) {
-                        const int row = 8 * (i / 4) + 4 * half + i % 4;
-                        if (__shfl(tg, row) == lx) s[i] -= mt[3 * ROWS + row];
+                    for (int q = Q * h; q < Q * h + Q; ++q) {
+                        const i32x4 t = *reinterpret_cast<const i32x4*>(mt + 2 * ROWS + 8 * q + 4 * half);
+                        const f32x4 w = *reinterpret_cast<const f32x4*>(mt + 3 * ROWS + 8 * q + 4 * half);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[4 * q + e] -= t[e] == static_cast<int>(x) ? w[e] : 0.f;
                     }
                 }
             } else {
@@ -558,19 +558,21 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     const Scal sc = *a.at<Scal>(p.o_scal);
     const bool known = row_known(a, n);
     const float *pm = a.at<float>(p.o_m) + n, *ps = a.at<float>(p.o_s) + n;
-    float m = -INFINITY, s = 0.f;
-    if (known)
-        for (int i = lane; i < p.splits_f; i += 64) m = fmaxf(m, pm[i * p.n_pad]);
-#pragma unroll
-    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (known)
-        for (int i = lane; i < p.splits_f; i += 64) {
-            const float mi = pm[i * p.n_pad], si = ps[i * p.n_pad];
-            s += m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi));
-        }
-    s = wave_sum_f32(s);
+    // (the first 64 splits' values and the target's are asked for together)
+    const float m0 = lane < p.splits_f ? pm[lane * p.n_pad] : -INFINITY, s0 = lane < p.splits_f ? ps[lane * p.n_pad] : 0.f;
     const int32_t tg = known ? a.target[n] : 0;
     const bool there = known && item_there(a, tg);
+    float m = known ? m0 : -INFINITY, s = 0.f;
+    if (known)
+        for (int i = lane + 64; i < p.splits_f; i += 64) m = fmaxf(m, pm[i * p.n_pad]);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    auto share = [&](float mi, float si) { return m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi)); };
+    if (known) {
+        if (lane < p.splits_f) s = share(m0, s0);
+        for (int i = lane + 64; i < p.splits_f; i += 64) s += share(pm[i * p.n_pad], ps[i * p.n_pad]);
+    }
+    s = wave_sum_f32(s);
     const E *h = static_cast<const E*>(a.H) + n * a.ldh, *wt = static_cast<const E*>(a.W) + tg * a.ldw;
     float lt = 0.f;
     if (there)
@@ -608,7 +610,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
                 // the factors of 64 splits, one a lane
                 float f = 0.f;
                 if (i0 + lane < p.splits_f) {
-                    const float mi = pm[(i0 + lane) * p.n_pad];
+                    const float mi = i0 ? pm[(i0 + lane) * p.n_pad] : m0;
                     f = __builtin_amdgcn_exp2f((mi - m) - shift_of(mi));
                 }
                 const int count = min(64, p.splits_f - i0);
@@ -635,17 +637,21 @@ template <typename E>
 __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
     const Scal sc = *a.at<Scal>(p.o_scal);
-    const int quads = p.kp / 4;
-    const int64_t i = wide_block() * 256 + threadIdx.x, v = i / quads;
-    const int c = static_cast<int>(i % quads) * 4;
+    const int quads = p.kp / 4;  // (a power of two)
+    const int64_t i = wide_block() * 256 + threadIdx.x, v = i >> __builtin_ctz(quads);
+    const int c = (static_cast<int>(i) & (quads - 1)) * 4;
     if (v >= p.v || c >= p.k) return;
     const float* O = a.at<float>(p.o_part) + v * p.kp + c;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < p.splits_w; ++s) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(O + s * p.v_pad * p.kp);
+    // eight splits' loads at a time: a split is read where it was just written, far from this CU
+    for (int s0 = 0; s0 < p.splits_w; s0 += 8) {
+        f32x4 x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += x[e];
+        for (int s = 0; s < 8; ++s) x[s] = s0 + s < p.splits_w ? *reinterpret_cast<const f32x4*>(O + (s0 + s) * p.v_pad * p.kp) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += x[s][e];
     }
     E* out = static_cast<E*>(a.dW) + v * a.lddw;
 #pragma unroll
@@ -687,7 +693,7 @@ void launch_all(const CeArgs& a, hipStream_t st) {
         const int64_t step = 256 / (p.kp / 8);  // rows of a block at a time
         int blocks = 0;
         if (!std::is_same<E, _Float16>::value || (p.grad && a.weight)) {
-            blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), 4 * step)));
+            blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), step)));
             ce_max_kernel<E, VEC><<<dim3(static_cast<uint32_t>(blocks), 3), 256, 0, st>>>(a);
             RS_HIP(hipGetLastError());
         }
