@@ -1,10 +1,13 @@
 // softmax_ce.hip -- softmax cross entropy over the item catalogue and its gradient, no logits kept (gfx950).
 //
 // Mathematics.  With x the "stationary" rows held by a wave and y the rows that stream past:
-//   forward: x = users' rows, y = items.  S[y, x] = W_y . H_x; a running maximum m_x and sum s_x of 2^(l2 - m_x), l2 the
-//     logit in base 2, and (for the gradient) O_x = sum_y 2^(l2 - m_x) W_y, all three rescaled when m_x grows.  So one
-//     pass over the catalogue gives lse and dH = weight (O / s - W_target).
-//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - m_y) / s_y - [target]) and dW_x += sum_y c H_y.
+//   forward: x = users' rows, y = items but the row's target.  S[y, x] = W_y . H_x; a running maximum m_x and sum s_x of
+//     2^(l2 - m_x), l2 the logit in base 2, and (for the gradient) O_x = sum_y 2^(l2 - m_x) W_y, all three rescaled when
+//     m_x grows.  The target joins at the end: with its own term t = 2^(l2_target - m_x), one pass over the catalogue
+//     gives lse and dH = weight (O - s W_target) / (s + t).  (With the target inside the sums dH would be the difference
+//     O / (s + t) - W_target of two near vectors where its probability is near one: 2^-12 of W_target, against 2^-12 of
+//     dH; the loss keeps its small values in the same way.)
+//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - m_y) / (s_y + t_y) - [target]) and dW_x += sum_y c H_y.
 // Both are one kernel: S = Y X^T, then acc[k, x] += Y^T f(S).  S comes out of the matrix unit with x over lanes and y
 // over registers, which is (up to an order of y, the same for both operands) what the second product takes as its
 // second operand: f(S) never leaves the registers.  Its first operand Y^T comes from the same LDS tile as Y by
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     constexpr int ROWS = 32 * SUB;                         // rows of a stage
     constexpr int PIECE = ROWS * KP;                       // elements of one piece of a stage
     constexpr int CHUNKS = ROWS * C * NP, PER = (CHUNKS + THREADS - 1) / THREADS;
-    constexpr int NM = items ? 4 : 1;                      // values per streamed row: bias, or m, weight / s, target, weight
+    constexpr int NM = items ? 4 : 1;                      // values per streamed row: bias, or m, weight / s, target, its coefficient
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // smem: [2][NP][ROWS][KP] fp16
     float* meta = reinterpret_cast<float*>(smem + 2 * NP * PIECE * 2);  // [2][NM][ROWS]
@@ -339,6 +342,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{0};
     float m_run = -INFINITY, sum = 0.f;
     const float bias_x = items ? a.at<float>(p.o_bias)[x] : 0.f;
+    const int target_x = !items && x < p.n ? a.target[x] : -1;
 
     // row-wise reads: row lx, chunk half + 2 ks.  Transposing reads hand lane i of a group of 16 the column i of the
     // 4 x 16 block whose rows its lanes address: row 4 half + (i / 4) of 8, chunk 2 (group mod 2) + (i mod 4) / 2.
@@ -346,14 +350,26 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     const int tr_row = 4 * half + (g4 >> 2), tr_chunk = oc0 / 8 + 2 * ((lane >> 4) & 1) + ((g4 & 3) >> 1);
     const int tr_base[2] = {LdsTile<KP>::base(tr_row, tr_chunk) + (g4 & 1) * 8, LdsTile<KP>::base(tr_row + 8, tr_chunk) + (g4 & 1) * 8};
 
-    // 32 streamed rows: the byte offset of their LDS tile and their values
-    auto block = [&](int tile, const float* mt) {
+    // 32 streamed rows from first_y on: the byte offset of their LDS tile and their values
+    auto block = [&](int first_y, int tile, const float* mt) {
         // the tile's offset has none of the bits that the chunks are mixed in: it joins the bases.  Wide rows take the
         // addresses anew for every block, or the compiler keeps all of them in registers and spills others (KP = 256: 168
         // bytes, 1221 / 2067 us against 1072 / 1215); narrow ones keep them (KP = 128: 126 us against 154)
         int rb = row_base + tile, tb[2] = {tr_base[0] + tile, tr_base[1] + tile};
         if (KP >= 256) asm volatile("" : "+v"(rb), "+v"(tb[0]), "+v"(tb[1]));
         f32x16 s = f32x16{0};
+        // A lane's target is not for these sums: its logit becomes -inf.  Asked for between the products where the registers
+        // allow it (8192 x 26744 x 128 without gradients: 100 us, 108 in the maximum's branch, 99 if it were left in),
+        // otherwise in the maximum's branch (1024 x 1e6 x 256 with gradients: 2440 us; 2472 between the products and the
+        // maximum, 2513 early, 2418 if it were left in)
+        constexpr bool kEarly = !items && NP * KP < 256;
+        const bool target_here = !items && __any(static_cast<uint32_t>(target_x - first_y) < 32u);
+        auto leave_out = [&] {
+            if (!target_here) return;
+            const int tg = target_x - first_y - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = tg == 8 * (i / 4) + i % 4 ? -INFINITY : s[i];
+        };
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const f16x8 y0 = *reinterpret_cast<const f16x8*>(smem + LdsTile<KP>::at(rb, ks * 2));
@@ -363,6 +379,8 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                 s = mfma16(y0, xf[1][ks], s);
                 s = mfma16(y1, xf[0][ks], s);
             }
+            if constexpr (kEarly)
+                if (ks == 0) leave_out();
         }
         // lane: column x; register i: row y = 8 (i / 4) + 4 half + i mod 4 of the block
         float off = 0.f;
@@ -380,16 +398,26 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                 }
             }
             top = fmaxf(top, __shfl_xor(top, 32));
-            if (__any(top > m_run + kLag)) {  // the first block, and rarely after it
-                const float m_new = top > m_run + kLag ? top : m_run;
-                const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) + (shift_of(m_new) - shift_of(m_run)));
-                m_run = m_new;
-                sum *= f;
-                if constexpr (MODE == kLossGrad)
+            const bool over = __any(top > m_run + kLag);  // the first block, and rarely after it
+            if (over || (!kEarly && target_here)) {
+                if constexpr (!kEarly) leave_out();
+                if (over) {
+                    if constexpr (!kEarly) {
+                        top = s[0];
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+                        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+                        top = fmaxf(top, __shfl_xor(top, 32));
+                    }
+                    const float m_new = top > m_run + kLag ? top : m_run;
+                    const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) + (shift_of(m_new) - shift_of(m_run)));
+                    m_run = m_new;
+                    sum *= f;
+                    if constexpr (MODE == kLossGrad)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                }
             }
             off = m_run == -INFINITY ? 0.f : m_run - shift_of(m_run);
         } else {
@@ -422,7 +450,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                         const i32x4 t = *reinterpret_cast<const i32x4*>(mt + 2 * ROWS + 8 * q + 4 * half);
                         const f32x4 w = *reinterpret_cast<const f32x4*>(mt + 3 * ROWS + 8 * q + 4 * half);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[4 * q + e] -= t[e] == static_cast<int>(x) ? w[e] : 0.f;
+                        for (int e = 0; e < 4; ++e) s[4 * q + e] = t[e] == static_cast<int>(x) ? w[e] : s[4 * q + e];
                     }
                 }
             } else {
@@ -477,7 +505,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
         const int b = (t - t0) & 1;
         if (t + 1 < t1) fetch(t + 1);
 #pragma unroll
-        for (int sub = 0; sub < SUB; ++sub) block(b * NP * PIECE * 2 + sub * (64 * KP), meta + b * NM * ROWS + sub * 32);
+        for (int sub = 0; sub < SUB; ++sub) block(t * ROWS + sub * 32, b * NP * PIECE * 2 + sub * (64 * KP), meta + b * NM * ROWS + sub * 32);
         if (t + 1 < t1) put(b ^ 1);
         __syncthreads();
     }
@@ -567,24 +595,29 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
         for (int i = lane + 64; i < p.splits_f; i += 64) m = fmaxf(m, pm[i * p.n_pad]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    auto share = [&](float mi, float si) { return m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi)); };
-    if (known) {
-        if (lane < p.splits_f) s = share(m0, s0);
-        for (int i = lane + 64; i < p.splits_f; i += 64) s += share(pm[i * p.n_pad], ps[i * p.n_pad]);
-    }
-    s = wave_sum_f32(s);
     const E *h = static_cast<const E*>(a.H) + n * a.ldh, *wt = static_cast<const E*>(a.W) + tg * a.ldw;
     float lt = 0.f;
     if (there)
         for (int c = lane; c < p.k; c += 64) lt = fmaf(static_cast<float>(h[c]), static_cast<float>(wt[c]), lt);
     lt = wave_sum_f32(lt);
-    // every item withdrawn: m stays -inf and s is 0
-    const bool empty = m == -INFINITY && s == 0.f;
-    // lse2 = m + log2 s, in two parts: where m is large they must not be joined before the target's logit goes
-    const float ls = log2f(s), lt2 = there ? lt * kLog2e + a.at<float>(p.o_bias)[tg] : 0.f;
+    // the target's logit in base 2, rounded as the passes round theirs; the maximum over all items
+    const float lt2 = there ? fmaf(lt, kLog2e, a.at<float>(p.o_bias)[tg]) : -INFINITY;
+    const bool first = lt2 >= m;
+    if (first) m = lt2;
+    auto share = [&](float mi, float si) { return m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi)); };
+    if (known) {
+        if (lane < p.splits_f) s = share(m0, s0);
+        for (int i = lane + 64; i < p.splits_f; i += 64) s += share(pm[i * p.n_pad], ps[i * p.n_pad]);
+    }
+    const float rest = wave_sum_f32(s);  // the others' sum
+    // every item withdrawn: m stays -inf and the sum is 0
+    const bool empty = m == -INFINITY && rest == 0.f;
+    s = there ? rest + __builtin_amdgcn_exp2f(lt2 - m) : rest;
+    // lse = m ln 2 + ls, in two parts: where m is large they must not be joined before the target's logit goes
+    const float ls = first ? log1pf(rest) : log2f(s) * kLn2;
     if (lane == 0 && n < p.n) {
-        a.lse[n] = !known ? 0.f : empty ? -INFINITY : fmaf(m, kLn2, ls * kLn2);
-        a.loss[n] = !known || empty ? 0.f : there ? ((m - lt2) + ls) * kLn2 : INFINITY;
+        a.lse[n] = !known ? 0.f : empty ? -INFINITY : fmaf(m, kLn2, ls);
+        a.loss[n] = !known || empty ? 0.f : there ? fmaf(m - lt2, kLn2, ls) : INFINITY;
     }
     if (!p.grad) return;
     const bool live = there && !empty;
@@ -594,11 +627,11 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
         row[0] = live ? m : INFINITY;
         row[p.n_pad] = live ? w * sc.cs / s : 0.f;
         row[2 * p.n_pad] = __int_as_float(live ? tg : -1);
-        row[3 * p.n_pad] = w * sc.cs;
+        row[3 * p.n_pad] = live ? -w * sc.cs * (rest / s) : 0.f;  // the target's coefficient, weight (p - 1)
     }
     if (n >= p.n) return;
     E* out = static_cast<E*>(a.dH) + n * a.lddh;
-    const float inv = sc.inv_w / s;
+    const float inv = sc.inv_w / s, share_rest = rest / s;
     // four columns a lane; where a row has fewer than 256, groups of lanes share the splits
     const int quads = p.kp / 4, lanes = quads < 64 ? quads : 64, groups = 64 / lanes, grp = lane / lanes;
     const float* O = a.at<float>(p.o_part) + n * p.kp;
@@ -628,7 +661,7 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
         if (grp == 0)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < p.k) out[c + e] = static_cast<E>(live ? w * (o[e] * inv - static_cast<float>(wt[c + e])) : 0.f);
+                if (c + e < p.k) out[c + e] = static_cast<E>(live ? w * (o[e] * inv - share_rest * static_cast<float>(wt[c + e])) : 0.f);
     }
 }
 

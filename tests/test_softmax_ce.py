@@ -284,6 +284,42 @@ def test_gradient_against_differences(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("v,k,top", [(2, 33, 4.0), (9, 64, 8.0), (300, 20, 12.0), (500, 100, 16.0)])
+def test_rows_that_are_nearly_learnt(ctx, ty, v, k, top):
+    """Targets with a probability near one (their bias is `top` above the others', a target's logit passes the others' by
+    up to 2 top): the gradients are the others' small coefficients c and their sum for the target, each off by 2 e_l and
+    8 u32 of itself (the target's besides by the roundings of a sum of v) and its own rounding, not by a step of the
+    target's row; the loss is their log1p, off by the same relative error."""
+    n = 64
+    H, W, _, _, w = make(n, v, k, ty, seed=v, spread=1.0)
+    target = torch.full((n,), v // 2, dtype=torch.int32, device="cuda")
+    b = torch.linspace(-0.5, 0.5, v, device="cuda")
+    b[v // 2] = top
+    loss, lse, dH, dW, db = (x.double().cpu() for x in ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True))
+    ref = reference(H, W, target, b, w)
+    e_l = (k + 10) * U32 * (ref["L"] + 1)
+    assert ((loss - ref["loss"]).abs() <= (2 * e_l + (v + 8) * U32) * ref["loss"]).all()
+    c, g = ref["c"], ref["g"]
+    others = c.clone()
+    others[:, v // 2] = 0.0
+    c[:, v // 2] = -others.sum(1)
+    u_c = 2 * U32 if ty == "f32" else 2.0 ** -11
+    ec = (2 * e_l[:, None] + 8 * U32 + u_c) * c.abs()
+    ec[:, v // 2] += v * U32 * c[:, v // 2].abs()
+    floor = float(g.max()) * 2.0 ** -38  # (fp16 coefficients of the items' pass)
+    Wm, Hm = W.double().cpu(), H.double().cpu()
+    for name, x, r, lim in (("dH", dH, c @ Wm, ec @ Wm.abs() + (v + 4) * U32 * (c.abs() @ Wm.abs())),
+                            ("dW", dW, c.T @ Hm, (ec + floor).T @ Hm.abs() + (n + 4) * U32 * (c.abs().T @ Hm.abs())),
+                            ("db", db, c.sum(0), (ec + floor).sum(0) + (n + 4) * U32 * c.abs().sum(0))):
+        ut = U32 if name == "db" else half_step(T[ty])
+        tiny = 2.0 ** -24 if ty == "f16" and name != "db" else 1e-38
+        err = (x - r).abs()
+        lim = lim * (1 + ut) + ut * r.abs() + tiny
+        assert (err <= lim).all(), (name, float((err / lim).max()))
+
+
+@pytest.mark.gpu
 def test_many_rows(ctx):
     """More rows than one axis of a launch holds waves for.  Two items of one factor: l = h w_v, p = sigmoid.  A few fp32
     roundings of lse; a coefficient's 2^-11 and half a step of bf16 for dH; the sums of dW and dbias besides by a rounding
