@@ -648,9 +648,10 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
                 }
                 const int count = min(64, p.splits_f - i0);
 #pragma unroll 8
-                for (int i = grp; i < count; i += groups) {
-                    const float fi = __shfl(f, i);
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(O + (i0 + i) * step + c);
+                for (int i = 0; i < count; i += groups) {  // (as often in every lane: a shuffle reads active lanes only)
+                    const float fi = __shfl(f, i + grp);
+                    if (i + grp >= count) continue;
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(O + (i0 + i + grp) * step + c);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], fi, o[e]);
                 }

@@ -125,6 +125,16 @@ def test_values_and_gradients(ctx, n, v, k, ty):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,v,k", [(1, 1100, 20), (2, 9000, 30), (309, 25322, 22), (4, 48241, 43), (1, 20000, 64), (33, 60000, 8),
+                                   (40, 9000, 110), (3, 5001, 200), (6000, 150, 25), (20000, 3, 9)])
+def test_split_sums(ctx, n, v, k, ty):
+    """A few rows against many items, and many rows against a few: the sums come from up to hundreds of pieces."""
+    H, W, target, b, w = make(n, v, k, ty, seed=n + v, bias=True, gone=0.1)
+    check(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), ty, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
 def test_no_bias_no_weight(ctx, ty):
     H, W, target, _, _ = make(77, 333, 40, ty, seed=3)
     check(ctx.softmax_ce(H, W, target, grad=True), reference(H, W, target), ty, 40)
