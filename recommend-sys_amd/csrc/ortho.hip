@@ -19,6 +19,7 @@ constexpr int kThreads = 512;     // the two passes over the table: 8 waves
 constexpr int kStage = 8192;      // table elements of one stage of the Gram pass (per panel)
 constexpr int kJoinGroups = 8;    // groups that many pieces of the Gram matrix are summed in first
 constexpr int kJoinDirect = 24;   // up to so many pieces are joined at once
+constexpr int kPieces64 = 16;     // pieces of the fp64 Gram pass at most
 
 struct OrthoPlan {
     int64_t r;       // long side
@@ -27,6 +28,8 @@ struct OrthoPlan {
     int32_t panels;  // the Gram matrix is panels x panels blocks of at most 256 x 256
     int32_t splits;  // pieces of the long side, one per workgroup
     int64_t per;     // long-side rows of a piece
+    int32_t blocks64, splits64;  // the fp64 Gram pass: 32 x 32 blocks of the lower triangle, pieces of the long side
+    int64_t per64;               // (0: not taken)
     int64_t o_part, o_sum, o_pscale, o_mat[6], o_t, o_scale, bytes;  // A0, A, M, U, Ta, Tb; T's fp16 pieces and their scales
 };
 
@@ -44,13 +47,24 @@ OrthoPlan make_plan(int64_t rows, int64_t cols) {
     p.splits = static_cast<int32_t>(std::min<int64_t>(256 / (p.panels * p.panels), want));
     p.per = ceil_div(stages, p.splits) * kr;
     p.splits = static_cast<int32_t>(ceil_div(p.r, p.per));
+    // fp32 tables take their Gram matrix in fp64 where that costs little and the shape may be near-square (fp32 sums / fp64:
+    // 1682 x 20 32.1 / 29.3 us, 512 x 512 256 / 253, 1024 x 512 261 / 263; but 6040 x 100 81 / 88, 4096 x 512 277 / 321,
+    // 26744 x 128 91 / 141, and there both give the same X: a long side of four short ones and more has no small
+    // singular values by chance)
+    const int32_t side = p.sm / 32;
+    p.blocks64 = side * (side + 1) / 2;
+    if (p.r <= 2048) {
+        const int64_t most = std::min(kPieces64, std::max(4, 512 / p.blocks64));
+        p.per64 = round_up(ceil_div(p.r, most), 128);
+        p.splits64 = static_cast<int32_t>(ceil_div(p.r, p.per64));
+    }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
         at += round_up(bytes, 256);
         return o;
     };
-    p.o_part = take(static_cast<int64_t>(p.splits) * p.sp * p.sp * 4);
+    p.o_part = take(std::max(static_cast<int64_t>(p.splits) * p.sp * p.sp * 4, static_cast<int64_t>(p.splits64) * p.sm * p.sm * 8));
     p.o_sum = take(p.splits > kJoinDirect ? static_cast<int64_t>(kJoinGroups) * p.sp * p.sp * 8 : 0);
     p.o_pscale = take(static_cast<int64_t>(p.splits) * p.panels * p.panels * 4);
     for (int64_t& o : p.o_mat) o = take(static_cast<int64_t>(p.sm) * p.sm * 8);
@@ -332,6 +346,79 @@ __global__ __launch_bounds__(1024) void ortho_gram_join_kernel(const P* __restri
     const double a = (sum(0, i, j) + sum(1, j, i)) * scale;
     A[static_cast<int64_t>(ib * 16 + i) * p.sm + jb * 16 + j] = a;
     if (ib != jb) A[static_cast<int64_t>(jb * 16 + j) * p.sm + ib * 16 + i] = a;
+}
+
+// ---- Gram matrix in fp64 (fp32 tables of a shorter long side) -------------------------------------------------------
+// The products of fp32 elements are exact.  Small singular values are lost in fp32 sums: their share of a near-square
+// update comes out up to a^steps = 486 times larger, with the sums' errors (random 10 x 12: 2.2e-6 of X with fp32 sums,
+// 2.6e-7 with these; 40 x 40: 1.0e-5 and 8.0e-7; the steps themselves in fp32: 5.1e-7 and 9.0e-7).  A workgroup takes 32 x 32 entries of the lower
+// triangle from a piece of the long side, its waves every fourth 32 rows, straight from memory: 16 loads feed 32
+// products of 64 cycles.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void ortho_gram64_kernel(const float* __restrict__ G, int64_t ld, OrthoPlan p, double* __restrict__ part) {
+    __shared__ double sm[3][16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 15, lk = lane >> 4;
+    int ib = 0, t = blockIdx.x;
+    while (t > ib) t -= ++ib;  // block t of the lower triangle: row ib, column t
+    const int i0 = ib * 32, j0 = t * 32;
+    const int64_t r0 = blockIdx.y * p.per64, r1 = min(p.r, r0 + p.per64);
+    f64x4 acc[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) acc[x][y] = f64x4{0};
+    auto load = [&](int64_t r, int i) { return r < r1 && i < p.s ? G[WIDE ? i * ld + r : r * ld + i] : 0.f; };
+    for (int64_t rb = r0 + wave * 32; rb < r1; rb += 128) {
+        float a[2][8], b[2][8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int64_t r = rb + (WIDE ? lk * 8 + u : u * 4 + lk);  // (any order of the rows, the same for both)
+                a[x][u] = load(r, i0 + 16 * x + lc);
+                b[x][u] = load(r, j0 + 16 * x + lc);
+            }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                    acc[x][y] = __builtin_amdgcn_mfma_f64_16x16x4f64(static_cast<double>(a[x][u]), static_cast<double>(b[y][u]), acc[x][y], 0, 0, 0);
+    }
+    if (wave)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sm[wave - 1][(x * 2 + y) * 4 + e][lane] = acc[x][y][e];
+    __syncthreads();
+    if (wave) return;
+    double* o = part + static_cast<int64_t>(blockIdx.y) * p.sm * p.sm;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int q = (x * 2 + y) * 4 + e;
+                o[static_cast<int64_t>(i0 + 16 * x + 4 * e + lk) * p.sm + j0 + 16 * y + lc] = ((acc[x][y][e] + sm[0][q][lane]) + sm[1][q][lane]) + sm[2][q][lane];
+            }
+}
+
+// A0 from the pieces' lower triangles, in their order; a thread per entry
+__global__ __launch_bounds__(256) void ortho_join64_kernel(const double* __restrict__ part, OrthoPlan p, double* __restrict__ A) {
+    const int at = blockIdx.x * 256 + threadIdx.x, i = at / p.sm, j = at % p.sm;
+    const bool lower = i / 32 >= j / 32;
+    const double* src = part + (lower ? at : static_cast<int64_t>(j) * p.sm + i);
+    const int64_t step = static_cast<int64_t>(p.sm) * p.sm;
+    double x[kPieces64], sum = 0.0;
+#pragma unroll
+    for (int n = 0; n < kPieces64; ++n) x[n] = n < p.splits64 ? src[n * step] : 0.0;
+#pragma unroll
+    for (int n = 0; n < kPieces64; ++n) sum += x[n];
+    A[at] = sum;
 }
 
 // trace of A0 over a block of N threads (the same sum in every block)
@@ -623,27 +710,40 @@ void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, d
     _Float16* tp = reinterpret_cast<_Float16*>(ws + p.o_t);
     float* scale = reinterpret_cast<float*>(ws + p.o_scale);
 
-    const int glds = 2 * (kF32 ? 2 : 1) * kStage * 2;
-    const dim3 ggrid(static_cast<uint32_t>(p.splits), static_cast<uint32_t>(p.panels * p.panels));
-    // (the groups' sums take up to 64 KB of the same LDS)
-    if (p.sp == 64)
-        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 64, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
-    else if (p.sp == 128)
-        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 128, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
-    else if (p.sp == 256)
-        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 1>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
-    else
-        launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 2>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
     const uint32_t t = static_cast<uint32_t>(p.sm / 16);
-    if (p.splits > kJoinDirect) {
-        double* sums = reinterpret_cast<double*>(ws + p.o_sum);
-        ortho_gram_sum_kernel<<<dim3(static_cast<uint32_t>(p.sp * p.sp / 1024), kJoinGroups), 256, 0, st>>>(part, part_scale, p, sums);
-        RS_HIP(hipGetLastError());
-        ortho_gram_join_kernel<double><<<t * (t + 1) / 2, 1024, 0, st>>>(sums, part_scale, p, kJoinGroups, kF32 ? 1.0 : 0.5, A0);
-    } else {
-        ortho_gram_join_kernel<float><<<t * (t + 1) / 2, 1024, 0, st>>>(part, part_scale, p, p.splits, kF32 ? 1.0 : 0.5, A0);
+    bool exact = false;
+    if constexpr (kF32) {
+        exact = p.per64 > 0;
+        if (exact) {
+            ortho_gram64_kernel<WIDE><<<dim3(static_cast<uint32_t>(p.blocks64), static_cast<uint32_t>(p.splits64)), 256, 0, st>>>(
+                G, ldg, p, reinterpret_cast<double*>(part));
+            RS_HIP(hipGetLastError());
+            ortho_join64_kernel<<<static_cast<uint32_t>(p.sm * p.sm / 256), 256, 0, st>>>(reinterpret_cast<const double*>(part), p, A0);
+            RS_HIP(hipGetLastError());
+        }
     }
-    RS_HIP(hipGetLastError());
+    if (!exact) {
+        const int glds = 2 * (kF32 ? 2 : 1) * kStage * 2;
+        const dim3 ggrid(static_cast<uint32_t>(p.splits), static_cast<uint32_t>(p.panels * p.panels));
+        // (the groups' sums take up to 64 KB of the same LDS)
+        if (p.sp == 64)
+            launch_lds(ortho_gram_kernel<E, WIDE, VEC, 64, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
+        else if (p.sp == 128)
+            launch_lds(ortho_gram_kernel<E, WIDE, VEC, 128, 1>, ggrid, kThreads, std::max(glds, 65536), st, G, ldg, p, part, part_scale);
+        else if (p.sp == 256)
+            launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 1>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
+        else
+            launch_lds(ortho_gram_kernel<E, WIDE, VEC, 256, 2>, ggrid, kThreads, glds, st, G, ldg, p, part, part_scale);
+        if (p.splits > kJoinDirect) {
+            double* sums = reinterpret_cast<double*>(ws + p.o_sum);
+            ortho_gram_sum_kernel<<<dim3(static_cast<uint32_t>(p.sp * p.sp / 1024), kJoinGroups), 256, 0, st>>>(part, part_scale, p, sums);
+            RS_HIP(hipGetLastError());
+            ortho_gram_join_kernel<double><<<t * (t + 1) / 2, 1024, 0, st>>>(sums, part_scale, p, kJoinGroups, kF32 ? 1.0 : 0.5, A0);
+        } else {
+            ortho_gram_join_kernel<float><<<t * (t + 1) / 2, 1024, 0, st>>>(part, part_scale, p, p.splits, kF32 ? 1.0 : 0.5, A0);
+        }
+        RS_HIP(hipGetLastError());
+    }
 
     if (p.sm == 32) {
         launch_lds(ortho_small_chain_kernel<32>, dim3(1), 256, 4 * 32 * 33 * 8, st, p, static_cast<const double*>(A0), T, steps, a, b, c);

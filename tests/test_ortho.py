@@ -25,8 +25,9 @@ U32 = 2.0 ** -24
 COEF = (3.4445, -4.7750, 2.0315)
 
 
-def reference(G, steps=5, coef=COEF):
-    """(X, bound): the steps in 64 bits, and what an element may be off before its own type's rounding."""
+def reference(G, steps=5, coef=COEF, gram=1.0):
+    """(X, bound): the steps in 64 bits, and what an element may be off before its own type's rounding (gram: how much of
+    the Gram matrix's variance counts)."""
     G = G.double().cpu()
     norm = torch.linalg.vector_norm(G)
     if norm == 0:
@@ -56,7 +57,7 @@ def reference(G, steps=5, coef=COEF):
     gap = w0[:, None] - w0[None, :]
     near = gap.abs() < 1e-7 * w0.max().clamp(min=1e-300)
     D = torch.where(near, torch.maximum(der.abs()[:, None], der.abs()[None, :]), ((val[:, None] - val[None, :]) / torch.where(near, torch.ones_like(gap), gap)).abs())
-    v = 83 * U32 ** 2 * (Y0.abs().T @ Y0.abs()) ** 2
+    v = gram * 83 * U32 ** 2 * (Y0.abs().T @ Y0.abs()) ** 2
     V2 = V ** 2
     move = 8 * ((Y0 @ V) ** 2 @ (D ** 2 * (V2.T @ v @ V2)) @ V2.T).sqrt()
     S = Y0.shape[1]
@@ -151,6 +152,20 @@ def test_strided_in_place_and_beside(ctx, rows, cols):
     assert torch.equal(big[:, 5:5 + cols], want)
     big[:, 5:5 + cols] = 3.0
     assert (big == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(1, 1), (2, 2), (10, 12), (33, 31), (40, 40), (64, 64), (100, 97), (129, 160), (260, 256),
+                                       (512, 512), (300, 511), (2048, 512), (2048, 5), (20, 2047)])
+def test_near_square_updates(ctx, rows, cols):
+    """Small singular values: the Gram matrix of an fp32 update of up to 2048 long-side rows is exact but for fp64's
+    roundings, so the errors are T's and the table's as pairs, S fp32 sums and the output's rounding, without what fp32 sums
+    of the Gram matrix would move T by (fp64's 2^-53 times the largest divided difference, under 486 S: nothing)."""
+    G = torch.randn(rows, cols, generator=torch.Generator().manual_seed(rows + cols)).cuda() * 1e-3
+    ref, bound = reference(G, gram=0.0)
+    err = (ctx.orthogonalize(G).double().cpu() - ref).abs()
+    lim = bound * (1 + U32) + 3 * U32 * ref.abs()
+    assert (err <= lim).all(), float((err / lim).max())
 
 
 @pytest.mark.gpu
