@@ -438,7 +438,10 @@ __device__ __forceinline__ double block_trace(const double* A0, const OrthoPlan&
     return t;
 }
 
-// ---- S x S products of symmetric, commuting matrices: C = X Y, 16 x 16 per workgroup, its four waves share k --------
+// ---- S x S products of symmetric, commuting matrices: C = X Y, 16 x 16 per workgroup, its four waves share k.  C is
+// symmetric too: of 512 x 512, where the operands' reads through L2 bound it, only the blocks of the lower triangle
+// are formed and mirrored (all steps of a 512 x 512 update 253 -> 201 us; of 128 x 128 and 256 x 256, where latency
+// does, all blocks: 81 us against 83 and 6.0 us a product against 6.2).
 struct ChainArgs {
     OrthoPlan p;
     const double* A0;        // unnormalised Gram matrix
@@ -450,11 +453,15 @@ struct ChainArgs {
     double a, b, c;
 };
 
+template <bool LOWER>  // only the lower triangle's blocks, by blockIdx.x
 __global__ __launch_bounds__(256) void ortho_chain_kernel(ChainArgs q) {
     __shared__ double sm[3][4][64];
     const int sm_ = q.p.sm, z = blockIdx.z;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lc = lane & 15, lk = lane >> 4;
-    const int i0 = blockIdx.x * 16, j0 = blockIdx.y * 16, kq = sm_ / 4;
+    int ib = blockIdx.x, jb = blockIdx.y;
+    if (LOWER)  // block x of the lower triangle: row ib, column jb
+        for (ib = 0, jb = blockIdx.x; jb > ib;) jb -= ++ib;
+    const int i0 = ib * 16, j0 = jb * 16, kq = sm_ / 4;
     // X and Y are symmetric: both operands are read along rows k
     const double *X = q.X[z] + static_cast<int64_t>(wave * kq + lk) * sm_ + i0 + lc, *Y = q.Y[z] + static_cast<int64_t>(wave * kq + lk) * sm_ + j0 + lc;
     // (the epilogue's values of X are on their way during the product: 3.9 us a product of 128 x 128, 4.1 read after it)
@@ -491,6 +498,7 @@ __global__ __launch_bounds__(256) void ortho_chain_kernel(ChainArgs q) {
         double v = (((acc[e] + sm[0][e][lane]) + sm[1][e][lane]) + sm[2][e][lane]) * inv;
         if (q.poly && z == 0) v = (i0 + 4 * e + lk == j0 + lc ? q.a : 0.0) + q.b * x[e] * inv + q.c * (v * inv);
         q.C[z][out + static_cast<int64_t>(4 * e) * sm_] = v;
+        if (LOWER && i0 != j0) q.C[z][static_cast<int64_t>(j0 + lc) * sm_ + i0 + 4 * e + lk] = v;
     }
 }
 
@@ -752,6 +760,13 @@ void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, d
     } else {
         ChainArgs q{};
         q.p = p, q.A0 = A0, q.a = a, q.b = b, q.c = c;
+        auto product = [&](int z) {
+            if (p.sm == 512)
+                ortho_chain_kernel<true><<<dim3(t * (t + 1) / 2, 1, static_cast<uint32_t>(z)), 256, 0, st>>>(q);
+            else
+                ortho_chain_kernel<false><<<dim3(t, t, static_cast<uint32_t>(z)), 256, 0, st>>>(q);
+            RS_HIP(hipGetLastError());
+        };
         const double* A = A0;
         for (int j = 0; j < steps; ++j) {
             const bool last = j + 1 == steps;
@@ -759,21 +774,18 @@ void run(const OrthoPlan& p, const E* G, int64_t ldg, int32_t steps, double a, d
             double* Mj = j == 0 ? T : M;  // T = M_0
             q.poly = 1;
             q.X[0] = q.Y[0] = A, q.C[0] = Mj;
-            ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
-            RS_HIP(hipGetLastError());
+            product(1);
             q.poly = 0;
             // A M (not after the last step) and T M (not in the first)
             int z = 0;
             if (!last) q.X[z] = A, q.Y[z] = Mj, q.C[z] = U, ++z;
             if (j) q.X[z] = T, q.Y[z] = Mj, q.C[z] = T2, ++z;
-            if (z) ortho_chain_kernel<<<dim3(t, t, static_cast<uint32_t>(z)), 256, 0, st>>>(q);
-            RS_HIP(hipGetLastError());
+            if (z) product(z);
             if (j) std::swap(T, T2);
             if (last) break;
             q.normalise = 0;
             q.X[0] = U, q.Y[0] = Mj, q.C[0] = mat[1];
-            ortho_chain_kernel<<<dim3(t, t, 1), 256, 0, st>>>(q);
-            RS_HIP(hipGetLastError());
+            product(1);
             A = mat[1];
         }
     }
