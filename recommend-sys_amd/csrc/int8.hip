@@ -10,38 +10,29 @@
 namespace rs {
 namespace {
 
-// ---- quantising rows: a wave per row -------------------------------------------------------------------------------
-// x / s to the nearest integer, ties to even, as if the quotient were exact.  The fp32 quotient decides all but the
-// neighbourhood of a tie (its error is below 2^-15 at |x / s| <= 127); there |x| is compared with (r + 1/2) s, which
-// is exact in fp64.
-__device__ __forceinline__ int quantize(float x, float s, float inv, bool safe) {
-    const float ax = fabsf(x);
-    float t = ax * inv;
-    if (!safe) t = static_cast<float>(static_cast<double>(ax) / static_cast<double>(s));
-    float r = floorf(t);
-    const float d = t - r;
-    int q;
-    if (d > 0.499f && d < 0.501f) {
-        const double tie = (static_cast<double>(r) + 0.5) * static_cast<double>(s), a = static_cast<double>(ax);
-        const int ri = static_cast<int>(r);
-        q = a > tie ? ri + 1 : a < tie ? ri : ri + (ri & 1);
-    } else {
-        q = static_cast<int>(rintf(t));
-    }
-    q = min(q, 127);
-    return x < 0.f ? -q : q;
+// ---- quantising rows -----------------------------------------------------------------------------------------------
+// |x| / s to the nearest integer, ties to even, as if the quotient were exact: the fp32 quotient gives its floor r (or an
+// integer beside it where the quotient is near one, far from the tie), the sign of the remainder |x| - (r + 1/2) s decides:
+// one fused multiply-add keeps that sign, and zero, exact.
+__device__ __forceinline__ int quantize(float ax, float s, float inv) {
+    const float r = floorf(ax * inv);
+    const int ri = static_cast<int>(r), d = static_cast<int>(__float_as_uint(fmaf(-(r + 0.5f), s, ax)));
+    return ri + (d + (ri & 1) > 0);  // above the tie, or on it beside an odd r
 }
 
-// Eight elements a lane at a time; rows of up to 64 * 8 * kKeep columns stay in registers between the maximum and the
-// rounding, longer ones are read again.  VEC: rows of X start at 16-byte addresses, rows of q at 8-byte ones.
-constexpr int kKeep = 8;
-template <typename E, bool VEC>
+// Lanes of a row: 16 up to 128 columns, 32 up to 256 (1e6 x 256 fp32 210 us, 6.1 TB/s; 412 with a wave a row), a wave, or
+// past kWideRow columns the four of a workgroup (64 x 32768 bf16 12 us, 46 with a wave; but 8192 x 1024 13 us, 8 with a
+// wave; 2048 columns give the same).  Bound by the bytes: 2048 x 4096 bf16 8 us with the launch.  Eight elements a lane
+// at a time; rows of up to eight times that stay in registers between the maximum and the rounding, longer ones are read
+// again.  VEC: rows of X start at 16-byte addresses, rows of q at 8-byte ones.
+constexpr int kWideRow = 2048;
+template <typename E, bool VEC, int LANES>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict__ X, int64_t ldx, int64_t rows, int64_t cols,
                                                            int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
     typedef __attribute__((ext_vector_type(16 / sizeof(E)))) E vec;
-    constexpr int V = 16 / sizeof(E);
-    const int lane = threadIdx.x & 63;
-    const int64_t r = wide_block() * 4 + (threadIdx.x >> 6);
+    constexpr int V = 16 / sizeof(E), STEP = 8 * LANES, kKeep = LANES < 64 ? 1 : 8;
+    const int at = threadIdx.x % LANES * 8;
+    const int64_t r = wide_block() * (256 / LANES) + threadIdx.x / LANES;
     if (r >= rows) return;
     const E* x = X + r * ldx;
     int8_t* o = q + r * ldq;
@@ -67,30 +58,45 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict_
         }
     };
     float kept[kKeep][8];
-    const bool fits = cols <= 512 * kKeep;
+    const bool fits = cols <= STEP * kKeep;
     if (fits) {
 #pragma unroll
         for (int i = 0; i < kKeep; ++i)
-            if (i * 512 < cols) load(i * 512 + lane * 8, kept[i]), see(kept[i]);
+            if (i * STEP < cols) load(i * STEP + at, kept[i]), see(kept[i]);
     } else {
-        for (int64_t c = lane * 8; c < cols; c += 512) {
+        for (int64_t c = at; c < cols; c += STEP) {
             float v[8];
             load(c, v);
             see(v);
         }
     }
-    m = wave_max_u32(m);
+    if constexpr (LANES < 64) {
+#pragma unroll
+        for (int l = LANES / 2; l; l >>= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), l)));
+    } else {
+        m = wave_max_u32(m);
+    }
+    if constexpr (LANES == 256) {
+        __shared__ uint32_t tops[4];
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
     const bool finite = m < 0x7F800000u;
     const float s = finite ? __uint_as_float(m) * (1.f / 127.f) : __uint_as_float(0x7FC00000u);
-    if (lane == 0) scale[r] = s;
-    const bool some = finite && s > 0.f, safe = s > 7.9e-31f;
-    const float inv = 1.f / s;
+    if (at == 0) scale[r] = s;
+    // a row of small numbers is scaled up (exactly) first, so that no remainder and no 1 / s leaves the normal numbers
+    const float pre = s > 7.9e-31f ? 1.f : 0x1p96f, sp = s * pre, inv = 1.f / sp;
+    const uint32_t some = finite && s > 0.f ? ~0u : 0u;
     auto write = [&](int64_t c, const float (&v)[8]) {
         if (c >= cols) return;
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (some) w[e / 4] |= static_cast<uint32_t>(quantize(v[e], s, inv, safe) & 255) << (8 * (e % 4));
+        for (int e = 0; e < 8; ++e) {
+            const int n = quantize(fabsf(v[e]) * pre, sp, inv);
+            w[e / 4] |= static_cast<uint32_t>((v[e] < 0.f ? -n : n) & 255) << (8 * (e % 4));
+        }
+        w[0] &= some, w[1] &= some;
         if (VEC && c + 8 <= cols) {
             *reinterpret_cast<uint2*>(o + c) = make_uint2(w[0], w[1]);
         } else {
@@ -102,9 +108,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict_
     if (fits) {
 #pragma unroll
         for (int i = 0; i < kKeep; ++i)
-            if (i * 512 < cols) write(i * 512 + lane * 8, kept[i]);
+            if (i * STEP < cols) write(i * STEP + at, kept[i]);
     } else {
-        for (int64_t c = lane * 8; c < cols; c += 512) {
+        for (int64_t c = at; c < cols; c += STEP) {
             float v[8];
             load(c, v);
             write(c, v);
@@ -375,11 +381,22 @@ extern "C" int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64
             using E = typename decltype(e)::type;
             const bool vec = (reinterpret_cast<uintptr_t>(X) | static_cast<uintptr_t>(ldx * static_cast<int64_t>(sizeof(E)))) % 16 == 0 &&
                              (reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ldq)) % 8 == 0;
-            const dim3 blocks = wide_grid(ceil_div(n_rows, 4));
-            if (vec)
-                quantize_rows_kernel<E, true><<<blocks, 256, 0, st>>>(static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
-            else
-                quantize_rows_kernel<E, false><<<blocks, 256, 0, st>>>(static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
+            auto go = [&](auto v, auto lanes) {
+                constexpr int LANES = decltype(lanes)::value;
+                quantize_rows_kernel<E, decltype(v)::value, LANES><<<wide_grid(ceil_div(n_rows, 256 / LANES)), 256, 0, st>>>(
+                    static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
+            };
+            auto width = [&](auto v) {
+                if (n_cols > kWideRow)
+                    go(v, std::integral_constant<int, 256>{});
+                else if (n_cols > 256)
+                    go(v, std::integral_constant<int, 64>{});
+                else if (n_cols > 128)
+                    go(v, std::integral_constant<int, 32>{});
+                else
+                    go(v, std::integral_constant<int, 16>{});
+            };
+            vec ? width(std::true_type{}) : width(std::false_type{});
         });
         RS_HIP(hipGetLastError());
         return RS_OK;

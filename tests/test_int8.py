@@ -72,7 +72,7 @@ def scales(m, seed):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 64), (70, 100), (33, 257), (9, 1025), (4, 4099)])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 7), (5, 64), (70, 100), (37, 128), (35, 129), (19, 256), (33, 257), (9, 1025), (6, 2048), (7, 2049), (4, 4099), (3, 16390)])
 def test_quantize(ctx, m, k, ty):
     g = torch.Generator().manual_seed(m * 100 + k)
     x = (torch.randn(m, k, generator=g) * torch.rand(m, 1, generator=g)).to(T[ty]).cuda()
