@@ -13,7 +13,8 @@
  * free for other use once the call's kernels have run, and two calls that may overlap need a workspace each.  The
  * caller's current device is put back before a call returns.  Calls whose sizes leave nothing to do return RS_OK
  * without a launch.  Sums are held in fp32, int32 or fp64 and each output is rounded once; results do not depend on
- * timing (no floating-point atomics).  Outputs and ws overlap neither the inputs nor each other.  n_factors up to RS_DENSE_MAX_FACTORS. */
+ * timing (no floating-point atomics).  Outputs and ws overlap neither the inputs nor each other.  n_factors up to
+ * RS_DENSE_MAX_FACTORS. */
 #ifndef RSGPU_DENSE_H
 #define RSGPU_DENSE_H
 
@@ -46,7 +47,10 @@ extern "C" {
  *   Finite biases are held to +-2^120: the type's lowest value is no withdrawal.
  * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
  * (hi + lo), so an element keeps 2^-24 of itself or 2^-38 of the matrix's largest element, whichever is more;
- * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below.
+ * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Coefficients c_nv
+ * are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise.  The target's coefficient is minus the sum of
+ * the row's others: the gradients of a row keep their precision where its target's probability is near one, as does
+ * its loss.
  * n_rows and n_items from 1 to 2^31 - 1025 (or both 0). */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);

@@ -161,7 +161,8 @@ __device__ __forceinline__ void store_scores(const I8Args& a, int64_t m, int64_t
 }
 
 // Few rows of A (m <= 64): they sit in LDS as MT tiles of 16; each wave takes 16 rows of B at a time straight from HBM
-// into 16x16x64 MFMAs (first operand B's rows, second A's), so B is read once.
+// into 16x16x64 MFMAs (first operand B's rows, second A's), so B is read once.  Bound by B's bytes: one row against 1e6 x 256
+// 52 us, 4.9 TB/s.
 constexpr int kFewRows = 64;
 constexpr int kFewLds = 64 * 1024;
 template <typename E, bool VEC, int MT>
@@ -206,6 +207,9 @@ __global__ __launch_bounds__(256) void i8_few_kernel(I8Args a) {
 // Many rows: TM x TN tiles of C, waves of WM x WN (32x32x32 MFMAs, first operand B's rows), steps of 64 along k through a
 // double-buffered LDS tile; the next step's rows are on their way in registers during the MFMAs.  C leaves through
 // LDS, so that a row's stores are contiguous.  OUT16: C's rows start at 16-byte addresses.
+// 2048 x 8192 x 4096 to bf16 84 us, 1.64 POP/s (a large product reaches 2.0); 4096 x 26744 x 128 to bf16 75 us, bound by
+// writing C at 2.9 TB/s (two steps on their way, or a workgroup that fetches its next tile while this one leaves, changed
+// nothing; 128 x 128 tiles 90 us).
 constexpr int kStep = 64;
 template <typename E, bool VEC, bool OUT16, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__((TM / WM) * (TN / WN) * 64) void i8_tile_kernel(I8Args a, int tiles_m, int tiles_n) {

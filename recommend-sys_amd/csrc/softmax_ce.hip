@@ -7,7 +7,8 @@
 //     gives lse and dH = weight (O - s W_target) / (s + t).  (With the target inside the sums dH would be the difference
 //     O / (s + t) - W_target of two near vectors where its probability is near one: 2^-12 of W_target, against 2^-12 of
 //     dH; the loss keeps its small values in the same way.)
-//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - m_y) / (s_y + t_y) - [target]) and dW_x += sum_y c H_y.
+//   dW: x = items, y = users' rows.  S is computed again, c = weight (2^(l2 - m_y) / (s_y + t_y) - [target]) and
+//     dW_x += sum_y c H_y.
 // Both are one kernel: S = Y X^T, then acc[k, x] += Y^T f(S).  S comes out of the matrix unit with x over lanes and y
 // over registers, which is (up to an order of y, the same for both operands) what the second product takes as its
 // second operand: f(S) never leaves the registers.  Its first operand Y^T comes from the same LDS tile as Y by
@@ -16,9 +17,16 @@
 // Operands are packed into the workspace first: rows padded to tiles and columns to KP with zeros, withdrawn items
 // and rows without a known target zeroed (so NaN or garbage in them reaches no product), as fp16 of the matrix scaled by
 // a power of two.  bf16's 8 bits fit fp16's 11: the products are those of bf16, but the coefficients f(S) keep 11 bits
-// where bf16 MFMAs would round them to 8 (dW's error then was 1.5 times that of its own rounding).  fp32 is split into
-// two pieces hi + lo (each rounds its rest: 2^-24 of the element is left); the product of two such is
-// hi hi + hi lo + lo hi, three fp16 MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
+// where bf16 MFMAs would round them to 8 (dW's error then was 1.5 times that of its own rounding).  fp16's gradients keep
+// 11 bits themselves, so its coefficients are two pieces (450 us on 8192 x 26744 x 128; one piece takes 354 and leaves up
+// to 2 times the error of dW's own rounding where it sums a few rows).  fp32 is split into two pieces hi + lo (each
+// rounds its rest: 2^-24 of the element is left); the product of two such is hi hi + hi lo + lo hi, three fp16 MFMAs
+// (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
+//
+// With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 36 cycles of exponential,
+// sums and packing for each of a lane's 16 logits (KP = 128).  1024 x 1e6 x 256 bf16 2.45 ms: passes 1.07 and 1.16 ms (0.98
+// and 0.90 PFLOP/s), packing 0.38; 8192 x 26744 x 128 bf16 0.33 ms; 4096 x 3706 x 100 fp32 93 us; 128 x 1682 x 20
+// fp32 27 us, five launches.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -92,7 +100,7 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
         const Shape sh = shape_for(p.np, p.kp, mode);
         const int64_t tx = ceil_div(rows_x, 32 * sh.waves) * p.z, ty = ceil_div(rows_y, kTileY);
         const bool alone = sh.waves == 8 || sh.occ == 1;
-        const double tile = static_cast<double>(kTileY) * 32 * sh.waves * (p.kp + p.oc) * 2 * (p.np == 2 ? 3 : 1) / (alone ? 3.4e6 : 2.4e6);
+        const double tile = static_cast<double>(kTileY) * 32 * sh.waves * (p.kp + p.oc) * 2 * (p.np == 2 ? 3.0 : type == RS_TYPE_F16 ? 1.5 : 1.0) / (alone ? 3.4e6 : 2.4e6);
         const double sums = static_cast<double>(rows_x) * p.kp * 8 / 8e6;
         double best = 0.0;
         for (int64_t s = 1, per = ty; s == 1 || tx * s <= 4096; s = ceil_div(ty, per)) {  // each length of a split once
@@ -283,6 +291,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     constexpr bool items = MODE == kItems;
     constexpr int THREADS = WAVES * 64;
     constexpr int OC = KP < 256 ? KP : 256, NB = MODE == kLoss ? 1 : OC / 32, KS = KP / 16, C = KP / 8;
+    constexpr int NC = std::is_same<E, __bf16>::value ? 1 : 2;  // pieces of a coefficient
     constexpr int ROWS = 32 * SUB;                         // rows of a stage
     constexpr int PIECE = ROWS * KP;                       // elements of one piece of a stage
     constexpr int CHUNKS = ROWS * C * NP, PER = (CHUNKS + THREADS - 1) / THREADS;
@@ -464,15 +473,15 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             if constexpr (MODE != kLoss) {
 #pragma unroll
                 for (int j = 2 * h / HALVES; j < 2 * (h + 1) / HALVES; ++j) {
-                    f16x8 c[NP];
+                    f16x8 c[NC];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float f = s[8 * j + e];
                         // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
                         // product before it would round to another hi now and then
-                        if (NP == 2) asm("" : "+v"(f));
+                        if (NC == 2) asm("" : "+v"(f));
                         c[0][e] = static_cast<_Float16>(f);
-                        if (NP == 2) c[NP - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[0][e]));
+                        if (NC == 2) c[NC - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[0][e]));
                     }
                     // Y^T: lane = column of Y, elements e = rows 16 j + 8 (e / 4) + 4 half + e mod 4, as c's
 #pragma unroll
@@ -488,10 +497,8 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                             yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
                         }
                         acc[nb] = mfma16(yt[0], c[0], acc[nb]);
-                        if constexpr (NP == 2) {
-                            acc[nb] = mfma16(yt[0], c[1], acc[nb]);
-                            acc[nb] = mfma16(yt[1], c[0], acc[nb]);
-                        }
+                        if constexpr (NC == 2) acc[nb] = mfma16(yt[0], c[1], acc[nb]);
+                        if constexpr (NP == 2) acc[nb] = mfma16(yt[1], c[0], acc[nb]);
                     }
                 }
             }

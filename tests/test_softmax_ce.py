@@ -5,8 +5,8 @@ Tolerances.  u = eps / 2 is half a step of a type.  A logit is a sum of k produc
 (k + 4) u32 sum |h w| plus, for the base-2 exponent, 3 u32 |l| (one rounding each for the scale, the sum with the
 bias and the difference); fp16 pairs leave 3 u32 |h w| of a product more.  With L the largest
 sum |h w| + |bias| of a row, e_l = (k + 10) u32 (L + 1) bounds a logit's error, the loss and lse take 2 e_l, and a
-probability is off by 2 e_l and 4 u32 of itself (its exponential, the sum, the division and a product).  A coefficient c = weight (p - [target]) is then rounded to the product's type:
-u16 of itself (fp32: a pair, 2 u32), and the sum over the rows or items adds (terms) u32 of the sum of magnitudes.
+probability is off by 2 e_l and 4 u32 of itself (its exponential, the sum, the division and a product).  A coefficient c = weight (p - [target]) is then rounded to
+fp16 or a pair of them (U_C), and the sum over the rows or items adds (terms) u32 of the sum of magnitudes.
 Outputs add half a step of their type.  (exp2 and log2 are good to 2 units, inside the 10.)
 """
 import ctypes as C
@@ -21,6 +21,7 @@ torch = pytest.importorskip("torch")
 
 T = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 U32 = 2.0 ** -24
+U_C = {"f32": 2 * U32, "bf16": 2.0 ** -11, "f16": 2.0 ** -22}  # a coefficient's rounding: a pair, one fp16 value, a pair
 
 
 def half_step(t):
@@ -86,7 +87,7 @@ def check(out, ref, ty, k, grad=True):
         assert (((x - r).abs() - 2 * e_l - 4 * U32 * r.abs())[fin] <= 0).all(), (name, float((x - r)[fin].abs().max()))
     if not grad:
         return
-    u_c = 2 * U32 if ty == "f32" else half_step(t)
+    u_c = U_C[ty]
     n, v = ref["c"].shape
     # error of a coefficient: its probability's, then its rounding; an fp16 coefficient of any type keeps at least 2^-25 of
     # 2^-13 of the largest weight (it is held scaled to below 2^14)
@@ -314,7 +315,7 @@ def test_rows_that_are_nearly_learnt(ctx, ty, v, k, top):
     others = c.clone()
     others[:, v // 2] = 0.0
     c[:, v // 2] = -others.sum(1)
-    u_c = 2 * U32 if ty == "f32" else 2.0 ** -11
+    u_c = U_C[ty]
     ec = (2 * e_l[:, None] + 8 * U32 + u_c) * c.abs()
     ec[:, v // 2] += v * U32 * c[:, v // 2].abs()
     floor = float(g.max()) * 2.0 ** -38  # (fp16 coefficients of the items' pass)
