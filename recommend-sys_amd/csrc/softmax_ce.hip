@@ -51,10 +51,10 @@ enum Mode { kLoss = 0, kLossGrad = 1, kItems = 2 };
 // Shape of a workgroup: waves of 32 stationary rows each, streamed rows of a stage (between two barriers) in blocks of
 // 32, waves per SIMD asked of the compiler.  Measured on 8192 x 26744 x 128 and 1024 x 1e6 x 256 (bf16), 4096 x 3706 x 100
 // (fp32), times of the two passes (users / items):
-//   KP = 128, one piece: 8 waves 148 / 196 us, 4 waves 161 / 184; stages of 4 blocks 135 for the users' pass, 2 for the
-//     items' (4 spill)
-//   KP = 256, one piece: 8 waves 1255 / 1536 us, 4 waves 1444 / 1617 (8 waves read the streamed tile once for 256 rows)
-//   KP = 128, two pieces: 4 waves 39 / 41 us, 8 waves 42 / 45
+//   KP = 128, one piece: 8 waves 148 / 183 us, 4 waves 162 / 194 and twice the pieces to join; stages of 4 blocks for the
+//     users' pass (of 2: 150), 2 for the items' (4 spill)
+//   KP = 256, one piece: 8 waves 1122 / 1222 us, 4 waves 1478 / 1431 (8 waves read the streamed tile once for 256 rows)
+//   KP = 128, two pieces: 4 waves 35.3 / 34.8 us, 8 waves 34.1 / 34.7
 //   wider: the row and its sums take more than half the registers: one wave per SIMD
 struct Shape {
     int waves, blocks, occ;
@@ -62,10 +62,9 @@ struct Shape {
 constexpr Shape shape_for(int np, int kp, int mode) {
     if (np * kp >= 512) return {4, 1, 1};
     if (np * kp == 256) return np == 1 ? Shape{8, 1, 2} : Shape{4, 1, 2};
-    if (np * kp == 128) return np == 2 ? Shape{4, 2, 2} : mode == kItems ? Shape{4, 2, 2} : Shape{8, 4, 2};
+    if (np * kp == 128) return np == 2 ? Shape{4, 2, 2} : mode == kItems ? Shape{8, 2, 2} : Shape{8, 4, 2};
     return {4, 2, 2};
 }
-
 
 // Device scalars (ws): the powers of two that scale H, W and the weights, and what undoes them.
 struct Scal {
