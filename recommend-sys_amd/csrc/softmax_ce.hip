@@ -24,9 +24,9 @@
 // (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
 //
 // With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 36 cycles of exponential,
-// sums and packing for each of a lane's 16 logits (KP = 128).  1024 x 1e6 x 256 bf16 2.45 ms: passes 1.07 and 1.16 ms (0.98
-// and 0.90 PFLOP/s), packing 0.38; 8192 x 26744 x 128 bf16 0.33 ms; 4096 x 3706 x 100 fp32 93 us; 128 x 1682 x 20
-// fp32 27 us, five launches.
+// sums and packing for each of a lane's 16 logits (KP = 128).  1024 x 1e6 x 256 bf16 2.5 ms: passes 1.09 and 1.19 ms (0.96
+// and 0.88 PFLOP/s), packing 0.38; 8192 x 26744 x 128 bf16 0.315 ms; 4096 x 3706 x 100 fp32 93 us; 128 x 1682 x 20
+// fp32 28 us, five launches.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
