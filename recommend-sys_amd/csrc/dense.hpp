@@ -92,6 +92,18 @@ int dense_guard(rs_ctx* ctx, F&& body) {
     }
 }
 
+// A C entry's whole body: no exception leaves it, the argument checks' strings included (which then have no message).
+template <typename F>
+int no_throw(F&& body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return RS_ERR_NOMEM;
+    } catch (...) {
+        return RS_ERR_INVALID;
+    }
+}
+
 // NULL: the ctx stream (as everywhere in the C-ABI); RS_STREAM_DEFAULT: the device's null stream
 inline hipStream_t pick_stream(rs_ctx* ctx, void* stream) {
     if (stream == RS_STREAM_DEFAULT) return nullptr;

@@ -371,69 +371,73 @@ void launch_i8(const I8Args& a, hipStream_t st) {
 
 extern "C" int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_cols, const void* X, int64_t ldx, int8_t* q,
                                 int64_t ldq, float* scale, void* stream) {
-    using namespace rs;
-    if (!type_ok(type)) return set_error(ctx, RS_ERR_INVALID, "type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
-    if (n_rows < 0 || n_rows > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "n_rows out of range");
-    if (n_cols < 1) return set_error(ctx, RS_ERR_INVALID, "n_cols must be at least 1");
-    if (n_rows == 0) return RS_OK;
-    for (const std::string& b : {check_matrix("X", X, n_cols, ldx, type_size(type)), check_matrix("q", q, n_cols, ldq, 1),
-                                 check_matrix("scale", scale, 1, 1, 4)})
-        if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
-    return dense_guard(ctx, [&]() -> int {
-        const hipStream_t st = pick_stream(ctx, stream);
-        with_type(type, [&](auto e) {
-            using E = typename decltype(e)::type;
-            const bool vec = (reinterpret_cast<uintptr_t>(X) | static_cast<uintptr_t>(ldx * static_cast<int64_t>(sizeof(E)))) % 16 == 0 &&
-                             (reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ldq)) % 8 == 0;
-            auto go = [&](auto v, auto lanes) {
-                constexpr int LANES = decltype(lanes)::value;
-                quantize_rows_kernel<E, decltype(v)::value, LANES><<<wide_grid(ceil_div(n_rows, 256 / LANES)), 256, 0, st>>>(
-                    static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
-            };
-            auto width = [&](auto v) {
-                if (n_cols > kWideRow)
-                    go(v, std::integral_constant<int, 256>{});
-                else if (n_cols > 256)
-                    go(v, std::integral_constant<int, 64>{});
-                else if (n_cols > 128)
-                    go(v, std::integral_constant<int, 32>{});
-                else
-                    go(v, std::integral_constant<int, 16>{});
-            };
-            vec ? width(std::true_type{}) : width(std::false_type{});
+    return rs::no_throw([&]() -> int {
+        using namespace rs;
+        if (!type_ok(type)) return set_error(ctx, RS_ERR_INVALID, "type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
+        if (n_rows < 0 || n_rows > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "n_rows out of range");
+        if (n_cols < 1) return set_error(ctx, RS_ERR_INVALID, "n_cols must be at least 1");
+        if (n_rows == 0) return RS_OK;
+        for (const std::string& b : {check_matrix("X", X, n_cols, ldx, type_size(type)), check_matrix("q", q, n_cols, ldq, 1),
+                                     check_matrix("scale", scale, 1, 1, 4)})
+            if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
+        return dense_guard(ctx, [&]() -> int {
+            const hipStream_t st = pick_stream(ctx, stream);
+            with_type(type, [&](auto e) {
+                using E = typename decltype(e)::type;
+                const bool vec = (reinterpret_cast<uintptr_t>(X) | static_cast<uintptr_t>(ldx * static_cast<int64_t>(sizeof(E)))) % 16 == 0 &&
+                                 (reinterpret_cast<uintptr_t>(q) | static_cast<uintptr_t>(ldq)) % 8 == 0;
+                auto go = [&](auto v, auto lanes) {
+                    constexpr int LANES = decltype(lanes)::value;
+                    quantize_rows_kernel<E, decltype(v)::value, LANES><<<wide_grid(ceil_div(n_rows, 256 / LANES)), 256, 0, st>>>(
+                        static_cast<const E*>(X), ldx, n_rows, n_cols, q, ldq, scale);
+                };
+                auto width = [&](auto v) {
+                    if (n_cols > kWideRow)
+                        go(v, std::integral_constant<int, 256>{});
+                    else if (n_cols > 256)
+                        go(v, std::integral_constant<int, 64>{});
+                    else if (n_cols > 128)
+                        go(v, std::integral_constant<int, 32>{});
+                    else
+                        go(v, std::integral_constant<int, 16>{});
+                };
+                vec ? width(std::true_type{}) : width(std::false_type{});
+            });
+            RS_HIP(hipGetLastError());
+            return RS_OK;
         });
-        RS_HIP(hipGetLastError());
-        return RS_OK;
     });
 }
 
 extern "C" int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, int64_t lda, const float* a_scale,
                             const int8_t* B, int64_t ldb, const float* b_scale, const float* row_bias, const float* col_bias,
                             int32_t out_type, void* C, int64_t ldc, void* stream) {
-    using namespace rs;
-    if (!type_ok(out_type)) return set_error(ctx, RS_ERR_INVALID, "out_type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
-    if (m < 0 || m > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "m out of range");
-    if (n < 0 || n > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "n out of range");
-    if (ceil_div(m, 128) * ceil_div(n, 128) > INT32_MAX / 512) return set_error(ctx, RS_ERR_UNSUPPORTED, "m x n is too large for one call");
-    if (k < 1) return set_error(ctx, RS_ERR_INVALID, "k must be at least 1");
-    if (k > RS_I8_MAX_K) return set_error(ctx, RS_ERR_UNSUPPORTED, "k must be at most 65536 (exact int32 sums)");
-    if (m == 0 || n == 0) return RS_OK;
-    for (const std::string& b : {check_matrix("A", A, k, lda, 1), check_matrix("B", B, k, ldb, 1), check_matrix("a_scale", a_scale, 1, 1, 4),
-                                 check_matrix("b_scale", b_scale, 1, 1, 4), check_matrix("C", C, n, ldc, type_size(out_type)),
-                                 row_bias ? check_matrix("row_bias", row_bias, 1, 1, 4) : std::string(),
-                                 col_bias ? check_matrix("col_bias", col_bias, 1, 1, 4) : std::string()})
-        if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
-    I8Args a{A, B, m, n, k, lda, ldb, ldc, a_scale, b_scale, row_bias, col_bias, C};
-    const bool vec = (reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | static_cast<uintptr_t>(lda) | static_cast<uintptr_t>(ldb)) % 16 == 0;
-    return dense_guard(ctx, [&]() -> int {
-        const hipStream_t st = pick_stream(ctx, stream);
-        with_type(out_type, [&](auto e) {
-            using E = typename decltype(e)::type;
-            if (vec)
-                launch_i8<E, true>(a, st);
-            else
-                launch_i8<E, false>(a, st);
+    return rs::no_throw([&]() -> int {
+        using namespace rs;
+        if (!type_ok(out_type)) return set_error(ctx, RS_ERR_INVALID, "out_type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
+        if (m < 0 || m > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "m out of range");
+        if (n < 0 || n > INT32_MAX) return set_error(ctx, RS_ERR_INVALID, "n out of range");
+        if (ceil_div(m, 128) * ceil_div(n, 128) > INT32_MAX / 512) return set_error(ctx, RS_ERR_UNSUPPORTED, "m x n is too large for one call");
+        if (k < 1) return set_error(ctx, RS_ERR_INVALID, "k must be at least 1");
+        if (k > RS_I8_MAX_K) return set_error(ctx, RS_ERR_UNSUPPORTED, "k must be at most 65536 (exact int32 sums)");
+        if (m == 0 || n == 0) return RS_OK;
+        for (const std::string& b : {check_matrix("A", A, k, lda, 1), check_matrix("B", B, k, ldb, 1), check_matrix("a_scale", a_scale, 1, 1, 4),
+                                     check_matrix("b_scale", b_scale, 1, 1, 4), check_matrix("C", C, n, ldc, type_size(out_type)),
+                                     row_bias ? check_matrix("row_bias", row_bias, 1, 1, 4) : std::string(),
+                                     col_bias ? check_matrix("col_bias", col_bias, 1, 1, 4) : std::string()})
+            if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
+        I8Args a{A, B, m, n, k, lda, ldb, ldc, a_scale, b_scale, row_bias, col_bias, C};
+        const bool vec = (reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B) | static_cast<uintptr_t>(lda) | static_cast<uintptr_t>(ldb)) % 16 == 0;
+        return dense_guard(ctx, [&]() -> int {
+            const hipStream_t st = pick_stream(ctx, stream);
+            with_type(out_type, [&](auto e) {
+                using E = typename decltype(e)::type;
+                if (vec)
+                    launch_i8<E, true>(a, st);
+                else
+                    launch_i8<E, false>(a, st);
+            });
+            return RS_OK;
         });
-        return RS_OK;
     });
 }

@@ -834,51 +834,55 @@ std::string check_sizes(int64_t rows, int64_t cols) {
 }  // namespace rs
 
 extern "C" int rs_orthogonalize_workspace(rs_ctx* ctx, int64_t rows, int64_t cols, int64_t* bytes) {
-    if (!bytes) return rs::set_error(ctx, RS_ERR_INVALID, "bytes is NULL");
-    *bytes = 0;
-    const std::string bad = rs::check_sizes(rows, cols);
-    if (!bad.empty()) return rs::set_error(ctx, RS_ERR_INVALID, bad);
-    if (std::min(rows, cols) > RS_DENSE_MAX_FACTORS)
-        return rs::set_error(ctx, RS_ERR_UNSUPPORTED, "the shorter side must be at most 512");
-    if (rows && cols) *bytes = rs::make_plan(rows, cols).bytes;
-    return RS_OK;
+    return rs::no_throw([&]() -> int {
+        if (!bytes) return rs::set_error(ctx, RS_ERR_INVALID, "bytes is NULL");
+        *bytes = 0;
+        const std::string bad = rs::check_sizes(rows, cols);
+        if (!bad.empty()) return rs::set_error(ctx, RS_ERR_INVALID, bad);
+        if (std::min(rows, cols) > RS_DENSE_MAX_FACTORS)
+            return rs::set_error(ctx, RS_ERR_UNSUPPORTED, "the shorter side must be at most 512");
+        if (rows && cols) *bytes = rs::make_plan(rows, cols).bytes;
+        return RS_OK;
+    });
 }
 
 extern "C" int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, const void* G, int64_t ldg, int32_t steps,
                                 double a, double b, double c, void* X, int64_t ldx, void* ws, int64_t ws_bytes, void* stream) {
-    using namespace rs;
-    if (!type_ok(type)) return set_error(ctx, RS_ERR_INVALID, "type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
-    const std::string bad = check_sizes(rows, cols);
-    if (!bad.empty()) return set_error(ctx, RS_ERR_INVALID, bad);
-    if (std::min(rows, cols) > RS_DENSE_MAX_FACTORS) return set_error(ctx, RS_ERR_UNSUPPORTED, "the shorter side must be at most 512");
-    if (steps < 1 || steps > RS_ORTHO_MAX_STEPS) return set_error(ctx, RS_ERR_INVALID, "steps must be in [1, 16]");
-    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return set_error(ctx, RS_ERR_INVALID, "coefficients must be finite");
-    if (rows == 0 || cols == 0) return RS_OK;
-    for (const std::string& m : {check_matrix("G", G, cols, ldg, type_size(type)), check_matrix("X", X, cols, ldx, type_size(type))})
-        if (!m.empty()) return set_error(ctx, RS_ERR_INVALID, m);
-    if (G == X && ldg != ldx) return set_error(ctx, RS_ERR_INVALID, "X is G with another row stride");
-    if (G != X && overlap(G, ldg, X, ldx, rows, cols, type_size(type)))
-        return set_error(ctx, RS_ERR_INVALID, "X overlaps G");
-    if (G == X && std::min(rows, cols) > 256) return set_error(ctx, RS_ERR_UNSUPPORTED, "X may be G only where the shorter side is at most 256");
-    const OrthoPlan p = make_plan(rows, cols);
-    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");
-    if (ws_bytes < p.bytes)
-        return set_error(ctx, RS_ERR_INVALID, "ws holds " + std::to_string(ws_bytes) + " bytes, " + std::to_string(p.bytes) + " needed");
-    return dense_guard(ctx, [&]() -> int {
-        const hipStream_t st = pick_stream(ctx, stream);
-        with_type(type, [&](auto e) {
-            using E = typename decltype(e)::type;
-            // four elements at once where every row starts on a multiple of four
-            const bool vec = reinterpret_cast<uintptr_t>(G) % (4 * sizeof(E)) == 0 && ldg % 4 == 0;
-            auto go = [&](auto wide, auto v) {
-                run<E, decltype(wide)::value, decltype(v)::value>(p, static_cast<const E*>(G), ldg, steps, a, b, c, static_cast<E*>(X), ldx,
-                                                                  static_cast<char*>(ws), st);
-            };
-            if (rows >= cols)
-                vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
-            else
-                vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+    return rs::no_throw([&]() -> int {
+        using namespace rs;
+        if (!type_ok(type)) return set_error(ctx, RS_ERR_INVALID, "type must be RS_TYPE_F32, RS_TYPE_BF16 or RS_TYPE_F16");
+        const std::string bad = check_sizes(rows, cols);
+        if (!bad.empty()) return set_error(ctx, RS_ERR_INVALID, bad);
+        if (std::min(rows, cols) > RS_DENSE_MAX_FACTORS) return set_error(ctx, RS_ERR_UNSUPPORTED, "the shorter side must be at most 512");
+        if (steps < 1 || steps > RS_ORTHO_MAX_STEPS) return set_error(ctx, RS_ERR_INVALID, "steps must be in [1, 16]");
+        if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return set_error(ctx, RS_ERR_INVALID, "coefficients must be finite");
+        if (rows == 0 || cols == 0) return RS_OK;
+        for (const std::string& m : {check_matrix("G", G, cols, ldg, type_size(type)), check_matrix("X", X, cols, ldx, type_size(type))})
+            if (!m.empty()) return set_error(ctx, RS_ERR_INVALID, m);
+        if (G == X && ldg != ldx) return set_error(ctx, RS_ERR_INVALID, "X is G with another row stride");
+        if (G != X && overlap(G, ldg, X, ldx, rows, cols, type_size(type)))
+            return set_error(ctx, RS_ERR_INVALID, "X overlaps G");
+        if (G == X && std::min(rows, cols) > 256) return set_error(ctx, RS_ERR_UNSUPPORTED, "X may be G only where the shorter side is at most 256");
+        const OrthoPlan p = make_plan(rows, cols);
+        if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");
+        if (ws_bytes < p.bytes)
+            return set_error(ctx, RS_ERR_INVALID, "ws holds " + std::to_string(ws_bytes) + " bytes, " + std::to_string(p.bytes) + " needed");
+        return dense_guard(ctx, [&]() -> int {
+            const hipStream_t st = pick_stream(ctx, stream);
+            with_type(type, [&](auto e) {
+                using E = typename decltype(e)::type;
+                // four elements at once where every row starts on a multiple of four
+                const bool vec = reinterpret_cast<uintptr_t>(G) % (4 * sizeof(E)) == 0 && ldg % 4 == 0;
+                auto go = [&](auto wide, auto v) {
+                    run<E, decltype(wide)::value, decltype(v)::value>(p, static_cast<const E*>(G), ldg, steps, a, b, c, static_cast<E*>(X), ldx,
+                                                                      static_cast<char*>(ws), st);
+                };
+                if (rows >= cols)
+                    vec ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
+                else
+                    vec ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
+            });
+            return RS_OK;
         });
-        return RS_OK;
     });
 }

@@ -782,55 +782,59 @@ std::string check_sizes(int32_t type, int64_t n, int64_t v, int32_t k) {
 
 extern "C" int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors,
                                        int32_t with_grad, int64_t* bytes) {
-    if (!bytes) return rs::set_error(ctx, RS_ERR_INVALID, "bytes is NULL");
-    *bytes = 0;
-    const std::string bad = rs::check_sizes(type, n_rows, n_items, n_factors);
-    if (!bad.empty()) return rs::set_error(ctx, RS_ERR_INVALID, bad);
-    if (n_factors > RS_DENSE_MAX_FACTORS) return rs::set_error(ctx, RS_ERR_UNSUPPORTED, "n_factors must be at most 512");
-    if (n_rows && n_items) *bytes = rs::make_plan(type, n_rows, n_items, n_factors, with_grad).bytes;
-    return RS_OK;
+    return rs::no_throw([&]() -> int {
+        if (!bytes) return rs::set_error(ctx, RS_ERR_INVALID, "bytes is NULL");
+        *bytes = 0;
+        const std::string bad = rs::check_sizes(type, n_rows, n_items, n_factors);
+        if (!bad.empty()) return rs::set_error(ctx, RS_ERR_INVALID, bad);
+        if (n_factors > RS_DENSE_MAX_FACTORS) return rs::set_error(ctx, RS_ERR_UNSUPPORTED, "n_factors must be at most 512");
+        if (n_rows && n_items) *bytes = rs::make_plan(type, n_rows, n_items, n_factors, with_grad).bytes;
+        return RS_OK;
+    });
 }
 
 extern "C" int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, const void* H,
                              int64_t ldh, const void* W, int64_t ldw, const float* bias, const int32_t* target,
                              const float* weight, float* loss, float* lse, void* dH, int64_t lddh, void* dW, int64_t lddw,
                              float* dbias, void* ws, int64_t ws_bytes, void* stream) {
-    using namespace rs;
-    std::string bad = check_sizes(type, n_rows, n_items, n_factors);
-    if (!bad.empty()) return set_error(ctx, RS_ERR_INVALID, bad);
-    if (n_factors > RS_DENSE_MAX_FACTORS) return set_error(ctx, RS_ERR_UNSUPPORTED, "n_factors must be at most 512");
-    const int grads = (dH != nullptr) + (dW != nullptr) + (dbias != nullptr);
-    if (grads != 0 && grads != 3 && n_rows && n_items)
-        return set_error(ctx, RS_ERR_INVALID, "dH, dW and dbias are given together or not at all");
-    if (n_rows == 0 && n_items == 0) return RS_OK;
-    if (n_rows == 0 || n_items == 0)
-        return set_error(ctx, RS_ERR_INVALID, n_rows ? "n_items is 0" : "n_rows is 0");
-    const int64_t e = type_size(type);
-    for (const std::string& b : {check_matrix("H", H, n_factors, ldh, e), check_matrix("W", W, n_factors, ldw, e),
-                                 check_matrix("target", target, 1, 1, 4), check_matrix("loss", loss, 1, 1, 4),
-                                 check_matrix("lse", lse, 1, 1, 4),
-                                 grads ? check_matrix("dH", dH, n_factors, lddh, e) : std::string(),
-                                 grads ? check_matrix("dW", dW, n_factors, lddw, e) : std::string(),
-                                 grads ? check_matrix("dbias", dbias, 1, 1, 4) : std::string(),
-                                 bias ? check_matrix("bias", bias, 1, 1, 4) : std::string(),
-                                 weight ? check_matrix("weight", weight, 1, 1, 4) : std::string()})
-        if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
-    CeArgs a{};
-    a.p = make_plan(type, n_rows, n_items, n_factors, grads == 3);
-    if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");
-    if (ws_bytes < a.p.bytes)
-        return set_error(ctx, RS_ERR_INVALID, "ws holds " + std::to_string(ws_bytes) + " bytes, " + std::to_string(a.p.bytes) + " needed");
-    a.H = H, a.W = W, a.ldh = ldh, a.ldw = ldw, a.bias = bias, a.target = target, a.weight = weight;
-    a.loss = loss, a.lse = lse, a.dH = dH, a.dW = dW, a.lddh = lddh, a.lddw = lddw, a.dbias = dbias;
-    a.ws = static_cast<char*>(ws);
-    return dense_guard(ctx, [&]() -> int {
-        const hipStream_t st = pick_stream(ctx, stream);
-        if (type == RS_TYPE_F32)
-            launch_all<float, 2>(a, st);
-        else if (type == RS_TYPE_BF16)
-            launch_all<__bf16, 1>(a, st);
-        else
-            launch_all<_Float16, 1>(a, st);
-        return RS_OK;
+    return rs::no_throw([&]() -> int {
+        using namespace rs;
+        std::string bad = check_sizes(type, n_rows, n_items, n_factors);
+        if (!bad.empty()) return set_error(ctx, RS_ERR_INVALID, bad);
+        if (n_factors > RS_DENSE_MAX_FACTORS) return set_error(ctx, RS_ERR_UNSUPPORTED, "n_factors must be at most 512");
+        const int grads = (dH != nullptr) + (dW != nullptr) + (dbias != nullptr);
+        if (grads != 0 && grads != 3 && n_rows && n_items)
+            return set_error(ctx, RS_ERR_INVALID, "dH, dW and dbias are given together or not at all");
+        if (n_rows == 0 && n_items == 0) return RS_OK;
+        if (n_rows == 0 || n_items == 0)
+            return set_error(ctx, RS_ERR_INVALID, n_rows ? "n_items is 0" : "n_rows is 0");
+        const int64_t e = type_size(type);
+        for (const std::string& b : {check_matrix("H", H, n_factors, ldh, e), check_matrix("W", W, n_factors, ldw, e),
+                                     check_matrix("target", target, 1, 1, 4), check_matrix("loss", loss, 1, 1, 4),
+                                     check_matrix("lse", lse, 1, 1, 4),
+                                     grads ? check_matrix("dH", dH, n_factors, lddh, e) : std::string(),
+                                     grads ? check_matrix("dW", dW, n_factors, lddw, e) : std::string(),
+                                     grads ? check_matrix("dbias", dbias, 1, 1, 4) : std::string(),
+                                     bias ? check_matrix("bias", bias, 1, 1, 4) : std::string(),
+                                     weight ? check_matrix("weight", weight, 1, 1, 4) : std::string()})
+            if (!b.empty()) return set_error(ctx, RS_ERR_INVALID, b);
+        CeArgs a{};
+        a.p = make_plan(type, n_rows, n_items, n_factors, grads == 3);
+        if (!ws || reinterpret_cast<uintptr_t>(ws) % 16) return set_error(ctx, RS_ERR_INVALID, "ws is NULL or not 16-byte aligned");
+        if (ws_bytes < a.p.bytes)
+            return set_error(ctx, RS_ERR_INVALID, "ws holds " + std::to_string(ws_bytes) + " bytes, " + std::to_string(a.p.bytes) + " needed");
+        a.H = H, a.W = W, a.ldh = ldh, a.ldw = ldw, a.bias = bias, a.target = target, a.weight = weight;
+        a.loss = loss, a.lse = lse, a.dH = dH, a.dW = dW, a.lddh = lddh, a.lddw = lddw, a.dbias = dbias;
+        a.ws = static_cast<char*>(ws);
+        return dense_guard(ctx, [&]() -> int {
+            const hipStream_t st = pick_stream(ctx, stream);
+            if (type == RS_TYPE_F32)
+                launch_all<float, 2>(a, st);
+            else if (type == RS_TYPE_BF16)
+                launch_all<__bf16, 1>(a, st);
+            else
+                launch_all<_Float16, 1>(a, st);
+            return RS_OK;
+        });
     });
 }
