@@ -108,6 +108,7 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
                                 : static_cast<double>(std::max<int64_t>(tx * s, 256)) / 256 * (one + 2.0) + 0.5 * one;
             if (s > 1 || mode != kItems) cost += static_cast<double>(s) * sums;
             if (s > 1 && mode == kItems) cost += 5.0;  // the join's launch
+            if (mode != kItems) cost += 0.05 * static_cast<double>(s);  // a row's pieces are read one after the other
             if (s == 1 || cost < best) best = cost, *splits = static_cast<int32_t>(s), *tiles = static_cast<int32_t>(per);
             if (per == 1) break;
             per = ceil_div(ty, ceil_div(ty, per - 1));
@@ -581,12 +582,14 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     }
 }
 
-// ---- joining the splits of the catalogue: lse, loss, dH and what the dW pass reads of each row; a wave per row -----
-template <typename E>
-__global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
+// ---- joining the splits of the catalogue: lse, loss, dH and what the dW pass reads of each row --------------------
+// W waves per row: one, or where few rows have many splits the eight of a workgroup, which share the splits (27 x 635201
+// x 92 fp32, 1655 splits: 89 us, 355 with one; 1024 x 1e6 x 256, 64 splits: 18 us and 30).
+template <typename E, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
-    const int lane = threadIdx.x & 63;
-    const int64_t n = wide_block() * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t n = W == 1 ? wide_block() * 4 + wave : wide_block();
     const int64_t rows = p.grad ? p.n_pad : p.n;
     if (n >= rows) return;
     const Scal sc = *a.at<Scal>(p.o_scal);
@@ -621,14 +624,14 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     s = there ? rest + __builtin_amdgcn_exp2f(lt2 - m) : rest;
     // lse = m ln 2 + ls, in two parts: where m is large they must not be joined before the target's logit goes
     const float ls = first ? log1pf(rest) : log2f(s) * kLn2;
-    if (lane == 0 && n < p.n) {
+    if (lane == 0 && (W == 1 || wave == 0) && n < p.n) {
         a.lse[n] = !known ? 0.f : empty ? -INFINITY : fmaf(m, kLn2, ls);
         a.loss[n] = !known || empty ? 0.f : there ? fmaf(m - lt2, kLn2, ls) : INFINITY;
     }
     if (!p.grad) return;
     const bool live = there && !empty;
     const float w = live ? (a.weight ? a.weight[n] : 1.f) : 0.f;
-    if (lane == 0) {
+    if (lane == 0 && (W == 1 || wave == 0)) {
         float* row = a.at<float>(p.o_row) + n;
         row[0] = live ? m : INFINITY;
         row[p.n_pad] = live ? w * sc.cs / s : 0.f;
@@ -642,17 +645,18 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
     const int quads = p.kp / 4, lanes = quads < 64 ? quads : 64, groups = 64 / lanes, grp = lane / lanes;
     const float* O = a.at<float>(p.o_part) + n * p.kp;
     const int64_t step = p.n_pad * p.kp;
+    const int share_w = (p.splits_f + W - 1) / W, i_first = W == 1 ? 0 : wave * share_w, i_last = min(p.splits_f, i_first + share_w);
     for (int c = lane % lanes * 4; c < p.kp; c += 256) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         if (live)
-            for (int i0 = 0; i0 < p.splits_f; i0 += 64) {
+            for (int i0 = i_first; i0 < i_last; i0 += 64) {
                 // the factors of 64 splits, one a lane
                 float f = 0.f;
-                if (i0 + lane < p.splits_f) {
+                if (i0 + lane < i_last) {
                     const float mi = i0 ? pm[(i0 + lane) * p.n_pad] : m0;
                     f = __builtin_amdgcn_exp2f((mi - m) - shift_of(mi));
                 }
-                const int count = min(64, p.splits_f - i0);
+                const int count = min(64, i_last - i0);
 #pragma unroll 8
                 for (int i = 0; i < count; i += groups) {  // (as often in every lane: a shuffle reads active lanes only)
                     const float fi = __shfl(f, i + grp);
@@ -665,7 +669,18 @@ __global__ __launch_bounds__(256) void ce_join_kernel(CeArgs a) {
         for (int g = lanes; g < 64; g <<= 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], g);
-        if (grp == 0)
+        if constexpr (W > 1) {
+            __shared__ f32x4 sums[W - 1][64];
+            if (wave) sums[wave - 1][lane] = o;
+            __syncthreads();
+            if (wave == 0)
+#pragma unroll
+                for (int w = 0; w < W - 1; ++w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] += sums[w][lane][e];
+            __syncthreads();
+        }
+        if (grp == 0 && (W == 1 || wave == 0))
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (c + e < p.k) out[c + e] = static_cast<E>(live ? w * (o[e] * inv - share_rest * static_cast<float>(wt[c + e])) : 0.f);
@@ -758,7 +773,10 @@ void launch_all(const CeArgs& a, hipStream_t st) {
         mode(std::integral_constant<int, kLossGrad>{});
     else
         mode(std::integral_constant<int, kLoss>{});
-    ce_join_kernel<E><<<wide_grid(ceil_div(p.grad ? p.n_pad : p.n, 4)), 256, 0, st>>>(a);
+    if (p.grad && p.splits_f >= 16 && p.n <= 2048)
+        ce_join_kernel<E, 8><<<wide_grid(p.grad ? p.n_pad : p.n), 512, 0, st>>>(a);
+    else
+        ce_join_kernel<E, 1><<<wide_grid(ceil_div(p.grad ? p.n_pad : p.n, 4)), 256, 0, st>>>(a);
     RS_HIP(hipGetLastError());
     if (!p.grad) return;
     mode(std::integral_constant<int, kItems>{});
