@@ -38,6 +38,8 @@ namespace {
 
 constexpr int kPad = 256;        // rows are padded to this: a multiple of what a workgroup holds or a stage streams
 constexpr int kTileY = 128;      // streamed rows are split over workgroups in multiples of this
+constexpr int kFewRows = 4;      // rows that the table is read for as it is, without gradients
+constexpr int kFewItems = 128;   // items that a workgroup has on their way then: 8 waves x 4 x 4
 constexpr int kMaxBlocks = 1024;  // blocks of the maxima pass at most, per matrix
 // p = 2^(l2 - m) is held as 2^shift_of(m) p (fp16's range below 1 is short; beside a large m the shift would be lost in
 // the difference), and m may lag the maximum by kLag: moving it at each new maximum costs a pass over the sums in most
@@ -78,6 +80,7 @@ struct Scal {
 struct CePlan {
     int64_t n, v, n_pad, v_pad;
     int32_t k, kp, np, oc, z, type, grad;
+    int32_t few;  // ce_few_kernel: no packed tables
     int32_t splits_f, tiles_f, splits_w, tiles_w;  // splits of the streamed rows and their tiles each
     int64_t o_max, o_scal, o_h, o_w, o_bias, o_m, o_s, o_row, o_part, o_db, bytes;
 };
@@ -116,6 +119,8 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
     };
     split(n, v, kLossGrad, &p.splits_f, &p.tiles_f);
     split(v, n, kItems, &p.splits_w, &p.tiles_w);
+    p.few = !grad && n <= kFewRows;
+    if (p.few) p.splits_f = static_cast<int32_t>(std::min<int64_t>(512, ceil_div(v, kFewItems)));
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t o = at;
@@ -124,9 +129,9 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
     };
     p.o_max = take(3 * kMaxBlocks * 4);
     p.o_scal = take(sizeof(Scal));
-    p.o_h = take(p.n_pad * p.kp * 2 * p.np);
-    p.o_w = take(p.v_pad * p.kp * 2 * p.np);
-    p.o_bias = take(p.v_pad * 4);
+    p.o_h = take(p.few ? 0 : p.n_pad * p.kp * 2 * p.np);
+    p.o_w = take(p.few ? 0 : p.v_pad * p.kp * 2 * p.np);
+    p.o_bias = take(p.few ? 0 : p.v_pad * 4);
     p.o_m = take(p.splits_f * p.n_pad * 4);
     p.o_s = take(p.splits_f * p.n_pad * 4);
     if (grad) {
@@ -582,6 +587,89 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     }
 }
 
+// ---- a few rows without gradients: the table is read once, as it is ------------------------------------------------
+// Packing it for four rows would cost more than its products (2 x 108938 x 317 bf16, rows not aligned: 90 us in all, 173
+// packed; aligned, 4 x 108944 x 320 43 us and the join's 9, one row 19 and 9: 3.7 TB/s).  The rows
+// stay in registers in fp32; sixteen lanes take an item, eight columns each at a time, and sum its products by shuffles;
+// lane l keeps the running maximum and sum of row l mod R (one row, or
+// up to four).  KC: 128 columns each.
+template <typename E, bool VEC, int KC, int R>
+__global__ __launch_bounds__(512) void ce_few_kernel(CeArgs a) {
+#pragma clang fp contract(fast)
+    const CePlan& p = a.p;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, sub = lane >> 4, row = l & (R - 1);
+    const E *H = static_cast<const E*>(a.H), *W = static_cast<const E*>(a.W);
+    float h[R][KC][8];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < KC; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[r][j][e] = 0.f;
+            if (r < p.n && l * 8 + j * 128 < p.k) load8<E, VEC>(H + r * a.ldh, l * 8 + j * 128, p.k, h[r][j]);
+        }
+    constexpr int U = KC == 4 ? 2 : 4;  // items of a lane on their way (four of 512 columns would not fit the registers)
+    const int64_t target = row < p.n ? a.target[row] : -1;
+    float m = -INFINITY, s = 0.f;
+    for (int64_t v0 = static_cast<int64_t>(blockIdx.x) * kFewItems + wave * 16; v0 < p.v; v0 += static_cast<int64_t>(gridDim.x) * kFewItems) {
+#pragma unroll 1
+        for (int q = 0; q < 4; q += U) {
+            float w[U][KC][8], b[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t v = min(v0 + (q + u) * 4 + sub, p.v - 1);
+                b[u] = bounded_bias(a.bias ? a.bias[v] : 0.f) * kLog2e;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[u][j][e] = 0.f;
+                    if (l * 8 + j * 128 < p.k) load8<E, VEC>(W + v * a.ldw, l * 8 + j * 128, p.k, w[u][j]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t v = v0 + (q + u) * 4 + sub;
+                float dot[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    dot[r] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < KC; ++j)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dot[r] = fmaf(h[r][j][e], w[u][j][e], dot[r]);
+#pragma unroll
+                    for (int o = 8; o; o >>= 1) dot[r] += __shfl_xor(dot[r], o);
+                }
+                const float mine = R == 1 || row == 0 ? dot[0] : row == 1 ? dot[1 % R] : row == 2 ? dot[2 % R] : dot[3 % R];
+                // a withdrawn item may hold anything; the row's target joins at the end
+                const float l2 = v >= p.v || b[u] == -INFINITY || v == target ? -INFINITY : fmaf(mine, kLog2e, b[u]);
+                const float top = fmaxf(m, l2);
+                if (top > -INFINITY || l2 != l2) {
+                    s = s * __builtin_amdgcn_exp2f(m - top) + __builtin_amdgcn_exp2f(l2 - top);
+                    m = top;
+                }
+            }
+        }
+    }
+    // the four items at a time, then the waves
+    auto meet = [&](float m2, float s2) {
+        const float top = fmaxf(m, m2);
+        s = top == -INFINITY ? s + s2 : s * __builtin_amdgcn_exp2f(m - top) + s2 * __builtin_amdgcn_exp2f(m2 - top);
+        m = top;
+    };
+    meet(__shfl_xor(m, 16), __shfl_xor(s, 16));
+    meet(__shfl_xor(m, 32), __shfl_xor(s, 32));
+    __shared__ float sm[2][8][R];
+    if (lane < R) sm[0][wave][lane] = m, sm[1][wave][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < R) {
+        for (int w = 1; w < 8; ++w) meet(sm[0][w][lane], sm[1][w][lane]);
+        const int64_t at = blockIdx.x * p.n_pad + lane;
+        a.at<float>(p.o_m)[at] = m;
+        a.at<float>(p.o_s)[at] = s * __builtin_amdgcn_exp2f(shift_of(m));  // (as the passes keep it)
+    }
+}
+
 // ---- joining the splits of the catalogue: lse, loss, dH and what the dW pass reads of each row --------------------
 // W waves per row: one, or where few rows have many splits the eight of a workgroup, which share the splits (27 x 635201
 // x 92 fp32, 1655 splits: 89 us, 355 with one; 1024 x 1e6 x 256, 64 splits: 18 us and 30).
@@ -610,7 +698,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a
         for (int c = lane; c < p.k; c += 64) lt = fmaf(static_cast<float>(h[c]), static_cast<float>(wt[c]), lt);
     lt = wave_sum_f32(lt);
     // the target's logit in base 2, rounded as the passes round theirs; the maximum over all items
-    const float lt2 = there ? fmaf(lt, kLog2e, a.at<float>(p.o_bias)[tg]) : -INFINITY;
+    const float lt2 = there ? fmaf(lt, kLog2e, bounded_bias(a.bias ? a.bias[tg] : 0.f) * kLog2e) : -INFINITY;
     const bool first = lt2 >= m;
     if (first) m = lt2;
     auto share = [&](float mi, float si) { return m == -INFINITY ? si : si * __builtin_amdgcn_exp2f((mi - m) - shift_of(mi)); };
@@ -755,6 +843,29 @@ void launch_all(const CeArgs& a, hipStream_t st) {
         ce_pack_kernel<E, NP, VEC><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(p.n_pad + p.v_pad, step), 8192)), 256, 0, st>>>(a, blocks);
         RS_HIP(hipGetLastError());
     };
+    if (p.few) {
+        auto few = [&](auto v, auto kc) {
+            constexpr bool VEC = decltype(v)::value;
+            constexpr int KC = decltype(kc)::value;
+            if (p.n == 1)
+                ce_few_kernel<E, VEC, KC, 1><<<static_cast<uint32_t>(p.splits_f), 512, 0, st>>>(a);
+            else
+                ce_few_kernel<E, VEC, KC, kFewRows><<<static_cast<uint32_t>(p.splits_f), 512, 0, st>>>(a);
+            RS_HIP(hipGetLastError());
+        };
+        auto wide = [&](auto v) {
+            if (p.k <= 128)
+                few(v, std::integral_constant<int, 1>{});
+            else if (p.k <= 256)
+                few(v, std::integral_constant<int, 2>{});
+            else
+                few(v, std::integral_constant<int, 4>{});
+        };
+        vec ? wide(std::true_type{}) : wide(std::false_type{});
+        ce_join_kernel<E, 1><<<wide_grid(ceil_div(p.n, 4)), 256, 0, st>>>(a);
+        RS_HIP(hipGetLastError());
+        return;
+    }
     if (vec)
         prepare(std::true_type{});
     else

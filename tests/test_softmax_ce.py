@@ -136,6 +136,28 @@ def test_split_sums(ctx, n, v, k, ty):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,v,k", [(1, 1, 1), (1, 17, 8), (2, 130, 100), (3, 129, 128), (4, 1000, 129), (4, 5000, 256), (1, 70001, 257), (2, 9001, 317),
+                                   (4, 2000, 512), (5, 2000, 60)])
+def test_a_few_rows_without_gradients(ctx, n, v, k, ty):
+    H, W, target, b, _ = make(n, v, k, ty, seed=n + v, bias=v > 1, gone=0.1)
+    big = torch.full((v, k + 3), math.nan, dtype=T[ty], device="cuda")
+    big[:, :k] = W
+    for table in (W, big[:, :k]):  # (aligned rows, and others)
+        check(ctx.softmax_ce(H, table, target, bias=b), reference(H, W, target, b), ty, k, grad=False)
+    if n > 1:
+        target[1], H[1] = -1, math.nan
+        W[v // 2] = math.nan
+        if b is not None and v > 2:
+            b[v // 2] = -math.inf
+            check(ctx.softmax_ce(H, W, target, bias=b), reference(H, W, target, b), ty, k, grad=False)
+    gone = torch.full((v,), -math.inf, device="cuda")
+    loss, lse = ctx.softmax_ce(H, W, target, bias=gone)
+    known = target >= 0
+    assert (lse[known] == -math.inf).all() and (loss == 0).all() and (lse[~known] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
 def test_no_bias_no_weight(ctx, ty):
     H, W, target, _, _ = make(77, 333, 40, ty, seed=3)
     check(ctx.softmax_ce(H, W, target, grad=True), reference(H, W, target), ty, 40)
