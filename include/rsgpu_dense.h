@@ -60,10 +60,10 @@ int rs_softmax_ce(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, in
                   void* ws, int64_t ws_bytes, void* stream);
 
 /* Rows in 8 bits with a scale each: scale_r = max_c |x_rc| * (1/127), both factors and the product in fp32,
- * q_rc = x_rc / scale_r to the nearest integer, ties to even, decided on the exact quotient; |q| <= 127.  A row of
- * zeros, or whose scale underflows to 0, has scale 0 and q 0; a row with an infinity or NaN has scale NaN and q 0, so
- * that all its products are NaN.  X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as they
- * are.  n_cols >= 1. */
+ * q_rc = x_rc / scale_r to the nearest integer, ties to even, decided on the exact quotient, held to |q| <= 127 (a
+ * subnormal scale may be rounded down so far that the quotient passes it).  A row of zeros, or whose scale underflows
+ * to 0, has scale 0 and q 0; a row with an infinity or NaN has scale NaN and q 0, so that all its products are NaN.
+ * X of `type`, q int8 with row stride ldq (bytes); columns past n_cols are left as they are.  n_cols >= 1. */
 int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_cols, const void* X, int64_t ldx, int8_t* q,
                      int64_t ldq, float* scale, void* stream);
 

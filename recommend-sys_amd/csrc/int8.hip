@@ -93,7 +93,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const E* __restrict_
         uint32_t w[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int n = quantize(fabsf(v[e]) * pre, sp, inv);
+            // (a subnormal scale may be rounded down by a third of itself: the quotient of the row's largest then passes 127)
+            const int n = min(quantize(fabsf(v[e]) * pre, sp, inv), 127);
             w[e / 4] |= static_cast<uint32_t>((v[e] < 0.f ? -n : n) & 255) << (8 * (e % 4));
         }
         w[0] &= some, w[1] &= some;

@@ -291,3 +291,22 @@ def test_entry_point_refusals():
     for kw in (dict(), dict(ty=3), dict(r=-1), dict(c=0), dict(X=None), dict(X=p + 1), dict(ldx=3), dict(q=None), dict(ldq=3), dict(s=None)):
         assert quant(**kw) == rsgpu.RS_ERR_INVALID, kw
     assert quant(r=0) == rsgpu.RS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_quantize_subnormal_scales(ctx, ty):
+    """max * (1/127) below 2^-126 is rounded to a multiple of 2^-149, by up to half of itself: the quotient of the largest
+    value passes 127 (190 * 2^-149 has the scale 2^-149) and is held there."""
+    units = torch.cat([torch.arange(1, 700), torch.arange(700, 16200, 37), torch.tensor([16064, 16065, 16128, 16129, 65536, 131072, 8388607, 8388608])])
+    x = torch.zeros(2 * len(units), 5)
+    x[:, 0] = torch.cat([units, units]).to(torch.int32).view(torch.float32)
+    x[:, 1] = -x[:, 0]
+    x[:, 2] = (torch.cat([units, units]) * 2 // 3).to(torch.int32).view(torch.float32)
+    x[:, 3] = -1.0 * torch.ones(1, dtype=torch.int32).view(torch.float32)
+    x[len(units):] *= -1
+    x = x.to(T[ty]).cuda()
+    q, s = ctx.quantize_rows(x)
+    rq, rs = quantize_reference(x)
+    assert torch.equal(s.cpu(), rs) and torch.equal(q.cpu().long(), rq)
+    assert (q.cpu().long().abs() <= 127).all()
