@@ -48,9 +48,10 @@ extern "C" {
  * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
  * (hi + lo), so an element keeps 2^-24 of itself or 2^-38 of the matrix's largest element, whichever is more;
  * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Coefficients c_nv
- * are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise.  The target's coefficient is minus the sum of
- * the row's others: the gradients of a row keep their precision where its target's probability is near one, as does
- * its loss.
+ * are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise, or to 2^-32 (dH) and 2^-33 (dW) of the largest
+ * so far in the same sum, whichever is more: each row of dW keeps its precision however improbable its item and small the
+ * weights.  A probability below 2^-126 counts as zero.  The target's coefficient is minus the sum of the row's others:
+ * the gradients of a row keep their precision where its target's probability is near one, as does its loss.
  * n_rows and n_items from 1 to 2^31 - 1025 (or both 0). */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);

@@ -45,6 +45,11 @@ constexpr int kMaxBlocks = 1024;  // blocks of the maxima pass at most, per matr
 // the difference), and m may lag the maximum by kLag: moving it at each new maximum costs a pass over the sums in most
 // tiles (32 columns a wave, each with its own records)
 constexpr float kLag = 8.f;
+// a column's coefficients in the items' pass, weight p / s, are held times a power of two that brings the largest so far
+// to [2^kCoefAt, 2^15]: whatever the item's probabilities and the weights, none is rounded by more than its 11 bits (two
+// pieces: 22) or 2^-25, 2^-33 of the largest (one scale for the batch left nothing of an item that no row thinks likely).
+// Brought to 2^11: 1024 x 1e6 x 256 bf16 2.81 ms, 2.69 with 2^8, where the scale moves less often.
+constexpr int kCoefAt = 8;
 __device__ __forceinline__ float shift_of(float m) { return fabsf(m) < 32768.f ? 7.f : 0.f; }
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -68,13 +73,11 @@ constexpr Shape shape_for(int np, int kp, int mode) {
     return {4, 2, 2};
 }
 
-// Device scalars (ws): the powers of two that scale H, W and the weights, and what undoes them.
+// Device scalars (ws): the powers of two that scale H and W, and what undoes them.
 struct Scal {
-    float hs, wsc, cs;   // H, W, weights are multiplied by these
-    float logit;         // S -> base-2 logit: log2(e) / (hs wsc)
-    float inv_w;         // 1 / wsc
-    float inv_dw;        // 1 / (cs hs)
-    float inv_cs;        // 1 / cs
+    float hs, wsc;  // H, W are multiplied by these
+    float logit;    // S -> base-2 logit: log2(e) / (hs wsc)
+    float inv_w, inv_h;
 };
 
 struct CePlan {
@@ -127,7 +130,7 @@ CePlan make_plan(int32_t type, int64_t n, int64_t v, int32_t k, int32_t grad) {
         at += round_up(bytes, 256);
         return o;
     };
-    p.o_max = take(3 * kMaxBlocks * 4);
+    p.o_max = take(2 * kMaxBlocks * 4);
     p.o_scal = take(sizeof(Scal));
     p.o_h = take(p.few ? 0 : p.n_pad * p.kp * 2 * p.np);
     p.o_w = take(p.few ? 0 : p.v_pad * p.kp * 2 * p.np);
@@ -195,14 +198,12 @@ __device__ __forceinline__ float scale_for(uint32_t max_bits) {
     return __uint_as_float(static_cast<uint32_t>(min(max(e, -100), 100) + 127) << 23);
 }
 
-__device__ __forceinline__ Scal scales(float hs, float wsc, float cs) {
-    Scal s;
-    s.hs = hs, s.wsc = wsc, s.cs = cs;
-    s.logit = kLog2e / hs / wsc;
-    s.inv_w = 1.f / wsc;
-    s.inv_dw = 1.f / cs / hs;
-    s.inv_cs = 1.f / cs;
-    return s;
+__device__ __forceinline__ Scal scales(float hs, float wsc) { return {hs, wsc, kLog2e / hs / wsc, 1.f / wsc, 1.f / hs}; }
+
+// 2^e with x 2^e in [2^kCoefAt, 2^(kCoefAt + 1)), for x > 0 (as far as the power and its inverse are normal numbers)
+__device__ __forceinline__ float coef_scale(float x) {
+    const int e = kCoefAt + 127 - static_cast<int>(__float_as_uint(x) >> 23);
+    return __uint_as_float(static_cast<uint32_t>(min(e, 126) + 127) << 23);
 }
 
 __device__ __forceinline__ void see_largest(uint32_t& m, float x) {
@@ -210,30 +211,25 @@ __device__ __forceinline__ void see_largest(uint32_t& m, float x) {
     if (b < 0x7F800000u && b > m) m = b;
 }
 
-// ---- largest finite magnitudes of H, W and the weights (blockIdx.y = 0, 1, 2), one value per block ----------------
+// ---- largest finite magnitudes of H and W (blockIdx.y = 0, 1), one value per block ---------------------------------
 template <typename E, bool VEC>
 __global__ __launch_bounds__(256) void ce_max_kernel(CeArgs a) {
     const CePlan& p = a.p;
     const int which = blockIdx.y;
     uint32_t m = 0;
-    if (which < 2) {
-        const E* X = static_cast<const E*>(which ? a.W : a.H);
-        const int64_t rows = which ? p.v : p.n, ld = which ? a.ldw : a.ldh;
-        const int lanes = p.kp / 8, at = threadIdx.x / lanes, c = threadIdx.x % lanes * 8;
-        const int64_t step = static_cast<int64_t>(gridDim.x) * (256 / lanes);
+    const E* X = static_cast<const E*>(which ? a.W : a.H);
+    const int64_t rows = which ? p.v : p.n, ld = which ? a.ldw : a.ldh;
+    const int lanes = p.kp / 8, at = threadIdx.x / lanes, c = threadIdx.x % lanes * 8;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (256 / lanes);
 #pragma unroll 4
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / lanes) + at; r < rows; r += step) {
-            if (c >= p.k) continue;
-            float v[8];
-            load8<E, VEC>(X + r * ld, c, p.k, v);
-            uint32_t t = 0;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * (256 / lanes) + at; r < rows; r += step) {
+        if (c >= p.k) continue;
+        float v[8];
+        load8<E, VEC>(X + r * ld, c, p.k, v);
+        uint32_t t = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) see_largest(t, v[e]);
-            if (t > m && (which ? item_there(a, r) : row_known(a, r))) m = t;  // (looked up for new records only)
-        }
-    } else if (a.weight) {
-        for (int64_t r = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; r < p.n; r += static_cast<int64_t>(gridDim.x) * 256)
-            if (row_known(a, r)) see_largest(m, a.weight[r]);
+        for (int e = 0; e < 8; ++e) see_largest(t, v[e]);
+        if (t > m && (which ? item_there(a, r) : row_known(a, r))) m = t;  // (looked up for new records only)
     }
     m = wave_max_u32(m);
     __shared__ uint32_t sm[4];
@@ -247,8 +243,8 @@ template <typename E, int NP, bool VEC>
 __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) {
     constexpr bool kScaled = !std::is_same<E, _Float16>::value;
     const CePlan& p = a.p;
-    __shared__ uint32_t sm[3];
-    if (threadIdx.x < 192) {
+    __shared__ uint32_t sm[2];
+    if (kScaled && threadIdx.x < 128) {
         const int which = threadIdx.x >> 6;
         uint32_t m = 0;
         for (int i = threadIdx.x & 63; i < max_blocks; i += 64) m = max(m, a.at<uint32_t>(p.o_max)[which * kMaxBlocks + i]);
@@ -257,8 +253,7 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
     }
     __syncthreads();
     const float hs = kScaled ? scale_for(sm[0]) : 1.f, wsc = kScaled ? scale_for(sm[1]) : 1.f;
-    // coefficients c = weight (p - [target]): |c| <= |weight| cs < 2^14
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.at<Scal>(p.o_scal) = scales(hs, wsc, scale_for(a.weight ? sm[2] : 0x3F800000u));
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.at<Scal>(p.o_scal) = scales(hs, wsc);
     const int lanes = p.kp / 8, at = threadIdx.x / lanes, c0 = threadIdx.x % lanes * 8, step = 256 / lanes;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * step + at; row < p.n_pad + p.v_pad; row += static_cast<int64_t>(gridDim.x) * step) {
         const bool w = row >= p.n_pad;
@@ -355,6 +350,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{0};
     float m_run = -INFINITY, sum = 0.f;
+    float coef = 1.f, coef_top = 0.f;  // items: a column's coefficients are held times coef, up to coef_top of their own size
     const float bias_x = items ? a.at<float>(p.o_bias)[x] : 0.f;
     const int target_x = !items && x < p.n ? a.target[x] : -1;
 
@@ -467,6 +463,19 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                         for (int e = 0; e < 4; ++e) s[4 * q + e] = t[e] == static_cast<int>(x) ? w[e] : s[4 * q + e];
                     }
                 }
+                float top = 0.f;
+#pragma unroll
+                for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) top = fmaxf(top, fabsf(s[i]));
+                if (__any(top > coef_top)) {  // the first block, and rarely after it
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float next = top > coef_top ? coef_scale(top) : coef, f = next / coef;
+                    if (top > coef_top) coef_top = 0x1p15f / next;
+                    coef = next;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                }
             } else {
 #pragma unroll
                 for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - off);
@@ -483,8 +492,9 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                     for (int e = 0; e < 8; ++e) {
                         float f = s[8 * j + e];
                         // the fp32 value itself is what both pieces come from: fused into the rounding of one of them, the
-                        // product before it would round to another hi now and then
+                        // product before it would round to another hi now and then (a power of two may be: it is exact)
                         if (NC == 2) asm("" : "+v"(f));
+                        if (items) f *= coef;
                         c[0][e] = static_cast<_Float16>(f);
                         if (NC == 2) c[NC - 1][e] = static_cast<_Float16>(f - static_cast<float>(c[0][e]));
                     }
@@ -523,8 +533,8 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     }
 
     const float total = sum + __shfl_xor(sum, 32);
-    // a split's sums: four columns of row x at a time
-    auto partial = [&](int64_t rows) {
+    // a split's sums, times `back`: four columns of row x at a time
+    auto partial = [&](int64_t rows, float back) {
         float* O = a.at<float>(p.o_part) + (split * rows + x) * KP + oc0;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -532,7 +542,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             for (int q = 0; q < 4; ++q) {
                 f32x4 o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * q + e];
+                for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * q + e] * back;
                 *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * q + 4 * half) = o;
             }
     };
@@ -541,12 +551,13 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             a.at<float>(p.o_m)[split * p.n_pad + x] = m_run;
             a.at<float>(p.o_s)[split * p.n_pad + x] = total;
         }
-        if constexpr (MODE == kLossGrad) partial(p.n_pad);
+        if constexpr (MODE == kLossGrad) partial(p.n_pad, 1.f);
     } else if (p.splits_w > 1) {
         if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = total;
-        partial(p.v_pad);
+        partial(p.v_pad, sc.inv_h / coef);
     } else {
-        if (x < p.v && blockIdx.z == 0 && half == 0) a.dbias[x] = total * sc.inv_cs;
+        if (x < p.v && blockIdx.z == 0 && half == 0) a.dbias[x] = total;
+        const float back = sc.inv_h / coef;
         // dW through LDS, so that a row's stores are contiguous: OW columns at a time, 16-byte chunk c of row r at
         // chunk c ^ (r mod the row's chunks)
         constexpr int OW = OC < 128 / static_cast<int>(sizeof(E)) ? OC : 128 / static_cast<int>(sizeof(E));
@@ -562,7 +573,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             for (int q = 0; q < OW / 8; ++q) {
                 e4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][4 * (q % 4) + e] * sc.inv_dw);
+                for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][4 * (q % 4) + e] * back);
                 const int byte = (8 * q + 4 * half) * static_cast<int>(sizeof(E));
                 *reinterpret_cast<words*>(mine + lx * kRow + (((byte >> 4) ^ (lx & (CH - 1))) << 4) + (byte & 15)) = __builtin_bit_cast(words, v);
             }
@@ -722,9 +733,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a
     if (lane == 0 && (W == 1 || wave == 0)) {
         float* row = a.at<float>(p.o_row) + n;
         row[0] = live ? m : INFINITY;
-        row[p.n_pad] = live ? w * sc.cs / s : 0.f;
+        row[p.n_pad] = live ? w / s : 0.f;
         row[2 * p.n_pad] = __int_as_float(live ? tg : -1);
-        row[3 * p.n_pad] = live ? -w * sc.cs * (rest / s) : 0.f;  // the target's coefficient, weight (p - 1)
+        row[3 * p.n_pad] = live ? -w * (rest / s) : 0.f;  // the target's coefficient, weight (p - 1)
     }
     if (n >= p.n) return;
     E* out = static_cast<E*>(a.dH) + n * a.lddh;
@@ -779,7 +790,6 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a
 template <typename E>
 __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
-    const Scal sc = *a.at<Scal>(p.o_scal);
     const int quads = p.kp / 4;  // (a power of two)
     const int64_t i = wide_block() * 256 + threadIdx.x, v = i >> __builtin_ctz(quads);
     const int c = (static_cast<int>(i) & (quads - 1)) * 4;
@@ -799,11 +809,11 @@ __global__ __launch_bounds__(256) void ce_items_join_kernel(CeArgs a) {
     E* out = static_cast<E*>(a.dW) + v * a.lddw;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (c + e < p.k) out[c + e] = static_cast<E>(o[e] * sc.inv_dw);
+        if (c + e < p.k) out[c + e] = static_cast<E>(o[e]);
     if (c == 0) {
         float d = 0.f;
         for (int s = 0; s < p.splits_w; ++s) d += a.at<float>(p.o_db)[s * p.v_pad + v];
-        a.dbias[v] = d * sc.inv_cs;
+        a.dbias[v] = d;
     }
 }
 
@@ -835,9 +845,9 @@ void launch_all(const CeArgs& a, hipStream_t st) {
         constexpr bool VEC = decltype(v)::value;
         const int64_t step = 256 / (p.kp / 8);  // rows of a block at a time
         int blocks = 0;
-        if (!std::is_same<E, _Float16>::value || (p.grad && a.weight)) {
+        if (!std::is_same<E, _Float16>::value) {
             blocks = static_cast<int>(std::min<int64_t>(kMaxBlocks, ceil_div(std::max(p.n, p.v), step)));
-            ce_max_kernel<E, VEC><<<dim3(static_cast<uint32_t>(blocks), 3), 256, 0, st>>>(a);
+            ce_max_kernel<E, VEC><<<dim3(static_cast<uint32_t>(blocks), 2), 256, 0, st>>>(a);
             RS_HIP(hipGetLastError());
         }
         ce_pack_kernel<E, NP, VEC><<<static_cast<uint32_t>(std::min<int64_t>(ceil_div(p.n_pad + p.v_pad, step), 8192)), 256, 0, st>>>(a, blocks);

@@ -1,0 +1,93 @@
+"""Softmax cross entropy over the catalogue, row by row: every row of the gradients is held to its own terms, however
+improbable the item, small the weight or large the table's elements.
+
+Tolerances.  The names are test_softmax_ce.py's: a logit is off by e_l, a probability by 2 e_l and 4 u32 of itself, a
+coefficient c besides by its rounding U_C and by FLOOR of the largest coefficient of its own sum: a sum holds its
+coefficients times a power of two that keeps the largest so far at 2^8 (dW; 2^7: dH) or more, and fp16 rounds to steps
+of 2^-24, half of one at most.  A probability below 2^-126 counts as zero.  An element of an fp32 table is held as a
+pair: off by 2^-23 of itself (the step of the second piece, half of it), or by 2^-38 of the largest one.  The sums
+take a rounding (u32 of their magnitudes) for each term, outputs half a step of their type, subnormal ones two steps.
+"""
+import math
+
+import pytest
+
+import rsgpu  # noqa: F401  (the library is built)
+
+torch = pytest.importorskip("torch")
+
+from test_softmax_ce import T, U32, U_C, half_step, make, reference  # noqa: E402
+
+FLOOR = {"dH": 2.0 ** -32, "dW": 2.0 ** -33}
+
+
+def check_rows(out, ref, ty, k):
+    e_l = (k + 10) * U32 * (ref["L"] + 1)
+    loss, lse = out[0].double().cpu(), out[1].double().cpu()
+    assert ((loss - ref["loss"]).abs() <= 2 * e_l + 4 * U32 * ref["loss"].abs()).all()
+    assert ((lse - ref["lse"]).abs() <= 2 * e_l + 4 * U32 * ref["lse"].abs()).all()
+    n, v = ref["c"].shape
+    c, g, p, Hm, Wm = ref["c"].abs(), ref["g"].abs(), ref["p"], ref["Hm"].abs(), ref["Wm"].abs()
+    ec = g[:, None] * (2 * e_l[:, None] + 4 * U32) * p + U_C[ty] * c + g[:, None] * 2.0 ** -126
+    lost = 2.0 ** -38 if ty == "f32" else 0.0
+    size_H, size_W = c @ Wm, c.T @ Hm
+    # the target's share of dH is the sum of the others' in fp32, not a difference (a target that takes all): its error is theirs
+    eh = ec + FLOOR["dH"] * c.amax(1, keepdim=True)
+    ew = ec + FLOOR["dW"] * c.amax(0, keepdim=True)
+    bound = {"dH": eh @ Wm + (v + 12) * U32 * size_H + lost * Wm.max() * c.sum(1)[:, None],
+             "dW": ew.T @ Hm + (n + 12) * U32 * size_W + lost * Hm.max() * c.sum(0)[:, None],
+             "db": ec.sum(0) + (n + 4) * U32 * c.sum(0)}
+    for name, x in (("dH", out[2]), ("dW", out[3]), ("db", out[4])):
+        r, b, ut = ref[name], bound[name], half_step(x.dtype)
+        tiny = 2 * torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+        err = (x.double().cpu() - r).abs()
+        lim = b * (1 + ut) + ut * r.abs() + tiny
+        assert (err <= lim).all(), (name, float((err / lim).max()), int((err > lim).sum()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,v,k", [(128, 20000, 8), (128, 20000, 64), (1500, 900, 20), (20000, 60, 9), (65, 700, 200), (40, 300, 300)])
+def test_improbable_items(ctx, n, v, k, ty):
+    """Logits that spread over tens: most items of a row have probabilities of 1e-9 and less."""
+    H, W, target, _, w = make(n, v, k, ty, seed=n + v, spread=10.0)
+    check_rows(ctx.softmax_ce(H, W, target, weight=w, grad=True), reference(H, W, target, None, w), ty, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(70, 800), (3000, 300)])
+def test_items_that_nobody_takes(ctx, ty, n, v):
+    """Biases down to -75: probabilities of 1e-33, and a row of dW that is made of them alone."""
+    k = 24
+    H, W, target, _, w = make(n, v, k, ty, seed=n, spread=1.0)
+    b = torch.linspace(0.0, -75.0, v, device="cuda")
+    target %= v // 8
+    out = ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True)
+    check_rows(out, reference(H, W, target, b, w), ty, k)
+    assert (out[3].float().abs().amax(1) > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("n,v", [(70, 3000), (3000, 300)])
+def test_weights_far_apart(ctx, ty, n, v):
+    """Weights over thirty powers of ten, ascending, descending and mixed along the batch."""
+    k = 20
+    H, W, target, b, _ = make(n, v, k, ty, seed=n, bias=True)
+    w = torch.logspace(-25, 5, n, device="cuda")
+    target[:] = torch.arange(n, device="cuda") % v  # an item has few rows of its own
+    for order in (w, w.flip(0), w[torch.randperm(n, generator=torch.Generator().manual_seed(1))]):
+        check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=order, grad=True), reference(H, W, target, b, order), ty, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+def test_one_item_takes_nearly_all(ctx, ty):
+    """An item far above all others, which is nobody's target: the others' probabilities are 2^-30 and less."""
+    n, v, k = 60, 5000, 16
+    H, W, target, _, w = make(n, v, k, ty, seed=2, spread=1.0)
+    b = torch.zeros(v, device="cuda")
+    b[v // 2] = 24.0
+    target[target == v // 2] = 0
+    check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), ty, k)
