@@ -45,9 +45,10 @@ extern "C" {
  *   Every item withdrawn: lse -inf, loss 0, no gradient.  target withdrawn, others not: lse as defined, loss +inf,
  *     no gradient from that row.
  *   Finite biases are held to +-2^120: the type's lowest value is no withdrawal.
- * The products run on fp16, each matrix scaled by a power of two from its largest finite element: RS_TYPE_F32 as pairs
- * (hi + lo), so an element keeps 2^-24 of itself or 2^-38 of the matrix's largest element, whichever is more;
- * RS_TYPE_BF16 exactly down to 2^-27 of the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Coefficients c_nv
+ * The products run on fp16, each matrix scaled by a power of two from its largest finite element, which may be of any
+ * size: RS_TYPE_F32 as pairs (hi + lo), so an element is off by at most 2^-23 of itself or 2^-38 of the matrix's largest
+ * element, whichever is more, and the product lo lo (2^-22 at most) is left out; RS_TYPE_BF16 exactly down to 2^-27 of
+ * the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Logits beyond fp32's range have no defined outputs.  Coefficients c_nv
  * are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise, or to 2^-32 (dH) and 2^-33 (dW) of the largest
  * so far in the same sum, whichever is more: each row of dW keeps its precision however improbable its item and small the
  * weights.  A probability below 2^-126 counts as zero.  The target's coefficient is minus the sum of the row's others:

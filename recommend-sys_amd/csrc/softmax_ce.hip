@@ -20,8 +20,9 @@
 // where bf16 MFMAs would round them to 8 (dW's error then was 1.5 times that of its own rounding).  fp16's gradients keep
 // 11 bits themselves, so its coefficients are two pieces (450 us on 8192 x 26744 x 128; one piece takes 354 and leaves up
 // to 2 times the error of dW's own rounding where it sums a few rows).  fp32 is split into two pieces hi + lo (each
-// rounds its rest: 2^-24 of the element is left); the product of two such is hi hi + hi lo + lo hi, three fp16 MFMAs
-// (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.
+// rounds its rest: at most 2^-23 of the element is left); the product of two such is hi hi + hi lo + lo hi, three fp16
+// MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.  lo lo, at most 2^-22 of the product and of either sign, is
+// left out: over a row's sum it is below what the fp32 sums round.
 //
 // With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 36 cycles of exponential,
 // sums and packing for each of a lane's 16 logits (KP = 128).  1024 x 1e6 x 256 bf16 2.5 ms: passes 1.09 and 1.19 ms (0.96
@@ -73,11 +74,11 @@ constexpr Shape shape_for(int np, int kp, int mode) {
     return {4, 2, 2};
 }
 
-// Device scalars (ws): the powers of two that scale H and W, and what undoes them.
+// Device scalars (ws): the powers of two that scale H and W.  They and their inverses may be no fp32 numbers (a largest
+// element of 2^-140, or of 2^127 in both): only exponents are kept, and undone by ldexp.
 struct Scal {
-    float hs, wsc;  // H, W are multiplied by these
-    float logit;    // S -> base-2 logit: log2(e) / (hs wsc)
-    float inv_w, inv_h;
+    int eh, ew;   // H, W are multiplied by 2^eh, 2^ew
+    float logit;  // S -> base-2 logit: log2(e) 2^-(eh + ew)
 };
 
 struct CePlan {
@@ -191,14 +192,14 @@ __device__ __forceinline__ void load8(const E* row, int c, int k, float (&v)[8])
     }
 }
 
-// 2^e with max * 2^e in [2^13, 2^14), e bounded so that the power and its inverse are normal numbers
-__device__ __forceinline__ float scale_for(uint32_t max_bits) {
-    if (max_bits == 0) return 1.f;
-    const int e = 13 + 127 - static_cast<int>(max_bits >> 23);
-    return __uint_as_float(static_cast<uint32_t>(min(max(e, -100), 100) + 127) << 23);
+// e with max * 2^e in [2^13, 2^14): -114 to 162
+__device__ __forceinline__ int scale_for(uint32_t max_bits) {
+    return max_bits ? 14 - __builtin_amdgcn_frexp_expf(__uint_as_float(max_bits)) : 0;
 }
 
-__device__ __forceinline__ Scal scales(float hs, float wsc) { return {hs, wsc, kLog2e / hs / wsc, 1.f / wsc, 1.f / hs}; }
+// Past 2^126 the logits leave fp32 with their factor (S is a multiple of 2^-48: 2^78 at least, or 0); below 2^-126 they
+// vanish beside any bias (S is below 2^37), but the factor stays above 0: a target left out is -inf times it.
+__device__ __forceinline__ Scal scales(int eh, int ew) { return {eh, ew, __builtin_amdgcn_ldexpf(kLog2e, max(min(-(eh + ew), 126), -126))}; }
 
 // 2^e with x 2^e in [2^kCoefAt, 2^(kCoefAt + 1)), for x > 0 (as far as the power and its inverse are normal numbers)
 __device__ __forceinline__ float coef_scale(float x) {
@@ -252,8 +253,8 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         if ((threadIdx.x & 63) == 0) sm[which] = m;
     }
     __syncthreads();
-    const float hs = kScaled ? scale_for(sm[0]) : 1.f, wsc = kScaled ? scale_for(sm[1]) : 1.f;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.at<Scal>(p.o_scal) = scales(hs, wsc);
+    const int eh = kScaled ? scale_for(sm[0]) : 0, ew = kScaled ? scale_for(sm[1]) : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.at<Scal>(p.o_scal) = scales(eh, ew);
     const int lanes = p.kp / 8, at = threadIdx.x / lanes, c0 = threadIdx.x % lanes * 8, step = 256 / lanes;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * step + at; row < p.n_pad + p.v_pad; row += static_cast<int64_t>(gridDim.x) * step) {
         const bool w = row >= p.n_pad;
@@ -266,11 +267,11 @@ __global__ __launch_bounds__(256) void ce_pack_kernel(CeArgs a, int max_blocks) 
         }
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (there) load8<E, VEC>(static_cast<const E*>(w ? a.W : a.H) + r * (w ? a.ldw : a.ldh), c0, p.k, v);
-        const float sc = w ? wsc : hs;
+        const int sc = w ? ew : eh;
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float y = v[e] * sc;  // (a power of two: exact)
+            const float y = __builtin_amdgcn_ldexpf(v[e], sc);
             hi[e] = static_cast<_Float16>(y);
             if (NP == 2) lo[e] = static_cast<_Float16>(y - static_cast<float>(hi[e]));
         }
@@ -533,8 +534,9 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     }
 
     const float total = sum + __shfl_xor(sum, 32);
-    // a split's sums, times `back`: four columns of row x at a time
-    auto partial = [&](int64_t rows, float back) {
+    const int back = 127 - static_cast<int>(__float_as_uint(coef) >> 23) - sc.eh;  // (items)
+    // a split's sums, times 2^back: four columns of row x at a time
+    auto partial = [&](int64_t rows, int back) {
         float* O = a.at<float>(p.o_part) + (split * rows + x) * KP + oc0;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -542,7 +544,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             for (int q = 0; q < 4; ++q) {
                 f32x4 o;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = acc[nb][4 * q + e] * back;
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_amdgcn_ldexpf(acc[nb][4 * q + e], back);
                 *reinterpret_cast<f32x4*>(O + nb * 32 + 8 * q + 4 * half) = o;
             }
     };
@@ -551,13 +553,12 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             a.at<float>(p.o_m)[split * p.n_pad + x] = m_run;
             a.at<float>(p.o_s)[split * p.n_pad + x] = total;
         }
-        if constexpr (MODE == kLossGrad) partial(p.n_pad, 1.f);
+        if constexpr (MODE == kLossGrad) partial(p.n_pad, 0);
     } else if (p.splits_w > 1) {
         if (blockIdx.z == 0 && half == 0) a.at<float>(p.o_db)[split * p.v_pad + x] = total;
-        partial(p.v_pad, sc.inv_h / coef);
+        partial(p.v_pad, back);
     } else {
         if (x < p.v && blockIdx.z == 0 && half == 0) a.dbias[x] = total;
-        const float back = sc.inv_h / coef;
         // dW through LDS, so that a row's stores are contiguous: OW columns at a time, 16-byte chunk c of row r at
         // chunk c ^ (r mod the row's chunks)
         constexpr int OW = OC < 128 / static_cast<int>(sizeof(E)) ? OC : 128 / static_cast<int>(sizeof(E));
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
             for (int q = 0; q < OW / 8; ++q) {
                 e4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(acc[(w0 + 8 * q) / 32][4 * (q % 4) + e] * back);
+                for (int e = 0; e < 4; ++e) v[e] = static_cast<E>(__builtin_amdgcn_ldexpf(acc[(w0 + 8 * q) / 32][4 * (q % 4) + e], back));
                 const int byte = (8 * q + 4 * half) * static_cast<int>(sizeof(E));
                 *reinterpret_cast<words*>(mine + lx * kRow + (((byte >> 4) ^ (lx & (CH - 1))) << 4) + (byte & 15)) = __builtin_bit_cast(words, v);
             }
@@ -739,7 +740,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a
     }
     if (n >= p.n) return;
     E* out = static_cast<E*>(a.dH) + n * a.lddh;
-    const float inv = sc.inv_w / s, share_rest = rest / s;
+    // weight (O / s - W_target rest / s), in W's scale; the weight's exponent goes with the scale's at the end, so that no
+    // step before the last leaves fp32
+    const float inv = 1.f / s, share_rest = rest / s, w_frac = __builtin_amdgcn_frexp_mantf(w);
+    const int back = __builtin_amdgcn_frexp_expf(w) - sc.ew;
     // four columns a lane; where a row has fewer than 256, groups of lanes share the splits
     const int quads = p.kp / 4, lanes = quads < 64 ? quads : 64, groups = 64 / lanes, grp = lane / lanes;
     const float* O = a.at<float>(p.o_part) + n * p.kp;
@@ -782,7 +786,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a
         if (grp == 0 && (W == 1 || wave == 0))
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (c + e < p.k) out[c + e] = static_cast<E>(live ? w * (o[e] * inv - share_rest * static_cast<float>(wt[c + e])) : 0.f);
+                if (c + e < p.k) {
+                    const float t = __builtin_amdgcn_ldexpf(static_cast<float>(wt[c + e]), sc.ew);
+                    out[c + e] = static_cast<E>(live ? __builtin_amdgcn_ldexpf(w_frac * (o[e] * inv - share_rest * t), back) : 0.f);
+                }
     }
 }
 

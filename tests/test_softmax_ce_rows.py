@@ -91,3 +91,33 @@ def test_one_item_takes_nearly_all(ctx, ty):
     b[v // 2] = 24.0
     target[target == v // 2] = 0
     check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), ty, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("eh,ew", [(117, -117), (-117, 117), (124, -124), (-124, 122), (90, -90), (-140, 124), (60, -100), (-100, -100)])
+def test_elements_of_any_size(ctx, ty, eh, ew):
+    """Finite elements up to the type's largest and down to its subnormal ones, the logits between them of ordinary size or
+    none."""
+    n, v, k = 70, 500, 40
+    H, W, target, b, w = make(n, v, k, ty, seed=3, spread=1.0, bias=True)
+    H, W = (H.double() * 2.0 ** eh).to(T[ty]), (W.double() * 2.0 ** ew).to(T[ty])
+    assert torch.isfinite(H).all() and torch.isfinite(W).all()
+    ref = reference(H, W, target, b, w)
+    check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), ref, ty, k)
+    e_l = (k + 10) * U32 * (ref["L"] + 1)
+    for rows in (70, 3):  # the loss alone, and its path for a few rows
+        loss, _ = ctx.softmax_ce(H[:rows], W, target[:rows], bias=b)
+        assert ((loss.double().cpu() - ref["loss"][:rows]).abs() <= (2 * e_l + 4 * U32 * ref["loss"])[:rows]).all()
+
+
+@pytest.mark.gpu
+def test_zeros_between_the_largest_elements(ctx):
+    """Both tables at the type's largest, in columns where the other one is zero: logits of exactly the biases."""
+    n, v, k = 40, 90, 32
+    H, W, target, b, w = make(n, v, k, "f32", seed=4, bias=True)
+    H[:, ::2], W[:, 1::2] = 0.0, 0.0
+    H[:, 1::2] *= 2.0 ** 120
+    W[:, ::2] *= 2.0 ** 120
+    w = w * 2.0 ** -30
+    check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), "f32", k)
