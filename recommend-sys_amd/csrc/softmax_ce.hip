@@ -533,7 +533,13 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
         __syncthreads();
     }
 
-    const float total = sum + __shfl_xor(sum, 32);
+    float total = sum + __shfl_xor(sum, 32);
+    // a withdrawn item's coefficients are exp2(-inf), NaN beside a row that is not finite: it takes no part
+    if (items && bias_x == -INFINITY) {
+        total = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x16{0};
+    }
     const int back = 127 - static_cast<int>(__float_as_uint(coef) >> 23) - sc.eh;  // (items)
     // a split's sums, times 2^back: four columns of row x at a time
     auto partial = [&](int64_t rows, int back) {

@@ -121,3 +121,21 @@ def test_zeros_between_the_largest_elements(ctx):
     W[:, ::2] *= 2.0 ** 120
     w = w * 2.0 ** -30
     check_rows(ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True), reference(H, W, target, b, w), "f32", k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,v", [(50, 400), (5000, 130)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_withdrawn_items_beside_rows_that_are_not_finite(ctx, ty, n, v, bad):
+    """A known row that holds a NaN or an infinity reaches the items that are there, and the rows of dW and dbias of no
+    withdrawn one: those are zero."""
+    H, W, target, b, w = make(n, v, 24, ty, seed=5, bias=True, gone=0.3)
+    gone = b == -math.inf
+    target = torch.where(gone[target.long()], torch.zeros_like(target), target)
+    H[7, 3] = bad
+    loss, lse, dH, dW, db = ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True)
+    assert (dW[gone] == 0).all() and (db[gone] == 0).all()
+    assert torch.isnan(loss[7]) and torch.isnan(dW[~gone].float()).any(1).all()
+    rest = [i for i in range(n) if i != 7]
+    assert torch.isfinite(loss[rest]).all() and torch.isfinite(dH[rest].float()).all()
