@@ -104,8 +104,9 @@ int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, cons
  *     times: its gradients are added in batch order)
  *   b_i -= lr g_bi
  *   Q   -= q_lr (O + reg Q), O = rs_orthogonalize(g_Q) with 5 steps of (3.4445, -4.7750, 2.0315)
- * *loss (may be NULL): the mean loss before the step; NaN, and nothing changed, where no interaction is known.  The
- * call waits for the step.  Needs scratch on the device, kept with the plan: about 3 n_items x n_factors floats
+ * *loss (may be NULL): the mean loss before the step; NaN, and nothing changed, where no interaction is known.  A step
+ * that would make a finite factor or bias infinite or NaN (a logit that is not finite does) changes nothing either:
+ * RS_ERR_NUMERIC, *loss NaN.  The call waits for the step.  Needs scratch on the device, kept with the plan: about 3 n_items x n_factors floats
  * and the batch.  A plan joined to a group is refused (RS_ERR_UNSUPPORTED): its factors are replicas.  n <= 2^20. */
 int rs_svd_plan_rank_step(rs_svd_plan* plan, int64_t n, const int32_t* users, const int32_t* items, double lr, double q_lr,
                           double reg, double* loss);

@@ -39,32 +39,44 @@ __global__ __launch_bounds__(256) void rank_row_bias_kernel(const float* __restr
     out[r] = static_cast<float>(gb[0] + (known ? static_cast<double>(P[static_cast<int64_t>(u) * ld + k]) : 0.0));
 }
 
+// A value's step.  APPLY: it is written, unless the step was found to make some finite value no number; otherwise that is
+// found out (*bad), and nothing written.
+template <bool APPLY>
+__device__ __forceinline__ void take_step(float* at, float next, int32_t* bad) {
+    if (APPLY)
+        *at = next;
+    else if (!(fabsf(next) < INFINITY) && fabsf(*at) < INFINITY)
+        *bad = 1;
+}
+
 // one user of the batch a wave: its rows of dH in batch order, then its step
+template <bool APPLY>
 __global__ __launch_bounds__(256) void rank_users_kernel(float* __restrict__ P, int32_t ld, int32_t k, const int32_t* __restrict__ seg,
                                                         const int32_t* __restrict__ seg_user, const int32_t* __restrict__ rows, int64_t n_seg,
-                                                        const float* __restrict__ dH, float lr, float decay) {
+                                                        const float* __restrict__ dH, float lr, float decay, int32_t* bad) {
     const int lane = threadIdx.x & 63;
     const int64_t s = wide_block() * 4 + (threadIdx.x >> 6);
-    if (s >= n_seg) return;
+    if (s >= n_seg || (APPLY && *bad)) return;
     const int32_t a = seg[s], b = seg[s + 1];
     float* p = P + static_cast<int64_t>(seg_user[s]) * ld;
     const float shrink = decay * static_cast<float>(b - a);
     for (int c = lane; c < k; c += 64) {
         float g = 0.f;
         for (int32_t i = a; i < b; ++i) g += dH[static_cast<int64_t>(rows[i]) * k + c];
-        p[c] -= lr * (g + shrink * p[c]);
+        take_step<APPLY>(p + c, p[c] - lr * (g + shrink * p[c]), bad);
     }
 }
 
 // Q -= q_lr (O + reg Q), b -= lr db
+template <bool APPLY>
 __global__ __launch_bounds__(256) void rank_items_kernel(float* __restrict__ Q, int32_t ld, int32_t k, int64_t n_items, const float* __restrict__ O,
-                                                        const float* __restrict__ db, float lr, float q_lr, float reg) {
+                                                        const float* __restrict__ db, float lr, float q_lr, float reg, int32_t* bad) {
     const int lane = threadIdx.x & 63;
     const int64_t v = wide_block() * 4 + (threadIdx.x >> 6);
-    if (v >= n_items) return;
+    if (v >= n_items || (APPLY && *bad)) return;
     float* q = Q + v * ld;
-    for (int c = lane; c < k; c += 64) q[c] -= q_lr * (O[v * k + c] + reg * q[c]);
-    if (lane == 0) q[k] -= lr * db[v];
+    for (int c = lane; c < k; c += 64) take_step<APPLY>(q + c, q[c] - q_lr * (O[v * k + c] + reg * q[c]), bad);
+    if (lane == 0) take_step<APPLY>(q + k, q[k] - lr * db[v], bad);
 }
 
 // a piece of the plan's workspace at a time
@@ -118,7 +130,7 @@ void rank_step(rs_svd_plan* pl, int64_t n, const int32_t* users, const int32_t* 
     const bool in_place = std::min<int64_t>(V, k) <= 256;
     Carver c;
     const int64_t o_users = c.take(n * 4), o_tgt = c.take(n * 4), o_w = c.take(n * 4), o_rows = c.take(m * 4), o_seg = c.take((n_seg + 1) * 4),
-                  o_su = c.take(n_seg * 4), o_loss = c.take(n * 4), o_lse = c.take(n * 4), o_h = c.take(n * k * 4), o_dh = c.take(n * k * 4),
+                  o_su = c.take(n_seg * 4), o_bad = c.take(4), o_loss = c.take(n * 4), o_lse = c.take(n * 4), o_h = c.take(n * k * 4), o_dh = c.take(n * k * 4),
                   o_bias = c.take(V * 4), o_db = c.take(V * 4), o_dw = c.take(V * k * 4), o_x = in_place ? o_dw : c.take(V * k * 4),
                   o_ws = c.take(std::max(ce_bytes, or_bytes));
     plan_sync_last(pl);
@@ -140,14 +152,26 @@ void rank_step(rs_svd_plan* pl, int64_t n, const int32_t* users, const int32_t* 
     check(pl, rs_softmax_ce(pl->ctx, RS_TYPE_F32, n, V, k, f(o_h), k, pl->Q.p, ld, f(o_bias), i32(o_tgt), f(o_w), f(o_loss), f(o_lse), f(o_dh), k,
                             f(o_dw), k, f(o_db), ws + o_ws, ce_bytes, nullptr));
     check(pl, rs_orthogonalize(pl->ctx, RS_TYPE_F32, V, k, f(o_dw), k, 5, 3.4445, -4.7750, 2.0315, f(o_x), k, ws + o_ws, or_bytes, nullptr));
-    rank_users_kernel<<<wide_grid(ceil_div(n_seg, 4)), 256, 0, s>>>(pl->P.p, ld, k, i32(o_seg), i32(o_su), i32(o_rows), n_seg, f(o_dh), lr,
-                                                                               reg / static_cast<float>(m));
-    RS_HIP(hipGetLastError());
-    rank_items_kernel<<<wide_grid(ceil_div(V, 4)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_x), f(o_db), lr, q_lr, reg);
-    RS_HIP(hipGetLastError());
-    plan_factors_changed(pl, s);
+    // both tables' steps are looked through before either is written: a step that a logit or the rates throw out of fp32
+    // leaves the plan as it was
+    RS_HIP(hipMemsetAsync(ws + o_bad, 0, 4, s));
+    auto step = [&](auto apply) {
+        constexpr bool APPLY = decltype(apply)::value;
+        rank_users_kernel<APPLY><<<wide_grid(ceil_div(n_seg, 4)), 256, 0, s>>>(pl->P.p, ld, k, i32(o_seg), i32(o_su), i32(o_rows), n_seg, f(o_dh), lr,
+                                                                               reg / static_cast<float>(m), i32(o_bad));
+        RS_HIP(hipGetLastError());
+        rank_items_kernel<APPLY><<<wide_grid(ceil_div(V, 4)), 256, 0, s>>>(pl->Q.p, ld, k, V, f(o_x), f(o_db), lr, q_lr, reg, i32(o_bad));
+        RS_HIP(hipGetLastError());
+    };
+    step(std::false_type{});
+    step(std::true_type{});
     std::vector<float> h(static_cast<size_t>(n));
+    int32_t bad = 0;
     RS_HIP(hipMemcpyAsync(h.data(), f(o_loss), static_cast<size_t>(n) * 4, hipMemcpyDeviceToHost, s));
+    RS_HIP(hipMemcpyAsync(&bad, ws + o_bad, 4, hipMemcpyDeviceToHost, s));
+    RS_HIP(hipStreamSynchronize(s));
+    if (bad) throw NumericError{"the ranking step would leave fp32 (a logit, a gradient or a stepped value that is not finite); the plan is unchanged"};
+    plan_factors_changed(pl, s);
     RS_HIP(hipStreamSynchronize(s));
     double sum = 0.0;
     for (int64_t r = 0; r < n; ++r)

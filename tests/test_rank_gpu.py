@@ -174,3 +174,57 @@ def test_entry_point_refusals():
     L = rsgpu.lib()
     assert L.rs_svd_plan_rank_step(None, 0, None, None, 0.1, 0.1, 0.0, None) == rsgpu.RS_ERR_INVALID
     assert L.rs_svd_plan_score_items(None, 0, None, None) == rsgpu.RS_ERR_INVALID
+
+
+def tables(plan):
+    return [x.copy() if isinstance(x, np.ndarray) else x for x in plan.download()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("why", ["logits", "row", "rate", "item rate", "bias"])
+def test_a_step_out_of_range_changes_nothing(ctx, why):
+    """A logit, a gradient or a stepped value that is not finite: RS_ERR_NUMERIC, and every factor and bias as it was."""
+    plan = make_plan(ctx)
+    users, items = np.arange(40, dtype=np.int32), (np.arange(40) * 2).astype(np.int32)
+    good = tables(plan)
+    P, Q, bu, bi, gb = tables(plan)
+    rates = dict(lr=0.5, q_lr=0.05)
+    if why == "logits":
+        P, Q = P * 1e22, Q * 1e22
+    elif why == "row":
+        P[7, 3] = np.nan
+    elif why == "bias":
+        bi[11] = np.inf
+    elif why == "rate":
+        rates["lr"] = 3e38
+        P, Q = P * 2.0, Q * 50.0
+    else:
+        rates["q_lr"] = 3e38
+        Q[5] = 3e38 * np.sign(Q[5] + 1e-3)
+        P = P * 1e-39
+    plan.upload(*(x.astype(np.float32) for x in (P, Q, bu, bi)), gb)
+    before = tables(plan)
+    with pytest.raises(rsgpu.RsError) as e:
+        plan.rank_step(users, items, reg=0.01, **rates)
+    assert e.value.code == rsgpu.RS_ERR_NUMERIC
+    for a, b in zip(before, tables(plan)):
+        assert np.array_equal(a, b, equal_nan=True)
+    plan.upload(*(x.astype(np.float32) for x in good[:4]), gb)  # and the plan goes on
+    assert np.isfinite(plan.rank_step(users, items))
+    assert all(np.isfinite(x).all() for x in plan.download()[:4])
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_a_withdrawn_item_stays_withdrawn(ctx):
+    """An item bias of -inf withdraws the item; a step leaves it so, and is none that leaves the range."""
+    plan = make_plan(ctx)
+    P, Q, bu, bi, gb = tables(plan)
+    bi[4] = -np.inf
+    plan.upload(*(x.astype(np.float32) for x in (P, Q, bu, bi)), gb)
+    users = np.arange(50, dtype=np.int32)
+    items = np.where(users % 90 == 4, 5, users).astype(np.int32)
+    assert np.isfinite(plan.rank_step(users, items))
+    got = plan.download()
+    assert got[3][4] == -np.inf and np.isfinite(np.delete(got[3], 4)).all() and all(np.isfinite(x).all() for x in got[:2])
+    plan.close()
