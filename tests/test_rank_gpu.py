@@ -228,3 +228,91 @@ def test_a_withdrawn_item_stays_withdrawn(ctx):
     got = plan.download()
     assert got[3][4] == -np.inf and np.isfinite(np.delete(got[3], 4)).all() and all(np.isfinite(x).all() for x in got[:2])
     plan.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_items,k", [(90, 5), (90, 100), (300, 280), (270, 300), (1200, 64)])
+@pytest.mark.parametrize("n", [1, 40, 300])
+def test_step_is_its_operators(ctx, n_items, k, n):
+    """A step is softmax_ce of the gathered rows with weights 1 / m, orthogonalize of its dW and the documented sums in fp32:
+    the same bits as those calls and numpy's fp32 give (each operator has its own tests against 64 bits)."""
+    torch = pytest.importorskip("torch")
+    plan = make_plan(ctx, n_items=n_items, k=k)
+    rng = np.random.default_rng(n + k)
+    users, items = rng.integers(0, 60, n).astype(np.int32), rng.integers(0, n_items, n).astype(np.int32)
+    if n > 1:
+        users[3], items[5], users[7], items[9] = -1, -1, 60, n_items   # unknown
+        users[10:14] = users[10]                                       # one user several times
+    P, Q, bu, bi, gb = plan.download()
+    P, Q, bi = P.astype(np.float32), Q.astype(np.float32), bi.astype(np.float32)
+    ok = (users >= 0) & (users < 60) & (items >= 0) & (items < n_items)
+    m = int(ok.sum())
+    H = np.where(((users >= 0) & (users < 60))[:, None], P[np.clip(users, 0, 59)], np.float32(0))
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()
+    loss, _, dH, dW, db = ctx.softmax_ce(dev(H), dev(Q), dev(np.where(ok, items, -1).astype(np.int32)), bias=dev(bi),
+                                         weight=torch.full((n,), 1.0 / m, device="cuda"), grad=True)
+    O = ctx.orthogonalize(dW).cpu().numpy()
+    dH, db = dH.cpu().numpy(), db.cpu().numpy()
+    lr, q_lr, reg = np.float32(0.7), np.float32(0.05), np.float32(0.01)
+    P1, Q1 = P.copy(), Q - q_lr * (O + reg * Q)
+    for u in np.unique(users[ok]):
+        rows = np.nonzero(ok & (users == u))[0]
+        g = np.zeros(k, np.float32)
+        for r in rows:
+            g = g + dH[r]
+        P1[u] = P[u] - lr * (g + (reg / np.float32(m) * np.float32(len(rows))) * P[u])
+    got = plan.rank_step(users, items, 0.7, 0.05, 0.01)
+    Pg, Qg, bug, big, gbg = plan.download()
+    assert np.array_equal(Pg.astype(np.float32), P1) and np.array_equal(Qg.astype(np.float32), Q1)
+    assert np.array_equal(big.astype(np.float32), bi - lr * db) and np.array_equal(bu, bug) and gb == gbg
+    assert got == float(loss.cpu().numpy().astype(np.float64)[ok].sum() / m) or abs(got - float(loss.double().sum()) / m) <= n * 2.0 ** -52 * got
+    plan.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_items,k,n", [(90, 100, 40), (90, 100, 1), (300, 280, 60)])
+def test_item_update_against_64_bits(ctx, n_items, k, n):
+    """The whole item update in 64 bits, with factors whose logits are near 0.  The gradient G is off by at most E = rel (|c|^T
+    |H|), rel the coefficients' and the sums' errors; the steps' polynomial of a matrix moves by at most its steepest slope,
+    a^5 = 485 at 0, times what moves G / |G|, 2 |E| / |G| at most; the operator's own error is test_ortho.py's bound, and
+    reading O back from the step costs 8 roundings of Q / q_lr.  All in all below a quarter: an update that is missing is off
+    by 1, one of the wrong sign by 2."""
+    import test_ortho
+    torch = pytest.importorskip("torch")
+    plan = make_plan(ctx, n_items=n_items, k=k)
+    rng = np.random.default_rng(k)
+    small = lambda *s: rng.normal(0, 0.03, s).astype(np.float32)
+    plan.upload(small(60, k), small(n_items, k), small(60), small(n_items), 3.5)
+    users, items = rng.integers(0, 60, n).astype(np.int32), rng.integers(0, n_items, n).astype(np.int32)
+    P, Q, bu, bi, gb = plan.download()
+    lr, q_lr, reg = 0.7, 0.05, 0.01
+    _, _, Q1, _, _, gQ = reference_step(P, Q, bi, users, items, lr, q_lr, reg)
+    plan.rank_step(users, items, lr, q_lr, reg)
+    Qg = plan.download()[1]
+    H = P[users]
+    e = (k + 10) * U32 * ((np.abs(H) @ np.abs(Q).T).max() + np.abs(bi).max() + 1)
+    z = H @ Q.T + bi
+    c = np.exp(z - z.max(1, keepdims=True))
+    c /= c.sum(1, keepdims=True)
+    c[np.arange(n), items] -= 1
+    E = (2 * e + 8 * U32 + (n + 4) * U32) * (np.abs(c).T @ np.abs(H)) / n
+    O, Og = (Q - Q1) / q_lr - reg * Q, (Q - Qg) / q_lr - reg * Q
+    _, own = test_ortho.reference(torch.from_numpy(gQ), gram=0.0)
+    tol = 2 * COEF[0] ** 5 * np.linalg.norm(E) / np.linalg.norm(gQ)
+    tol = tol + float(own.norm()) + 8 * U32 * np.linalg.norm(Q) / q_lr
+    assert tol < 0.25 * np.linalg.norm(O)
+    assert np.linalg.norm(Og - O) <= tol
+    plan.close()
+
+
+@pytest.mark.gpu
+def test_scores_in_several_batches(ctx):
+    """More scores than are held on the device at a time (2^26): a user's row is the same wherever it stands."""
+    plan = make_plan(ctx, k=7)
+    users = np.concatenate([np.arange(-1, 61), np.random.default_rng(1).integers(-1, 61, 2 ** 26 // 90 + 700)]).astype(np.int32)
+    out = plan.score_items(users)
+    one = plan.score_items(np.arange(-1, 61))
+    assert out.shape == (len(users), 90)
+    for a in range(0, len(users), 1 << 17):
+        assert np.array_equal(out[a:a + (1 << 17)], one[users[a:a + (1 << 17)] + 1])
+    plan.close()

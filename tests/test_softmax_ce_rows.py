@@ -139,3 +139,32 @@ def test_withdrawn_items_beside_rows_that_are_not_finite(ctx, ty, n, v, bad):
     assert torch.isnan(loss[7]) and torch.isnan(dW[~gone].float()).any(1).all()
     rest = [i for i in range(n) if i != 7]
     assert torch.isfinite(loss[rest]).all() and torch.isfinite(dH[rest].float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_the_last_rows_of_many(ctx, grad):
+    """More rows than one axis of a launch holds waves for, known ones only here and there: one in 2^20 of the first 2^26 and
+    every third of the 300 behind them, so that each is seen in the sums.  Two items of one factor: bounds as in check_rows,
+    with sums of the known rows' terms alone."""
+    n, ty, k = 2 ** 26 + 300, "bf16", 1
+    h = (torch.randn(n, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) / 4).to(T[ty])
+    W = torch.tensor([[0.5], [-1.25]], device="cuda").to(T[ty])
+    target = torch.full((n,), -1, dtype=torch.int32, device="cuda")
+    known = torch.cat([torch.arange(5, 2 ** 26, 2 ** 20), torch.arange(2 ** 26, n, 3)]).cuda()
+    target[known] = (torch.arange(len(known), device="cuda") % 2).int()
+    w = torch.full((n,), math.nan, device="cuda")
+    w[known] = torch.rand(len(known), device="cuda", generator=torch.Generator("cuda").manual_seed(2)) + 0.5
+    ref = reference(h[known][:, None], W, target[known], None, w[known])
+    if not grad:
+        loss, lse = ctx.softmax_ce(h[:, None], W, target)
+        e_l = (k + 10) * U32 * (ref["L"] + 1)
+        assert ((loss[known].double().cpu() - ref["loss"]).abs() <= 2 * e_l + 4 * U32 * ref["loss"]).all()
+        assert int((loss != 0).sum()) == len(known) and int((lse != 0).sum()) <= len(known)
+        return
+    loss, lse, dH, dW, db = ctx.softmax_ce(h[:, None], W, target, weight=w, grad=True)
+    assert int((dH != 0).sum()) == len(known) and int((loss != 0).sum()) == len(known)
+    check_rows((loss[known], lse[known], dH[known], dW, db), ref, ty, k)
+    # a row less than all of them would be seen
+    least = float((ref["c"].abs() * ref["Hm"].abs())[-100:].amax(1).median())
+    assert least > 4 * float(half_step(T[ty]) * ref["dW"].abs().max())
