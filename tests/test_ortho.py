@@ -262,3 +262,24 @@ def test_entry_point_refusals():
         assert call(**kw) == rsgpu.RS_ERR_INVALID, kw  # (the first: no context)
     assert call(r=600, c=600, ldg=600, ldx=600) == rsgpu.RS_ERR_UNSUPPORTED
     assert call(r=0) == rsgpu.RS_OK
+
+
+LARGE = [("f32", 2049, 20), ("f32", 6041, 100), ("f32", 100, 6041), ("f32", 2500, 300), ("f32", 300, 2500), ("f32", 4099, 512), ("f32", 511, 4100)] + \
+    [(ty, r, c) for ty in ("f32", "bf16", "f16") for r, c in ((40001, 64), (64, 40001), (26745, 128), (20001, 250), (250, 20001), (9001, 500))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty,rows,cols", LARGE)
+def test_large_tables(ctx, ty, rows, cols):
+    """Past the fp64 Gram matrix (2048 long-side rows): up to 79 pieces of it, summed in groups, several tiles for each
+    workgroup of the last pass.  A piece is at most 1024 rows dealt to 8 groups of waves, or 512 or fewer to one or two: the
+    roundings of an entry stay within the 83 of the bound."""
+    G = update(rows, cols, ty, seed=rows + cols)
+    X = ctx.orthogonalize(G)
+    check(X, G)
+    if min(rows, cols) <= 256:  # in place, between columns that stay as they are
+        big = torch.full((rows, cols + 9), 3.0, dtype=G.dtype, device="cuda")
+        big[:, 4:4 + cols] = G
+        ctx.orthogonalize(big[:, 4:4 + cols], out=big[:, 4:4 + cols])
+        assert torch.equal(big[:, 4:4 + cols], X)
+        assert (big[:, :4] == 3.0).all() and (big[:, 4 + cols:] == 3.0).all()
