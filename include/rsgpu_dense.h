@@ -87,9 +87,11 @@ int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, 
  * shorter side at most 256), otherwise they must not overlap.  The shorter side is at most RS_DENSE_MAX_FACTORS,
  * 1 <= steps <= RS_ORTHO_MAX_STEPS.
  * The polynomials are formed on the shorter side's Gram matrix, so the table is read twice and written once.  The Gram
- * matrix is a sum of fp16 products in fp32, joined in fp64 (RS_TYPE_F32: of pairs, so an element keeps 2^-24 of itself
- * or 2^-37 of the largest element near it, whichever is more; fewer bits below 2^-114); the polynomials are fp64.  An
- * infinity or NaN in G makes all of X NaN. */
+ * matrix of RS_TYPE_F32 with at most 2048 long-side rows is fp64; otherwise it is a sum of fp16 products in fp32, joined
+ * in fp64 (RS_TYPE_F32: of pairs, so an element is off by at most 2^-23 of itself or 2^-37 of the largest element near
+ * it, whichever is more; fewer bits below 2^-114); the polynomials are fp64.  The last product takes an fp32 element to
+ * 2^-23 of itself or 2^-49 of |G|, a bf16 or fp16 one to 2^-38 of |G|, its sums are fp32.  An infinity or NaN in G makes
+ * all of X NaN.  ((3.4445, -4.7750, 2.0315) are the published coefficients of the orthogonalised-momentum optimiser.) */
 #define RS_ORTHO_MAX_STEPS 16
 int rs_orthogonalize_workspace(rs_ctx* ctx, int64_t rows, int64_t cols, int64_t* bytes);
 int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, const void* G, int64_t ldg, int32_t steps, double a,

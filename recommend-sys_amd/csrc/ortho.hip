@@ -24,6 +24,7 @@ constexpr int kStage = 8192;      // table elements of one stage of the Gram pas
 constexpr int kJoinGroups = 8;    // groups that many pieces of the Gram matrix are summed in first
 constexpr int kJoinDirect = 24;   // up to so many pieces are joined at once
 constexpr int kPieces64 = 16;     // pieces of the fp64 Gram pass at most
+constexpr float kLowUp = 2048.f;  // the second pieces of G's fp16 pairs are held up by this in the last pass (first pieces: 11 bits)
 
 struct OrthoPlan {
     int64_t r;       // long side
@@ -591,7 +592,10 @@ __global__ __launch_bounds__(64) void ortho_pack_kernel(OrthoPlan p, const doubl
 // ---- X = G T / |G| -------------------------------------------------------------------------------------------------
 // Each wave keeps 32 columns of T in registers (both pieces) for all its rows of G; a tile of G passes through LDS as fp16
 // (fp32: pairs) that all waves read: the table is read once from memory and X written once.  Products: hi T1 + hi T2
-// + lo T1.  SP: short side; KS = SP / 16 steps; WC waves cover the columns of a workgroup (all of them up to 256).
+// + lo T1.  G has one scale, so lo is held kLowUp times its value and meets T1 / kLowUp: fp16 ends at 2^-24, and rows of
+// 2^-15 of |G| and less would lose their second piece there (to 2^-38 of |G|; now 2^-49).  Sums of their own for the
+// small products instead: 200000 x 512 fp32 1.49 ms against 1.29.  SP: short side; KS = SP / 16 steps; WC waves cover the
+// columns of a workgroup (all of them up to 256).
 template <typename E, bool WIDE, bool VEC, int SP, int THREADS>
 __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_t ldg, OrthoPlan p, const _Float16* __restrict__ tp,
                                                              const float* __restrict__ scale, E* X, int64_t ldx) {
@@ -637,7 +641,7 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
             for (int e = 0; e < 4; ++e) {
                 const float x = st[i][e] * gscale;  // (a power of two: exact, fused or not)
                 h[e] = static_cast<_Float16>(x);
-                l[e] = static_cast<_Float16>(x - static_cast<float>(h[e]));
+                l[e] = static_cast<_Float16>((x - static_cast<float>(h[e])) * kLowUp);
             }
             if (WIDE) {
 #pragma unroll
@@ -662,18 +666,20 @@ __global__ __launch_bounds__(THREADS) void ortho_apply_kernel(const E* G, int64_
         E* out = X + (WIDE ? (j0 + 4 * half) * ldx + it * TR + grp * 32 + lx : (it * TR + grp * 32 + 4 * half) * ldx + j0 + lx);
         asm volatile("" : "+v"(rb), "+v"(out));
         f32x16 acc = f32x16{0};
+        // lanes run along the contiguous side of X
+        auto mm = [&](f16x8 u, f16x8 v) {
+            acc = WIDE ? __builtin_amdgcn_mfma_f32_32x32x16_f16(v, u, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(u, v, acc, 0, 0, 0);
+        };
+        int down = 0x1000;  // 1 / kLowUp, unknown to the compiler: it would keep T times it beside T
+        asm volatile("" : "+v"(down));
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             f16x8 g[NP];
 #pragma unroll
             for (int q = 0; q < NP; ++q) g[q] = *reinterpret_cast<const f16x8*>(smem + q * PIECE * 2 + LdsTile<SP>::at(rb, 2 * k));
-            // lanes run along the contiguous side of X
-            auto mm = [&](f16x8 u, f16x8 v) {
-                acc = WIDE ? __builtin_amdgcn_mfma_f32_32x32x16_f16(v, u, acc, 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x16_f16(u, v, acc, 0, 0, 0);
-            };
             mm(g[0], t[0][k]);
             mm(g[0], t[1][k]);
-            if constexpr (NP == 2) mm(g[1], t[0][k]);
+            if constexpr (NP == 2) mm(g[1], t[0][k] * __builtin_bit_cast(_Float16, static_cast<short>(down)));
         }
         if (it + hop < tiles) put(ready, b ^ 1);
 #pragma unroll

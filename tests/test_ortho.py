@@ -283,3 +283,39 @@ def test_large_tables(ctx, ty, rows, cols):
         ctx.orthogonalize(big[:, 4:4 + cols], out=big[:, 4:4 + cols])
         assert torch.equal(big[:, 4:4 + cols], X)
         assert (big[:, :4] == 3.0).all() and (big[:, 4 + cols:] == 3.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(30001, 100), (100, 30001), (20001, 250), (1500, 60)])
+@pytest.mark.parametrize("up", [True, False])
+def test_rows_of_growing_size(ctx, ty, rows, cols, up):
+    """The long side's elements grow (or shrink) by a factor of ten every eighth of it, over eight powers of ten: sums so far
+    follow the scale as it moves.  An fp32 element is off by 2^-23 of itself or 2^-49 of |G|, a bf16 one by 2^-38 of |G|:
+    small rows of X keep their own precision (bf16: what lies above that)."""
+    G = update(rows, cols, "f32", seed=rows, scale=1.0).double().cpu()
+    n = max(rows, cols)
+    f = 10.0 ** (torch.arange(n, dtype=torch.float64) * 8 // n - 4)
+    f = f if up else f.flip(0)
+    G = (G * (f[:, None] if rows >= cols else f)).to(T[ty]).cuda()
+    X = ctx.orthogonalize(G)
+    ref, bound = reference(G)
+    Gd = G.double().cpu()
+    Tm = transform(Gd)
+    floor = (2.0 ** -49 if ty == "f32" else 2.0 ** -38) * (Tm.abs().sum(0) if rows >= cols else Tm.abs().sum(0)[:, None])
+    ut = torch.finfo(X.dtype).eps / 2
+    err = (X.double().cpu() - ref).abs()
+    lim = (bound + floor) * (1 + ut) + (ut + 2 * U32) * ref.abs()
+    assert (err <= lim).all(), (float((err / lim).max()), int((err > lim).sum()))
+
+
+def transform(G, steps=5, coef=COEF):
+    """T of X = G T / |G| (T G / |G| where G is wide), in 64 bits."""
+    G = G / torch.linalg.vector_norm(G)
+    A = G.T @ G if G.shape[0] >= G.shape[1] else G @ G.T
+    a, b, c = coef
+    T_ = torch.eye(len(A), dtype=torch.float64)
+    for _ in range(steps):
+        M = a * torch.eye(len(A), dtype=torch.float64) + b * A + c * A @ A
+        T_, A = T_ @ M, M @ A @ M
+    return T_
