@@ -351,7 +351,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[b] = f32x16{0};
     float m_run = -INFINITY, sum = 0.f;
-    float coef = 1.f, coef_top = 0.f;  // items: a column's coefficients are held times coef, up to coef_top of their own size
+    float coef = 0x1p126f;  // items: what a column's coefficients are held times
     const float bias_x = items ? a.at<float>(p.o_bias)[x] : 0.f;
     const int target_x = !items && x < p.n ? a.target[x] : -1;
 
@@ -360,6 +360,32 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
     const int g4 = lane & 15, row_base = LdsTile<KP>::base(lx, half);
     const int tr_row = 4 * half + (g4 >> 2), tr_chunk = oc0 / 8 + 2 * ((lane >> 4) & 1) + ((g4 & 3) >> 1);
     const int tr_base[2] = {LdsTile<KP>::base(tr_row, tr_chunk) + (g4 & 1) * 8, LdsTile<KP>::base(tr_row + 8, tr_chunk) + (g4 & 1) * 8};
+
+    // The sums times f.  Where a wave has a SIMD for itself they stay in accumulator registers, which only matrix instructions
+    // work on, and are taken out one at a time: left to the compiler, all of them move to other registers for this rare step,
+    // and those to scratch (2048 x 26744 x 512 fp32 1.50 ms against 3.36, 512 bf16 0.62 against 0.68).  The waits stand for the
+    // compiler's, which does not look inside.
+    auto rescale = [&](float f) {
+        if constexpr (OCC == 1) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[nb]));  // (from a product to the read of its result: 19 at most)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float t;
+                    asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\tv_accvgpr_write_b32 %0, %1"
+                                 : "+a"(acc[nb][i]), "=&v"(t)
+                                 : "v"(f));
+                }
+                asm volatile("s_nop 15" : "+a"(acc[nb]));
+            }
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+        }
+    };
 
     // 32 streamed rows from first_y on: the byte offset of their LDS tile and their values
     auto block = [&](int first_y, int tile, const float* mt) {
@@ -423,11 +449,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                     const float f = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m_run - m_new) + (shift_of(m_new) - shift_of(m_run)));
                     m_run = m_new;
                     sum *= f;
-                    if constexpr (MODE == kLossGrad)
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                    if constexpr (MODE == kLossGrad) rescale(f);
                 }
             }
             off = m_run == -INFINITY ? 0.f : m_run - shift_of(m_run);
@@ -467,15 +489,11 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                 float top = 0.f;
 #pragma unroll
                 for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) top = fmaxf(top, fabsf(s[i]));
-                if (__any(top > coef_top)) {  // the first block, and rarely after it
+                if (__any(top * coef > 0x1p15f)) {  // the first block, and rarely after it
                     top = fmaxf(top, __shfl_xor(top, 32));
-                    const float next = top > coef_top ? coef_scale(top) : coef, f = next / coef;
-                    if (top > coef_top) coef_top = 0x1p15f / next;
+                    const float next = top * coef > 0x1p15f ? coef_scale(top) : coef, f = next / coef;
                     coef = next;
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[nb][i] *= f;
+                    rescale(f);
                 }
             } else {
 #pragma unroll
