@@ -168,3 +168,18 @@ def test_the_last_rows_of_many(ctx, grad):
     # a row less than all of them would be seen
     least = float((ref["c"].abs() * ref["Hm"].abs())[-100:].amax(1).median())
     assert least > 4 * float(half_step(T[ty]) * ref["dW"].abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("k", [64, 128, 256, 300, 512])
+def test_sums_whose_scale_keeps_moving(ctx, ty, k):
+    """Logits that ascend along the items by 100 (the users' sums follow a new maximum in every block) and weights that ascend
+    along the rows by ten powers of ten (the items' sums follow a new largest coefficient)."""
+    n, v = 600, 1000
+    H, W, target, _, _ = make(n, v, k, ty, seed=k, spread=1.0)
+    b = torch.linspace(-100.0, 0.0, v, device="cuda")
+    w = torch.logspace(-6, 4, n, device="cuda") if ty != "f16" else torch.logspace(-3, 1, n, device="cuda")
+    target[:] = torch.arange(n, device="cuda") % v
+    out = ctx.softmax_ce(H, W, target, bias=b, weight=w, grad=True)
+    check_rows(out, reference(H, W, target, b, w), ty, k)
