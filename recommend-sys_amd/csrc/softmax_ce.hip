@@ -201,11 +201,8 @@ __device__ __forceinline__ int scale_for(uint32_t max_bits) {
 // vanish beside any bias (S is below 2^37), but the factor stays above 0: a target left out is -inf times it.
 __device__ __forceinline__ Scal scales(int eh, int ew) { return {eh, ew, __builtin_amdgcn_ldexpf(kLog2e, max(min(-(eh + ew), 126), -126))}; }
 
-// 2^e with x 2^e in [2^kCoefAt, 2^(kCoefAt + 1)), for x > 0 (as far as the power and its inverse are normal numbers)
-__device__ __forceinline__ float coef_scale(float x) {
-    const int e = kCoefAt + 127 - static_cast<int>(__float_as_uint(x) >> 23);
-    return __uint_as_float(static_cast<uint32_t>(min(e, 126) + 127) << 23);
-}
+// frexp's exponent of the power of two that takes x to [2^kCoefAt, 2^(kCoefAt + 1))
+__device__ __forceinline__ int coef_exponent(float x) { return min(kCoefAt + 2 - __builtin_amdgcn_frexp_expf(x), 127); }
 
 __device__ __forceinline__ void see_largest(uint32_t& m, float x) {
     const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
@@ -393,7 +390,11 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
         // addresses anew for every block, or the compiler keeps all of them in registers and spills others (KP = 256: 168
         // bytes, 1221 / 2067 us against 1072 / 1215); narrow ones keep them (KP = 128: 126 us against 154)
         int rb = row_base + tile, tb[2] = {tr_base[0] + tile, tr_base[1] + tile};
-        if (KP >= 256) asm volatile("" : "+v"(rb), "+v"(tb[0]), "+v"(tb[1]));
+        if (KP >= 256) {
+            asm volatile("" : "+v"(rb), "+v"(tb[0]));
+            tb[1] = tb[0] ^ 128;  // (the chunks' order eight rows on; the rows themselves are a constant)
+        }
+        constexpr int kEight = KP >= 256 ? 8 * KP * 2 : 0;
         f32x16 s = f32x16{0};
         // A lane's target is not for these sums: its logit becomes -inf.  Asked for between the products where the registers
         // allow it (8192 x 26744 x 128 without gradients: 100 us, 108 in the maximum's branch, 99 if it were left in),
@@ -490,10 +491,11 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
 #pragma unroll
                 for (int i = 4 * Q * h; i < 4 * Q * (h + 1); ++i) top = fmaxf(top, fabsf(s[i]));
                 if (__any(top * coef > 0x1p15f)) {  // the first block, and rarely after it
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const float next = top * coef > 0x1p15f ? coef_scale(top) : coef, f = next / coef;
-                    coef = next;
-                    rescale(f);
+                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                    top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+                    const int down = top * coef > 0x1p15f ? coef_exponent(top) - __builtin_amdgcn_frexp_expf(coef) : 0;
+                    coef = __builtin_amdgcn_ldexpf(coef, down);
+                    rescale(__builtin_amdgcn_ldexpf(1.f, down));
                 }
             } else {
 #pragma unroll
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(WAVES * 64, OCC) void ce_main_kernel(CeArgs a) {
                         for (int q = 0; q < NP; ++q) {
                             auto rd = [&](int k) {
                                 return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                                    smem + q * PIECE * 2 + j * (32 * KP) + LdsTile<KP>::at(tb[k], nb * 4)));
+                                    smem + q * PIECE * 2 + j * (32 * KP) + LdsTile<KP>::at(tb[k], nb * 4) + k * kEight));
                             };
                             const s16x4 u = rd(0), w = rd(1);
                             yt[q] = __builtin_bit_cast(f16x8, __builtin_shufflevector(u, w, 0, 1, 2, 3, 4, 5, 6, 7));
