@@ -48,11 +48,12 @@ extern "C" {
  * The products run on fp16, each matrix scaled by a power of two from its largest finite element, which may be of any
  * size: RS_TYPE_F32 as pairs (hi + lo), so an element is off by at most 2^-23 of itself or 2^-38 of the matrix's largest
  * element, whichever is more, and the product lo lo (2^-22 at most) is left out; RS_TYPE_BF16 exactly down to 2^-27 of
- * the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Logits beyond fp32's range have no defined outputs.  Coefficients c_nv
- * are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise, or to 2^-32 (dH) and 2^-33 (dW) of the largest
- * so far in the same sum, whichever is more: each row of dW keeps its precision however improbable its item and small the
- * weights.  A probability below 2^-126 counts as zero.  The target's coefficient is minus the sum of the row's others:
- * the gradients of a row keep their precision where its target's probability is near one, as does its loss.
+ * the largest, and to 2^-38 of it below; RS_TYPE_F16 as it is.  Logits beyond fp32's range have no defined outputs.
+ * Coefficients c_nv are rounded to 11 bits before they meet a bf16 matrix, to 22 otherwise, or to 2^-32 (dH; 2^-25 where a
+ * row's logits pass 22700) and 2^-33 (dW) of the largest so far in the same sum, whichever is more: each row of dW keeps
+ * its precision however improbable its item and small the weights.  A probability below 2^-126 counts as zero.  The
+ * target's coefficient is minus the sum of the row's others: the gradients of a row keep their precision where its
+ * target's probability is near one, as does its loss.
  * n_rows and n_items from 1 to 2^31 - 1025 (or both 0). */
 int rs_softmax_ce_workspace(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_items, int32_t n_factors, int32_t with_grad,
                             int64_t* bytes);
@@ -72,7 +73,8 @@ int rs_quantize_rows(rs_ctx* ctx, int32_t type, int64_t n_rows, int64_t n_cols, 
 /* int8 product with a scale per row of A (a user, a token) and per row of B (an item, a channel):
  *   C_mn = a_scale_m * b_scale_n * sum_k A_mk B_nk + row_bias_m + col_bias_n
  * A (m x k), B (n x k) int8, any value, any alignment and stride (rows of 16-byte multiples at 16-byte addresses are
- * read fastest); the sums are exact in int32 (k <= RS_I8_MAX_K); the rest is fp32, C of out_type rounded once.
+ * read fastest); the sums are exact in int32 (k <= RS_I8_MAX_K); the rest is fp32, the two scales' product first (where
+ * that is no normal number, C has its precision), C of out_type rounded once.
  * row_bias, col_bias may be NULL.  An entry of col_bias of -inf gives -inf scores (a withdrawn item).  k >= 1. */
 #define RS_I8_MAX_K 65536
 int rs_i8_matmul(rs_ctx* ctx, int64_t m, int64_t n, int64_t k, const int8_t* A, int64_t lda, const float* a_scale,
@@ -108,15 +110,19 @@ int rs_orthogonalize(rs_ctx* ctx, int32_t type, int64_t rows, int64_t cols, cons
  *   Q   -= q_lr (O + reg Q), O = rs_orthogonalize(g_Q) with 5 steps of (3.4445, -4.7750, 2.0315)
  * *loss (may be NULL): the mean loss before the step; NaN, and nothing changed, where no interaction is known.  A step
  * that would make a finite factor or bias infinite or NaN (a logit that is not finite does) changes nothing either:
- * RS_ERR_NUMERIC, *loss NaN.  The call waits for the step.  Needs scratch on the device, kept with the plan: about 3 n_items x n_factors floats
- * and the batch.  A plan joined to a group is refused (RS_ERR_UNSUPPORTED): its factors are replicas.  n <= 2^20. */
+ * RS_ERR_NUMERIC, *loss NaN.  The call waits for the step.  Its scratch on the device stays with the plan, grown
+ * to its largest call: the gradient of the item table (twice where n_items and n_factors both pass 256), what
+ * rs_softmax_ce_workspace asks for fp32 with gradients, and the batch's rows (4096 x 3706 x 100: 41 MB; 1024 x 1e6 x 256:
+ * 2.1 GB).
+ * A plan joined to a group is refused (RS_ERR_UNSUPPORTED): its factors are replicas.  n <= 2^20. */
 int rs_svd_plan_rank_step(rs_svd_plan* plan, int64_t n, const int32_t* users, const int32_t* items, double lr, double q_lr,
                           double reg, double* loss);
 
 /* Scores of n users (inner ids, -1 = unknown) against all items, out[r][i] = GlobalBias + b_u + b_i + p_u . q_i in fp32 (n x
  * n_items, host), the products in 8 bits: p_u and q_i by rs_quantize_rows (their scales s_p, s_q), so a score is off by at
  * most sum_f (s_p |q_f| + s_q |p_f|) / 2 + s_p s_q / 4 and fp32 rounding.  Unknown users: GlobalBias + b_i (svd.go:39-48).
- * The item table is quantised once a call. */
+ * The item table is quantised once a call.  Scratch on the device, kept with the plan as rank_step's: the 8-bit table
+ * and up to 256 MiB of scores. */
 int rs_svd_plan_score_items(rs_svd_plan* plan, int64_t n, const int32_t* users, float* out);
 
 #ifdef __cplusplus

@@ -18,16 +18,17 @@
 // and rows without a known target zeroed (so NaN or garbage in them reaches no product), as fp16 of the matrix scaled by
 // a power of two.  bf16's 8 bits fit fp16's 11: the products are those of bf16, but the coefficients f(S) keep 11 bits
 // where bf16 MFMAs would round them to 8 (dW's error then was 1.5 times that of its own rounding).  fp16's gradients keep
-// 11 bits themselves, so its coefficients are two pieces (450 us on 8192 x 26744 x 128; one piece takes 354 and leaves up
+// 11 bits themselves, so its coefficients are two pieces (405 us on 8192 x 26744 x 128; one piece takes 306 and leaves up
 // to 2 times the error of dW's own rounding where it sums a few rows).  fp32 is split into two pieces hi + lo (each
 // rounds its rest: at most 2^-23 of the element is left); the product of two such is hi hi + hi lo + lo hi, three fp16
 // MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.  lo lo, at most 2^-22 of the product and of either sign, is
 // left out: over a row's sum it is below what the fp32 sums round.
 //
-// With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 36 cycles of exponential,
-// sums and packing for each of a lane's 16 logits (KP = 128).  1024 x 1e6 x 256 bf16 2.5 ms: passes 1.09 and 1.19 ms (0.96
-// and 0.88 PFLOP/s), packing 0.38; 8192 x 26744 x 128 bf16 0.315 ms; 4096 x 3706 x 100 fp32 93 us; 128 x 1682 x 20
-// fp32 28 us, five launches.
+// With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 40 cycles of exponential,
+// sums, maxima and packing for each of a lane's 16 logits (KP = 128: the matrix units are busy 41 and 39 % of the time, the
+// vector ones 51 and 56 %).  1024 x 1e6 x 256 bf16 2.4 ms: passes 1.03 and 1.20 ms (1.02 and 0.87 PFLOP/s), largest
+// elements and packing 0.38; 8192 x 26744 x 128 bf16 0.317 ms; 4096 x 3706 x 100 fp32 92 us; 128 x 1682 x 20 fp32 29 us,
+// five launches.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -39,7 +40,10 @@ namespace {
 
 constexpr int kPad = 256;        // rows are padded to this: a multiple of what a workgroup holds or a stage streams
 constexpr int kTileY = 128;      // streamed rows are split over workgroups in multiples of this
-constexpr int kFewRows = 4;      // rows that the table is read for as it is, without gradients
+// rows that the table is read for as it is, without gradients: 4 / 5 rows (as it is / packed) against 108944 x 320 bf16 52 /
+// 122 us, 1e6 x 256 bf16 216 / 460, 26744 x 100 fp32 16 / 30.  One launch holds four (a lane's registers); packed, 5 to 64
+// rows take the same time
+constexpr int kFewRows = 4;
 constexpr int kFewItems = 128;   // items that a workgroup has on their way then: 8 waves x 4 x 4
 constexpr int kMaxBlocks = 1024;  // blocks of the maxima pass at most, per matrix
 // p = 2^(l2 - m) is held as 2^shift_of(m) p (fp16's range below 1 is short; beside a large m the shift would be lost in
@@ -49,7 +53,7 @@ constexpr float kLag = 8.f;
 // a column's coefficients in the items' pass, weight p / s, are held times a power of two that brings the largest so far
 // to [2^kCoefAt, 2^15]: whatever the item's probabilities and the weights, none is rounded by more than its 11 bits (two
 // pieces: 22) or 2^-25, 2^-33 of the largest (one scale for the batch left nothing of an item that no row thinks likely).
-// Brought to 2^11: 1024 x 1e6 x 256 bf16 2.81 ms, 2.69 with 2^8, where the scale moves less often.
+// Brought to 2^11: the items' pass of 1024 x 1e6 x 256 bf16 1.34 ms, 1.20 with 2^8, where the scale moves less often.
 constexpr int kCoefAt = 8;
 __device__ __forceinline__ float shift_of(float m) { return fabsf(m) < 32768.f ? 7.f : 0.f; }
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -59,10 +63,10 @@ enum Mode { kLoss = 0, kLossGrad = 1, kItems = 2 };
 // Shape of a workgroup: waves of 32 stationary rows each, streamed rows of a stage (between two barriers) in blocks of
 // 32, waves per SIMD asked of the compiler.  Measured on 8192 x 26744 x 128 and 1024 x 1e6 x 256 (bf16), 4096 x 3706 x 100
 // (fp32), times of the two passes (users / items):
-//   KP = 128, one piece: 8 waves 148 / 183 us, 4 waves 162 / 194 and twice the pieces to join; stages of 4 blocks for the
-//     users' pass (of 2: 150), 2 for the items' (4 spill)
-//   KP = 256, one piece: 8 waves 1122 / 1222 us, 4 waves 1478 / 1431 (8 waves read the streamed tile once for 256 rows)
-//   KP = 128, two pieces: 4 waves 35.3 / 34.8 us, 8 waves 34.1 / 34.7
+//   KP = 128, one piece: 8 waves 149 / 186 us, 4 waves 171 / 196 and twice the pieces to join; stages of 4 blocks for the
+//     users' pass (of 2: 150 when they were chosen, 137 now that the target stays out of the sums), 2 for the items' (4 spill)
+//   KP = 256, one piece: 8 waves 1028 / 1200 us, 4 waves 1349 / 1323 (8 waves read the streamed tile once for 256 rows)
+//   KP = 128, two pieces: 4 waves 35.9 / 36.5 us, 8 waves 34.1 / 34.7 (before the items' maxima)
 //   wider: the row and its sums take more than half the registers: one wave per SIMD
 struct Shape {
     int waves, blocks, occ;
@@ -710,7 +714,7 @@ __global__ __launch_bounds__(512) void ce_few_kernel(CeArgs a) {
 
 // ---- joining the splits of the catalogue: lse, loss, dH and what the dW pass reads of each row --------------------
 // W waves per row: one, or where few rows have many splits the eight of a workgroup, which share the splits (27 x 635201
-// x 92 fp32, 1655 splits: 89 us, 355 with one; 1024 x 1e6 x 256, 64 splits: 18 us and 30).
+// x 92 fp32, 709 splits: all of a call 432 us, 534 with one; 1024 x 1e6 x 256 bf16, 64 splits: the join 18 us and 30).
 template <typename E, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void ce_join_kernel(CeArgs a) {
     const CePlan& p = a.p;
