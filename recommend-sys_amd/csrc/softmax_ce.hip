@@ -21,8 +21,8 @@
 // 11 bits themselves, so its coefficients are two pieces (405 us on 8192 x 26744 x 128; one piece takes 306 and leaves up
 // to 2 times the error of dW's own rounding where it sums a few rows).  fp32 is split into two pieces hi + lo (each
 // rounds its rest: at most 2^-23 of the element is left); the product of two such is hi hi + hi lo + lo hi, three fp16
-// MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.  lo lo, at most 2^-22 of the product and of either sign, is
-// left out: over a row's sum it is below what the fp32 sums round.
+// MFMAs (2.5 PF / 3) where an fp32 MFMA would run at 157 TF.  lo lo, at most 2^-22 of the product, of either sign and
+// about 2^-24.6 in the mean square, is left out.
 //
 // With gradients, bound by the instruction mix of the two passes: 16 MFMAs of 32 cycles beside about 40 cycles of exponential,
 // sums, maxima and packing for each of a lane's 16 logits (KP = 128: the matrix units are busy 41 and 39 % of the time, the

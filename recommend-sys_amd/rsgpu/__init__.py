@@ -727,7 +727,8 @@ class SvdPlan:
     def rank_step(self, users, items, lr=1.0, q_lr=0.02, reg=0.0):
         """One training step for ranking on the resident factors (rs_svd_plan_rank_step): softmax cross entropy of the
         interactions (inner ids, -1 = unknown) over the whole catalogue, SGD on the users' rows and the item biases, an
-        orthogonalised update of the item table.  Returns the mean loss before the step (NaN: no known interaction)."""
+        orthogonalised update of the item table.  Returns the mean loss before the step (NaN: no known interaction).
+        A step that would leave fp32 raises RsError (RS_ERR_NUMERIC) and changes nothing."""
         u, i = np.ascontiguousarray(users, np.int32), np.ascontiguousarray(items, np.int32)
         if u.shape != i.shape or u.ndim != 1:
             raise ValueError("users and items must be two lists of the same length")
